@@ -156,6 +156,87 @@ def rms_norm(x: Tensor, w: Tensor | None, eps: float) -> Tensor:
     return _RMSNorm.apply(x, w, eps)
 
 
+def _on_current_device(what: str, *tensors: Tensor | None) -> None:
+    """Kernels launch on the current device's stream: a tensor that lies elsewhere is refused."""
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise nv.NativeError(f"{what}: a tensor on {t.device}: the kernels run on a GPU")
+        if t is not None and t.device.index != torch._C._cuda_getDevice():
+            raise nv.NativeError(f"{what}: a tensor on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+def _dense(t: Tensor) -> Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Tensor:  # type: ignore[override]
+        d = x.shape[-1]
+        x2 = _dense(x.reshape(-1, d))
+        w, b = (None if p is None else _dense(p) for p in (w, b))
+        p_fp32 = any(p is not None and p.dtype == torch.float32 for p in (w, b))
+        rows = x2.shape[0]
+        y = torch.empty_like(x2)
+        stats = torch.empty(2, rows, device=x.device, dtype=torch.float32) if any(ctx.needs_input_grad) else None
+        if rows > 0:
+            lib = _lib()
+            lib.pd_layer_norm_fwd.argtypes = [C.c_void_p] * 6 + [C.c_longlong, C.c_int, C.c_float, C.c_int, C.c_int, C.c_void_p]
+            mean, rstd = (None, None) if stats is None else (stats[0].data_ptr(), stats[1].data_ptr())
+            _check(lib.pd_layer_norm_fwd(x2.data_ptr(), None if w is None else w.data_ptr(),
+                                         None if b is None else b.data_ptr(), y.data_ptr(), mean, rstd, rows, d, eps,
+                                         int(x.dtype == torch.float32), int(p_fp32), _s()), "layer_norm_fwd")
+        ctx.save_for_backward(x2, w, stats)
+        ctx.p_dtype = torch.float32 if p_fp32 else torch.bfloat16
+        return y.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy: Tensor):  # type: ignore[override]
+        x2, w, stats = ctx.saved_tensors
+        rows, d = x2.shape
+        dy2 = _dense(dy.reshape(x2.shape))
+        want_x, want_w, want_b, _ = ctx.needs_input_grad
+        dx = torch.empty_like(x2) if want_x else None
+        new = torch.zeros if rows == 0 else torch.empty
+        dw = new(d, device=x2.device, dtype=ctx.p_dtype) if want_w else None
+        db = new(d, device=x2.device, dtype=ctx.p_dtype) if want_b else None
+        if rows > 0:
+            lib = _lib()
+            partial = None
+            if want_w or want_b:
+                lib.pd_layer_norm_partial_rows.argtypes = [C.c_longlong, C.c_int]
+                partial = torch.empty(lib.pd_layer_norm_partial_rows(rows, d), 2, d, device=x2.device, dtype=torch.float32)
+                nv.count_launch()
+            lib.pd_layer_norm_bwd.argtypes = [C.c_void_p] * 9 + [C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p]
+            ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+            _check(lib.pd_layer_norm_bwd(x2.data_ptr(), ptr(w), dy2.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(),
+                                         ptr(dx), ptr(dw), ptr(db), ptr(partial), rows, d,
+                                         int(x2.dtype == torch.float32), int(ctx.p_dtype == torch.float32), _s()),
+                   "layer_norm_bwd")
+        return None if dx is None else dx.view(dy.shape), dw, db, None
+
+
+LAYER_NORM_MAX_COLUMNS = 12288
+
+
+def layer_norm(x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Tensor:
+    """`(x - mean) / sqrt(var + eps) * w + b` over the last axis, in `x`'s type; differentiable in `x`, `w` and `b`.
+
+    `x [..., d]` bf16 or fp32 with `1 <= d <= 12288`; `w`, `b` `[d]` (or None), bf16 or fp32 and of one type. Statistics and
+    weight gradients are summed in fp32, in an order that depends on the sizes alone; each output is rounded once."""
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"layer_norm: {x.dtype} is not bf16 or fp32")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= LAYER_NORM_MAX_COLUMNS:
+        raise ValueError(f"layer_norm: rows of 1 to {LAYER_NORM_MAX_COLUMNS} columns, not {tuple(x.shape)}")
+    given = [p for p in (w, b) if p is not None]
+    for p in given:
+        if p.shape != x.shape[-1:] or p.dtype not in (torch.bfloat16, torch.float32) or p.dtype != given[0].dtype:
+            raise ValueError(f"layer_norm: scale and shift are [{x.shape[-1]}] in bf16 or fp32 and of one type, "
+                             f"not {[(tuple(q.shape), q.dtype) for q in given]}")
+    _on_current_device("layer_norm", x, w, b)
+    return _LayerNorm.apply(x, w, b, eps)
+
+
 class _Rope(torch.autograd.Function):
     """Rotary embedding on `[B, T, H, hd]` (full head_dim). Out of place; backward = inverse rotation."""
 
