@@ -25,6 +25,8 @@ enum StatusCode : int {
   kTimeoutPeerFlag = 4,
   kBadExpert = 6,  // a job named an expert that does not exist
   kBadArgument = 5,
+  kBadToken = 7,   // a token id outside the embedding table
+  kBadColumn = 8,  // a column index outside the row of logits
 };
 
 // Two seconds in nanoseconds of %globaltimer: long against any tile, short against a watchdog.

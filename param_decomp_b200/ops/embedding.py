@@ -1,0 +1,84 @@
+"""Token embedding with scaling, and the gradient of its table (`csrc/embedding.cu`).
+
+`y[n] = scale * table[tokens[n]]`; the gradient of row `v` is `scale` times the sum of `dy` over the positions that hold
+token `v`, taken in fp32 in ascending order of position (positions sorted by token), so it does not change from run to
+run, and rounded once to the table's type. Every row of the gradient is written: rows of unseen tokens are zero.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+from torch import Tensor
+
+from param_decomp_b200.ops import native as nv
+from param_decomp_b200.ops.elementwise import _check, _dense, _on_current_device, _s
+
+_FLOAT = (torch.bfloat16, torch.float32)
+
+
+def _lib():
+    lib = nv.lib()
+    P, LL, I, F = C.c_void_p, C.c_longlong, C.c_int, C.c_float
+    lib.pd_embedding.argtypes = [P, I, P, P, LL, LL, I, F, I, I, P, P, P]
+    lib.pd_embedding_grad.argtypes = [P, I, P, P, LL, LL, I, F, I, I, P, P, P]
+    lib.pd_embedding_grad_ints.argtypes, lib.pd_embedding_grad_ints.restype = [LL], LL
+    lib.pd_embedding_grad_floats.argtypes, lib.pd_embedding_grad_floats.restype = [LL, I], LL
+    return lib
+
+
+def _grad(tokens: Tensor, dy: Tensor, rows: int, scale: float, dtype: torch.dtype) -> Tensor:
+    n, d = dy.shape
+    lib = _lib()
+    dE = torch.empty(rows, d, device=dy.device, dtype=dtype)
+    ints = torch.empty(lib.pd_embedding_grad_ints(n), device=dy.device, dtype=torch.int32)
+    partial = torch.empty(lib.pd_embedding_grad_floats(n, d), device=dy.device, dtype=torch.float32)
+    _check(lib.pd_embedding_grad(tokens.data_ptr(), int(tokens.dtype == torch.int64), dy.data_ptr(), dE.data_ptr(), n, rows,
+                                 d, scale, int(dy.dtype == torch.float32), int(dtype == torch.float32), ints.data_ptr(),
+                                 partial.data_ptr(), _s()), "embedding_grad")
+    nv.count_launch()
+    return dE
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table: Tensor, tokens: Tensor, scale: float, out_dtype: torch.dtype) -> Tensor:  # type: ignore[override]
+        table = _dense(table)
+        flat = _dense(tokens.reshape(-1))
+        rows, d = table.shape
+        y = torch.empty(flat.numel(), d, device=table.device, dtype=out_dtype)
+        if flat.numel() > 0:
+            _check(_lib().pd_embedding(flat.data_ptr(), int(flat.dtype == torch.int64), table.data_ptr(), y.data_ptr(),
+                                       flat.numel(), rows, d, scale, int(table.dtype == torch.float32),
+                                       int(out_dtype == torch.float32), nv.status_word().data_ptr(), nv.refused_ptr(),
+                                       _s()), "embedding")
+        ctx.save_for_backward(flat)
+        ctx.cfg = (rows, scale, table.dtype)
+        return y.view(*tokens.shape, d)
+
+    @staticmethod
+    def backward(ctx, dy: Tensor):  # type: ignore[override]
+        (flat,) = ctx.saved_tensors
+        rows, scale, dtype = ctx.cfg
+        return _grad(flat, _dense(dy.reshape(flat.numel(), dy.shape[-1])), rows, scale, dtype), None, None, None
+
+
+def embedding(tokens: Tensor, table: Tensor, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> Tensor:
+    """`scale * table[tokens]`: `tokens [...]` int32 or int64 in `[0, rows)`, `table [rows, d]` bf16 or fp32, the result
+    `[..., d]` in `out_dtype` (the table's type by default); differentiable in `table`.
+
+    A token outside the table is refused: its row is zero and takes no part in the gradient, `native.raise_refused` (made
+    by the next call) raises, `native.check_status` raises at once."""
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"embedding: token ids are int32 or int64, not {tokens.dtype}")
+    if table.dim() != 2 or table.dtype not in _FLOAT or 0 in table.shape:
+        raise ValueError(f"embedding: the table is [rows, d] in bf16 or fp32, not {tuple(table.shape)} {table.dtype}")
+    out_dtype = table.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _FLOAT:
+        raise ValueError(f"embedding: the result is bf16 or fp32, not {out_dtype}")
+    if tokens.numel() >= 1 << 30 or table.shape[0] >= 1 << 31:
+        raise ValueError(f"embedding: fewer than 2^30 tokens and 2^31 rows, not {tokens.numel()} and {table.shape[0]}")
+    _on_current_device("embedding", tokens, table)
+    nv.raise_refused()
+    return _Embedding.apply(table, tokens, float(scale), out_dtype)

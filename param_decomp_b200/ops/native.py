@@ -139,8 +139,10 @@ def raise_refused() -> None:
 
 def status_message(code: int) -> str:
     """What a status code says (`pd::StatusCode`)."""
-    if code == 6:
-        return "a routed job named an expert outside the bank (status code 6)"
+    refusals = {6: "a routed job named an expert outside the bank", 7: "a token id lies outside the embedding table",
+                8: "a column index lies outside the row of logits"}
+    if code in refusals:
+        return f"{refusals[code]} (status code {code})"
     return f"a device-side wait timed out (status code {code})"
 
 
