@@ -1,0 +1,210 @@
+"""The top logits of a teacher, and the distillation loss that reads them (`csrc/top_logits.cu`, `csrc/top_kl.cu`).
+
+A teacher's row of `V` logits is kept as its `k` largest (`top_logits`), their columns and `tail`, the logarithm of the
+sum of exponentials of all others: a distribution over `k + 1` events. `top_kl` is the divergence from it to the student's
+softmax, grouped into the same events. At `k = V - 1` and at `k = V` it is the divergence over the whole vocabulary that
+`vocab_kl` computes, below that never more; it reads one row of logits a position instead of two.
+
+With one slot and no tail, `top_kl` is the cross entropy of a target: `next_token_loss`.
+
+The `eager_*` functions are the same definitions in plain torch, for any device.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+from torch import Tensor
+
+from param_decomp_b200.ops import native as nv
+from param_decomp_b200.ops.elementwise import _check, _dense, _on_current_device, _s
+
+MAX_K = 256
+_FLOAT = (torch.bfloat16, torch.float32)
+
+
+class TopLogits(NamedTuple):
+    values: Tensor  # [..., k] the k largest logits, descending, in the logits' type
+    indices: Tensor  # [..., k] int32 columns; equal logits in the order of their columns
+    tail: Tensor  # [...] fp32 logsumexp of all other logits over the temperature (-inf where k is the whole row)
+
+
+def _lib():
+    lib = nv.lib()
+    P, LL, I, F, D = C.c_void_p, C.c_longlong, C.c_int, C.c_float, C.c_double
+    lib.pd_top_logits.argtypes = [P, LL, I, LL, I, F, P, P, P, I, P]
+    lib.pd_top_kl.argtypes = [P, LL, I, LL, P, I, P, I, I, P, D, P, P, LL, P, I, P, P, P]
+    lib.pd_top_kl_max_columns.argtypes, lib.pd_top_kl_max_columns.restype = [I], LL
+    return lib
+
+
+def _rows_of(logits: Tensor) -> Tensor:
+    """`[rows, V]` view with neighbouring columns and rows that do not overlap (a copy where there is none)."""
+    z = logits.reshape(-1, logits.shape[-1])
+    V = z.shape[1]
+    if (V > 1 and z.stride(1) != 1) or (z.shape[0] > 1 and z.stride(0) < V):
+        z = z.contiguous()
+    return z
+
+
+def _pitch(z: Tensor) -> int:
+    return z.stride(0) if z.shape[0] > 1 else z.shape[1]
+
+
+def _check_logits(what: str, logits: Tensor, temperature: float) -> None:
+    if logits.dtype not in _FLOAT:
+        raise ValueError(f"{what}: logits are bf16 or fp32, not {logits.dtype}")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 31:
+        raise ValueError(f"{what}: logits of shape {tuple(logits.shape)}")
+    if logits.numel() // logits.shape[-1] >= 1 << 31:
+        raise ValueError(f"{what}: fewer than 2^31 rows")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"{what}: the temperature is positive, not {temperature}")
+
+
+def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """The `k` largest of each row of `logits [..., V]` (bf16 or fp32, `1 <= k <= min(V, 256)`), their columns and the
+    logsumexp of `logits / temperature` over the rest of the row. NaN counts as the largest. Not differentiable."""
+    _check_logits("top_logits", logits, temperature)
+    V = logits.shape[-1]
+    if not 1 <= k <= min(V, MAX_K):
+        raise ValueError(f"top_logits: k from 1 to {min(V, MAX_K)}, not {k}")
+    _on_current_device("top_logits", logits)
+    lead = logits.shape[:-1]
+    z = _rows_of(logits.detach())
+    rows = z.shape[0]
+    values = torch.empty(rows, k, device=z.device, dtype=z.dtype)
+    indices = torch.empty(rows, k, device=z.device, dtype=torch.int32)
+    tail = torch.empty(rows, device=z.device, dtype=torch.float32)
+    if rows > 0:
+        _check(_lib().pd_top_logits(z.data_ptr(), rows, V, _pitch(z), k, 1.0 / temperature, values.data_ptr(),
+                                    indices.data_ptr(), tail.data_ptr(), int(z.dtype == torch.float32), _s()), "top_logits")
+    return TopLogits(values.view(*lead, k), indices.view(*lead, k), tail.view(lead))
+
+
+def _launch(z: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None, temperature: float, loss: Tensor | None,
+            dz: Tensor | None, scale: Tensor | None) -> None:
+    rows, V = z.shape
+    _check(_lib().pd_top_kl(z.data_ptr(), rows, V, _pitch(z), indices.data_ptr(), int(indices.dtype == torch.int64),
+                            values.data_ptr(), int(values.dtype == torch.float32), indices.shape[1],
+                            None if tail is None else tail.data_ptr(), 1.0 / temperature,
+                            None if loss is None else loss.data_ptr(), None if dz is None else dz.data_ptr(),
+                            0 if dz is None else dz.stride(0), None if scale is None else scale.data_ptr(),
+                            int(z.dtype == torch.float32), nv.status_word().data_ptr(), nv.refused_ptr(), _s()), "top_kl")
+
+
+def _grad_like(z: Tensor) -> Tensor:
+    """`[rows, V]` whose rows start at the same address modulo 16 bytes as the rows of `z`."""
+    per = 16 // z.element_size()
+    rows, V = z.shape
+    pitch = V + (_pitch(z) - V) % per
+    first = z.data_ptr() % 16 // z.element_size()
+    return torch.empty(first + rows * pitch, device=z.device, dtype=z.dtype).as_strided((rows, V), (pitch, 1), first)
+
+
+class _TopKL(torch.autograd.Function):
+    """The backward runs the kernel again with the upstream gradient of each row: 2 reads and a write of the logits for
+    both passes, against a read and two writes had the forward kept an unscaled gradient, and nothing is held between."""
+
+    @staticmethod
+    def forward(ctx, z: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None, temperature: float) -> Tensor:  # type: ignore[override]
+        loss = torch.empty(z.shape[0], device=z.device, dtype=torch.float32)
+        if z.shape[0] > 0:
+            _launch(z, indices, values, tail, temperature, loss, None, None)
+        ctx.save_for_backward(z, indices, values, tail)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss: Tensor):  # type: ignore[override]
+        z, indices, values, tail = ctx.saved_tensors
+        dz = _grad_like(z)
+        if z.shape[0] > 0:
+            _launch(z, indices, values, tail, ctx.temperature, None, dz, _dense(dloss.float()))
+        return dz, None, None, None, None
+
+
+def _arguments(what: str, logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None, temperature: float):
+    _check_logits(what, logits, temperature)
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if indices.dtype not in (torch.int32, torch.int64) or indices.shape[:-1] != lead or indices.dim() != logits.dim():
+        raise ValueError(f"{what}: columns are int32 or int64 of shape {tuple(lead)} + [k], not {indices.dtype} "
+                         f"{tuple(indices.shape)}")
+    k = indices.shape[-1]
+    if not 1 <= k <= MAX_K:
+        raise ValueError(f"{what}: 1 to {MAX_K} slots a row, not {k}")
+    if values.dtype not in _FLOAT or values.shape != indices.shape:
+        raise ValueError(f"{what}: values are bf16 or fp32 of shape {tuple(indices.shape)}, not {values.dtype} "
+                         f"{tuple(values.shape)}")
+    if tail is not None and (tail.dtype != torch.float32 or tail.shape != lead):
+        raise ValueError(f"{what}: the tail is fp32 of shape {tuple(lead)}, not {tail.dtype} {tuple(tail.shape)}")
+    _on_current_device(what, logits, indices, values, tail)
+    limit = _lib().pd_top_kl_max_columns(int(logits.dtype == torch.float32))
+    if V > limit:
+        raise ValueError(f"{what}: rows of at most {limit} {logits.dtype} logits, not {V}")
+    nv.raise_refused()
+    return (_rows_of(logits), _dense(indices.reshape(-1, k)), _dense(values.detach().reshape(-1, k)),
+            None if tail is None else _dense(tail.detach().reshape(-1)))
+
+
+def top_kl(logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None = None, temperature: float = 1.0) -> Tensor:
+    """Divergence of every row from its teacher, `[...]` fp32, differentiable in `logits`.
+
+    `logits [..., V]` bf16 or fp32: the student's. `indices`, `values [..., k]`: the teacher's logits and their columns
+    (int32 or int64; negative: an unused slot; a column named more than once has the sum of its probabilities; one that is
+    not below `V` is refused like an unused slot and reported as `native.raise_refused` does). `tail [...]`: the teacher's
+    logsumexp of all other logits over the temperature; without it the teacher has its `k` slots alone. Both sides are taken
+    at `temperature`. A row whose teacher has no mass counts zero, with a zero gradient."""
+    z, indices, values, tail = _arguments("top_kl", logits, indices, values, tail, temperature)
+    return _TopKL.apply(z, indices, values, tail, temperature).view(logits.shape[:-1])
+
+
+def top_kl_rows(logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None = None, temperature: float = 1.0,
+                want_grad: bool = True) -> tuple[Tensor, Tensor | None]:
+    """`top_kl` of `[rows, V]` logits and (optionally) its gradient with respect to them, each row's by its own loss, in
+    one pass over the logits (the counterpart of `elementwise.vocab_kl_rows`; no autograd)."""
+    if logits.dim() != 2:
+        raise ValueError(f"top_kl_rows: logits [rows, V], not {tuple(logits.shape)}")
+    z, indices, values, tail = _arguments("top_kl_rows", logits.detach(), indices, values, tail, temperature)
+    loss = torch.empty(z.shape[0], device=z.device, dtype=torch.float32)
+    dz = _grad_like(z) if want_grad else None
+    if z.shape[0] > 0:
+        _launch(z, indices, values, tail, temperature, loss, dz, None)
+    return loss, dz
+
+
+def next_token_loss(logits: Tensor, targets: Tensor) -> Tensor:
+    """Mean cross entropy of `targets [...]` (int32 or int64; negative: no target here, as it counts for nothing, not for
+    the mean either) under `logits [..., V]`."""
+    loss = top_kl(logits, targets.unsqueeze(-1), torch.zeros(*targets.shape, 1, device=logits.device))
+    return loss.sum() / (targets >= 0).sum()
+
+
+# ---- plain torch ----------------------------------------------------------------------------------------------------
+
+def eager_top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    indices = torch.sort(logits.detach(), dim=-1, descending=True, stable=True)[1][..., :k]
+    rest = (logits.detach().float() / temperature).scatter(-1, indices, float("-inf"))
+    return TopLogits(torch.gather(logits.detach(), -1, indices), indices.to(torch.int32), torch.logsumexp(rest, -1))
+
+
+def eager_top_kl(logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None = None,
+                 temperature: float = 1.0) -> Tensor:
+    used = indices >= 0
+    columns = indices.long().clamp(min=0)
+    logq = torch.log_softmax((logits if logits.dtype == torch.float64 else logits.float()) / temperature, -1)
+    low = torch.full_like(logq[..., :1], float("-inf"))
+    teacher = torch.where(used, values.to(logq.dtype) / temperature, low)
+    teacher = torch.cat([teacher, low if tail is None else tail.to(logq.dtype).unsqueeze(-1)], -1)
+    live = (teacher > float("-inf")).any(-1, keepdim=True)
+    logp = torch.log_softmax(torch.where(live, teacher, 0.0), -1)
+    # unused slots point at column 0 and must not name it
+    named = torch.zeros_like(logq).scatter_add_(-1, columns, used.to(logq.dtype)) > 0
+    others = logq.masked_fill(named, float("-inf"))
+    some = (others > float("-inf")).any(-1, keepdim=True)
+    rest = torch.where(some, torch.logsumexp(torch.where(some, others, 0.0), -1, keepdim=True), low)
+    events = torch.cat([torch.gather(logq, -1, columns), rest], -1)
+    counts = live & (logp > float("-inf"))
+    return torch.where(counts, logp.exp() * (logp - torch.where(counts, events, 0.0)), 0.0).sum(-1)

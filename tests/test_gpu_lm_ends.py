@@ -1,0 +1,541 @@
+"""Layer norm, token embedding, top logits and the distillation loss against plain statements in 64 bits.
+
+Tolerances are error bounds of the arithmetic, not fits: `u = 2^-24` is half a step of fp32, a sum of n terms in order is
+off by at most n u times the sum of its terms' sizes, a stored bf16 value by half a step (2^-8 of its size).
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+bf, f32 = torch.bfloat16, torch.float32
+U = 2.0**-24
+
+
+@pytest.fixture(scope="module")
+def nv():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from param_decomp_b200.ops import native
+
+    native.lib()  # must load: no silent fallback on a GPU box
+    return native
+
+
+def _done(nv):
+    torch.cuda.synchronize()
+    nv.check_status()
+
+
+def _within(got, want, bound, what):
+    """`got` is `want` (64 bits) to within `bound` and the rounding to the type that it is stored in."""
+    half_step = 2.0**-8 if got.dtype == bf else U
+    got, want = got.detach().double().cpu(), want.cpu()
+    limit = bound.cpu() * (1 + 2.0**-7) + want.abs() * half_step + 1e-300
+    off = (got - want).abs()
+    assert bool((off <= limit).all()), f"{what}: {float((off / limit).max()):.3f} of its bound"
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- layer norm -------------------------------------------------------------------------------------------------------
+
+
+def _norm_reference(x, w, b, dy, eps):
+    x, dy = x.double(), dy.double()
+    w = torch.ones(x.shape[1], dtype=torch.float64) if w is None else w.double()
+    b = torch.zeros(x.shape[1], dtype=torch.float64) if b is None else b.double()
+    mean = x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + eps)
+    xh = (x - mean) * rstd
+    g = dy * w
+    dx = rstd * (g - g.mean(1, keepdim=True) - xh * (g * xh).mean(1, keepdim=True))
+    # a row's sum: at most 24 terms a thread, 5 halvings in a warp, 16 warps; the mean's error is relative to mean |x|
+    n = 64
+    spread = xh.abs() + rstd * x.abs().mean(1, keepdim=True)
+    bounds = dict(
+        y=2 * n * U * (spread * w.abs() + b.abs()),
+        dx=4 * n * U * rstd * (g.abs() + g.abs().mean(1, keepdim=True) + spread * (g.abs() * spread).mean(1, keepdim=True)),
+        dw=(x.shape[0] + 2 * n) * U * (dy.abs() * spread).sum(0),
+        db=(x.shape[0] + n) * U * dy.abs().sum(0))
+    return dict(y=xh * w + b, dx=dx, dw=(dy * xh).sum(0), db=dy.sum(0)), bounds
+
+
+@pytest.mark.parametrize("p_type", [bf, f32])
+@pytest.mark.parametrize("x_type", [bf, f32])
+@pytest.mark.parametrize("rows,d", [(1, 1), (3, 7), (5, 8), (700, 33), (33, 256), (2500, 768), (257, 769), (64, 1000), (129, 1032),
+                                    (41, 2047), (300, 4096), (7, 8192), (9, 8193), (4, 12288)])
+def test_layer_norm_and_its_gradients(nv, rows, d, x_type, p_type):
+    from param_decomp_b200.ops.elementwise import layer_norm
+
+    g = _gen(rows * d)
+    x = (torch.randn(rows, d, generator=g) * 2 + 1).to(x_type)
+    w, b = (1 + 0.3 * torch.randn(d, generator=g)).to(p_type), torch.randn(d, generator=g).to(p_type)
+    dy = torch.randn(rows, d, generator=g).to(x_type)
+    want, bounds = _norm_reference(x, w, b, dy, 1e-5)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    y = layer_norm(*leaves, 1e-5)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.cuda())
+    _done(nv)
+    assert y.dtype == x_type and dx.dtype == x_type and dw.dtype == p_type and db.dtype == p_type
+    for name, got in dict(y=y, dx=dx, dw=dw, db=db).items():
+        _within(got, want[name], bounds[name], name)
+
+
+def test_layer_norm_options(nv):
+    """No parameters, one of them, frozen ones, only parameters trained, no gradient at all, empty batches, leading axes,
+    strided inputs and upstream gradients, and inputs at addresses that allow no 16-byte access."""
+    from param_decomp_b200.ops.elementwise import layer_norm
+
+    g = _gen(1)
+    x, dy = torch.randn(6, 10, 264, generator=g), torch.randn(6, 10, 264, generator=g)
+    w, b = torch.randn(264, generator=g), torch.randn(264, generator=g)
+    for use_w, use_b, train in [(False, False, "x"), (True, False, "xw"), (False, True, "xb"), (True, True, "x"), (True, True, "w"),
+                                (True, True, "b"), (True, True, "")]:
+        want, bounds = _norm_reference(x.view(60, 264), w if use_w else None, b if use_b else None, dy.view(60, 264), 1e-6)
+        leaf = {"x": x.cuda().requires_grad_("x" in train), "w": w.cuda().requires_grad_("w" in train) if use_w else None,
+                "b": b.cuda().requires_grad_("b" in train) if use_b else None}
+        y = layer_norm(leaf["x"], leaf["w"], leaf["b"], 1e-6)
+        assert y.shape == x.shape and y.requires_grad == bool(train)
+        _within(y.view(60, 264), want["y"], bounds["y"], "y")
+        if train:
+            for k, grad in zip(train, torch.autograd.grad(y, [leaf[k] for k in train], dy.cuda())):
+                _within(grad.reshape(want["d" + k].shape), want["d" + k], bounds["d" + k], "d" + k)
+    # a row of a wider tensor, an expanded upstream gradient, a tensor that starts 4 bytes into its storage
+    wide = torch.randn(40, 600, generator=g)
+    xs = wide.cuda()[:, 5:269].requires_grad_(True)
+    y = layer_norm(xs, w.cuda(), b.cuda(), 1e-6)
+    (dx,) = torch.autograd.grad(y.sum(), (xs,))
+    want, bounds = _norm_reference(wide[:, 5:269], w, b, torch.ones(40, 264), 1e-6)
+    _within(y, want["y"], bounds["y"], "y")
+    _within(dx, want["dx"], bounds["dx"], "dx")
+    flat = torch.randn(40 * 264 + 1, generator=g)
+    odd = flat.cuda()[1:].view(40, 264)
+    want, bounds = _norm_reference(flat[1:].view(40, 264), w, b, torch.ones(40, 264), 1e-6)
+    _within(layer_norm(odd, w.cuda(), b.cuda(), 1e-6), want["y"], bounds["y"], "y")
+    # nothing to norm
+    none = torch.zeros(0, 264, device="cuda", requires_grad=True)
+    wg, bg = w.cuda().requires_grad_(True), b.cuda().requires_grad_(True)
+    grads = torch.autograd.grad(layer_norm(none, wg, bg, 1e-6).sum(), (none, wg, bg))
+    assert grads[0].shape == (0, 264) and not bool(grads[1].any()) and not bool(grads[2].any())
+    _done(nv)
+
+
+def test_layer_norm_far_means_and_special_rows(nv):
+    """Rows far from zero keep their variance (it is summed around the mean), a constant row has the gradient of its eps, a
+    row with an infinity or NaN stays its own affair."""
+    from param_decomp_b200.ops.elementwise import layer_norm
+
+    g = _gen(2)
+    x = torch.randn(50, 768, generator=g) + 1000.0
+    x[7] = 3.0
+    w, b = torch.randn(768, generator=g), torch.randn(768, generator=g)
+    dy = torch.randn(50, 768, generator=g)
+    want, bounds = _norm_reference(x, w, b, dy, 1e-5)
+    xs = x.cuda().requires_grad_(True)
+    y = layer_norm(xs, w.cuda(), b.cuda(), 1e-5)
+    (dx,) = torch.autograd.grad(y, (xs,), dy.cuda())
+    _within(y, want["y"], bounds["y"], "y")
+    _within(dx, want["dx"], bounds["dx"], "dx")
+    bad = x.clone()
+    bad[3, 5], bad[9, 700] = float("nan"), float("inf")
+    yb = layer_norm(bad.cuda(), w.cuda(), b.cuda(), 1e-5)
+    keep = [i for i in range(50) if i not in (3, 9)]
+    assert torch.equal(yb[keep], y.detach()[keep]) and bool(yb[3].isnan().all()) and bool(yb[9].isnan().any())
+    _done(nv)
+
+
+def test_layer_norm_gradient_against_differences(nv):
+    from param_decomp_b200.ops.elementwise import layer_norm
+
+    g = _gen(3)
+    x, w, b = torch.randn(3, 40, generator=g), torch.randn(40, generator=g), torch.randn(40, generator=g)
+    dy = torch.randn(3, 40, generator=g)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    grads = torch.autograd.grad(layer_norm(*leaves, 1e-5), leaves, dy.cuda())
+
+    def loss(x, w, b):
+        m = x.mean(1, keepdim=True)
+        return float((((x - m) / torch.sqrt(((x - m) ** 2).mean(1, keepdim=True) + 1e-5) * w + b) * dy.double()).sum())
+
+    args = [t.double() for t in (x, w, b)]
+    for i, grad in enumerate(grads):
+        way = torch.randn(args[i].shape, generator=g, dtype=torch.float64)
+        h = 1e-5
+        plus, minus = ([a + s * h * way if j == i else a for j, a in enumerate(args)] for s in (1, -1))
+        slope = (loss(*plus) - loss(*minus)) / (2 * h)
+        size = float((grad.cpu().double().abs() * way.abs()).sum())
+        # differences: h^2 times the third derivative (order one here) and 2^-52 / h; the kernel: 512 u
+        assert abs(float((grad.cpu().double() * way).sum()) - slope) <= size * 512 * U + 1e-6
+
+
+# ---- embedding --------------------------------------------------------------------------------------------------------
+
+
+def _zipf(n, V, g):
+    p = 1.0 / torch.arange(1, V + 1, dtype=torch.float64)
+    return torch.multinomial(p, n, replacement=True, generator=g)
+
+
+@pytest.mark.parametrize("table_type,out_type", [(bf, bf), (f32, bf), (f32, f32), (bf, f32)])
+@pytest.mark.parametrize("n,V,d", [(1, 1, 1), (1, 50, 8), (33, 1, 24), (32, 7, 8), (2500, 3, 40), (1000, 2000, 264), (5000, 300, 33),
+                                   (4097, 50277, 16), (300, 400000, 8), (20000, 1000, 768), (777, 151936, 5), (2048, 147, 1032)])
+def test_embedding_and_its_gradient(nv, n, V, d, table_type, out_type):
+    """Rows seen never, once, up to a slab of tokens, and by more than a slab (one token fills a slab row exactly, runs that
+    start and end inside slabs, one id for all tokens)."""
+    from param_decomp_b200.ops.embedding import embedding
+
+    g = _gen(n + V + d)
+    tokens = _zipf(n, V, g) if V > 1 else torch.zeros(n, dtype=torch.int64)
+    table, dy = torch.randn(V, d, generator=g).to(table_type), torch.randn(n, d, generator=g).to(out_type)
+    scale = math.sqrt(d)
+    for ids in (tokens.cuda(), tokens.to(torch.int32).cuda()):
+        leaf = table.cuda().requires_grad_(True)
+        y = embedding(ids, leaf, scale, out_dtype=out_type)
+        (dE,) = torch.autograd.grad(y, (leaf,), dy.cuda())
+        _done(nv)
+        assert y.dtype == out_type and dE.dtype == table_type and y.shape == (n, d) and dE.shape == (V, d)
+        s = float(torch.tensor(scale, dtype=f32))
+        want = table.double()[tokens] * s
+        _within(y, want, 2 * U * want.abs(), "y")
+        wantE = torch.zeros(V, d, dtype=torch.float64).index_add_(0, tokens, dy.double()) * s
+        sizes = torch.zeros(V, d, dtype=torch.float64).index_add_(0, tokens, dy.double().abs()) * s
+        counts = torch.bincount(tokens, minlength=V).double()[:, None]
+        _within(dE, wantE, (counts + 2) * U * sizes, "dE")
+
+
+def test_embedding_gradient_is_the_same_every_time(nv):
+    from param_decomp_b200.ops.embedding import embedding
+
+    g = _gen(5)
+    tokens, table, dy = _zipf(30000, 500, g).cuda(), torch.randn(500, 136, generator=g).cuda().requires_grad_(True), torch.randn(
+        30000, 136, generator=g).cuda()
+    first = torch.autograd.grad(embedding(tokens, table), (table,), dy)[0]
+    for _ in range(10):
+        assert torch.equal(first, torch.autograd.grad(embedding(tokens, table), (table,), dy)[0])
+
+
+def test_embedding_options_and_refused_tokens(nv):
+    from param_decomp_b200.ops.embedding import embedding
+
+    g = _gen(6)
+    table = torch.randn(30, 24, generator=g).cuda().requires_grad_(True)
+    # leading axes, strided ids, ids of an odd storage offset, a transposed table, an expanded upstream gradient
+    ids = torch.randint(0, 30, (4, 9), generator=g).cuda()
+    want = table.detach()[ids.T]
+    y = embedding(ids.T, table)
+    assert torch.equal(y.detach(), want) and y.shape == (9, 4, 24)
+    (dE,) = torch.autograd.grad(y.sum(), (table,))
+    assert torch.equal(dE, torch.bincount(ids.view(-1), minlength=30)[:, None].expand(30, 24).float())
+    square = torch.randn(24, 30, generator=g).cuda()
+    assert torch.equal(embedding(ids.view(-1)[1:], square.T), square.T[ids.view(-1)[1:]])
+    # none
+    y = embedding(ids[:0], table)
+    assert y.shape == (0, 9, 24) and not bool(torch.autograd.grad(y.sum(), (table,))[0].any())
+    _done(nv)
+    # unknown ids: zero rows, no part in the gradient, reported to the next call and by the status word
+    bad = ids.view(-1).clone()
+    bad[3], bad[7], bad[20] = -1, 30, 2**40
+    y = embedding(bad, table)
+    (dE,) = torch.autograd.grad(y, (table,), torch.ones_like(y))
+    torch.cuda.synchronize()
+    good = torch.ones(36, dtype=torch.bool)
+    good[[3, 7, 20]] = False
+    assert torch.equal(y.detach().cpu()[good], table.detach().cpu()[bad.cpu()[good]]) and not bool(y.detach().cpu()[~good].any())
+    assert torch.equal(dE[:, 0].cpu(), torch.bincount(bad.cpu()[good], minlength=30).float())
+    with pytest.raises(nv.NativeError, match="token"):
+        embedding(ids, table)
+    embedding(bad, table)
+    with pytest.raises(nv.NativeError, match="token"):
+        nv.check_status()
+    embedding(ids, table)
+    _done(nv)
+
+
+# ---- top logits -------------------------------------------------------------------------------------------------------
+
+
+def _top_reference(z, k, T):
+    idx = torch.sort(z.double(), dim=1, descending=True, stable=True)[1][:, :k]
+    rest = (z.double() / T).scatter(1, idx, -math.inf)
+    return torch.gather(z, 1, idx), idx.to(torch.int32), torch.logsumexp(rest, 1)
+
+
+def _check_top(z, k, T=1.0):
+    from param_decomp_b200.ops.top_logits import top_logits
+
+    values, indices, tail = top_logits(z, k, T)
+    want = _top_reference(z.cpu(), k, T)
+    assert torch.equal(indices.cpu(), want[1])
+    assert torch.equal(values.cpu().view(torch.int16 if z.dtype == bf else torch.int32),
+                       want[0].view(torch.int16 if z.dtype == bf else torch.int32))
+    fine = want[2].isfinite()
+    assert torch.equal(tail.cpu()[~fine].double(), want[2][~fine])
+    # a thread adds V / 256 terms at most, each off by its argument's rounding (under 128 u) and the exponential's (4 u)
+    bound = (z.shape[1] / 256 + 64 + 132) * U + 4 * U * want[2][fine].abs()
+    assert bool(((tail.cpu()[fine].double() - want[2][fine]).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("n,V,k", [(1, 1, 1), (3, 5, 5), (2, 8, 3), (5, 100, 99), (4, 1000, 256), (9, 2000, 8), (700, 2003, 40),
+                                   (3, 4096, 128), (5, 4099, 1), (7, 50277, 64), (2, 151936, 256), (1, 300001, 200)])
+def test_top_logits_against_a_stable_sort(nv, n, V, k, kind):
+    z = (torch.randn(n, V, generator=_gen(n + V)) * 2.5).to(kind).cuda()
+    _check_top(z, k)
+    _check_top(z, k, 2.0)
+    _done(nv)
+
+
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("V,k", [(2003, 40), (50277, 64), (9000, 256)])
+def test_top_logits_of_awkward_rows(nv, V, k, kind):
+    """Equal logits in masses, few logits above -inf, infinities, zeros of both signs, values that rise or fall along the
+    row, one column far above the rest, all candidates in one block's columns, rows at odd addresses."""
+    g = _gen(V)
+    z = torch.randn(14, V, generator=g)
+    z[0] = 1.0
+    z[1] = (z[1] * 2).round()
+    z[2] = -math.inf
+    z[2, V // 2:V // 2 + k // 2] = 1.0
+    z[3] = -math.inf
+    z[4, 5:9] = math.inf
+    z[5, :k + 3] = math.inf
+    z[6] = torch.where(torch.arange(V) % 3 == 0, 0.0, -0.0)
+    z[7] = torch.linspace(-5, 5, V)
+    z[8] = torch.linspace(5, -5, V)
+    z[9] -= 200.0
+    z[9, :k] = 0.0
+    z[10, 17:17 + 2 * k] += 50.0
+    z[11] = torch.finfo(kind).min
+    z[11, 3::7] = -1.0
+    z[12] = torch.finfo(kind).min
+    z[13, 64:80] = 30.0
+    z = z.to(kind)
+    _check_top(z.cuda(), k)
+    wide = torch.full((14, V + 11), 99.0, dtype=kind)
+    wide[:, 3:3 + V] = z
+    _check_top(wide.cuda()[:, 3:3 + V], k)
+    _done(nv)
+
+
+def test_top_logits_shapes_and_nan(nv):
+    from param_decomp_b200.ops.top_logits import top_logits
+
+    g = _gen(9)
+    z = torch.randn(2, 3, 5000, generator=g)
+    z[0, 1, 77] = float("nan")
+    z[1, 2, 4000:4010] = float("nan")
+    out = top_logits(z.cuda(), 4)
+    assert out.values.shape == (2, 3, 4) and out.indices.shape == (2, 3, 4) and out.tail.shape == (2, 3)
+    assert int(out.indices[0, 1, 0]) == 77 and bool(out.values[0, 1, 0].isnan()) and bool(out.tail[0, 1].isfinite())
+    assert out.indices[1, 2].tolist() == [4000, 4001, 4002, 4003] and bool(out.tail[1, 2].isnan())
+    t = torch.randn(5000, 6, generator=g).cuda()
+    assert torch.equal(top_logits(t.T, 4).indices, top_logits(t.T.contiguous(), 4).indices)
+    e = top_logits(t[:, 0].expand(3, 5000), 4)
+    assert torch.equal(e.indices[0], e.indices[2])
+    assert top_logits(t.T[:0], 4).values.shape == (0, 4)
+    assert torch.equal(top_logits(t[:, 0], 4).indices, e.indices[0])
+    _done(nv)
+
+
+# ---- distillation loss ------------------------------------------------------------------------------------------------
+
+
+def _kl_reference(z, idx, t, tail, T):
+    """Loss, gradient and their error bounds, in 64 bits."""
+    n, V = z.shape
+    x = z.double() / T
+    used = (idx >= 0) & (idx < V)
+    col = torch.where(used, idx, 0).long()
+    low = torch.full((n, 1), -math.inf, dtype=torch.float64)
+    events = torch.cat([torch.where(used, t.double() / T, -math.inf), low if tail is None else tail.double()[:, None]], 1)
+    live = (events > -math.inf).any(1, keepdim=True)
+    logp = torch.log_softmax(torch.where(live, events, 0.0), 1)
+    p = torch.where(live, logp.exp(), 0.0)
+    named = torch.zeros(n, V, dtype=torch.float64).scatter_add_(1, col, used.double()) > 0
+    p_col = torch.zeros(n, V, dtype=torch.float64).scatter_add_(1, col, torch.where(used, p[:, :-1], 0.0))
+    q = torch.softmax(x, 1)
+    lse = torch.logsumexp(x, 1, keepdim=True)
+    others = x.masked_fill(named, -math.inf)
+    some = (others > -math.inf).any(1, keepdim=True)
+    lse_rest = torch.where(some, torch.logsumexp(torch.where(some, others, 0.0), 1, keepdim=True), low)
+    r = p[:, -1:]
+    logq = torch.cat([torch.gather(x, 1, col) - lse, lse_rest - lse], 1)
+    terms = torch.where(p > 0, p * (torch.where(p > 0, logp, 0.0) - torch.where(p > 0, logq, 0.0)), 0.0)
+    share = torch.where(some, (others - torch.where(some, lse_rest, 0.0)).exp(), 0.0)
+    dz = torch.where(named, q - p_col, q - r * share) / T
+    dz = torch.where(live, dz, 0.0)
+    # a sum of exponentials: V / 256 terms a thread, arguments' rounding under 128 u, 4 u an exponential, merges
+    lost = (V / 256 + 256) * U
+    loss_bound = 4 * lost + 16 * U * terms.abs().sum(1)
+    dz_bound = (4 * lost + 256 * U) * (q + r * share + p_col) / T
+    return terms.sum(1), dz, loss_bound, torch.where(live, dz_bound, 0.0)
+
+
+def _check_kl(z, idx, t, tail=None, T=1.0, scale=None):
+    from param_decomp_b200.ops.top_logits import top_kl, top_kl_rows
+
+    cpu = lambda a: None if a is None else a.cpu()  # noqa: E731
+    loss, dz, lb, db = _kl_reference(cpu(z), cpu(idx), cpu(t), cpu(tail), T)
+    got, grad = top_kl_rows(z, idx, t, tail, T)
+    assert grad.shape == z.shape and grad.dtype == z.dtype and got.dtype == f32
+    _within(got, loss, lb, "loss")
+    _within(grad, dz, db, "dz")
+    assert torch.equal(top_kl_rows(z, idx, t, tail, T, want_grad=False)[0], got)
+    leaf = z.detach().requires_grad_(True)
+    up = torch.rand(z.shape[0], generator=_gen(3)) + 0.5
+    auto = top_kl(leaf, idx, t, tail, T)
+    assert torch.equal(auto.detach(), got)
+    (grad,) = torch.autograd.grad(auto, (leaf,), up.cuda())
+    _within(grad, dz * up.double()[:, None], (db + 4 * U * dz.abs()) * up.double()[:, None], "dz")
+
+
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("n,V,K", [(1, 1, 1), (2, 2, 1), (3, 7, 7), (4, 8, 3), (5, 9, 2), (6, 1000, 256), (900, 2003, 9), (5, 8195, 64),
+                                   (310, 50277, 64), (3, 151936, 130), (40, 300001, 5)])
+def test_top_kl_and_its_gradient(nv, n, V, K, kind):
+    """Clusters of 1 to 8 blocks, several rows a cluster, rows at every address modulo 16, both index types."""
+    g = _gen(n + V + K)
+    z = (torch.randn(n, V, generator=g) * 2).to(kind)
+    teacher = z.float() + torch.randn(n, V, generator=g)
+    t, idx = torch.topk(teacher, K, dim=1)
+    tail = torch.logsumexp(teacher.scatter(1, idx, -math.inf) / 2.0, 1)
+    _check_kl(z.cuda(), idx.cuda(), t.to(kind).cuda(), None)
+    if tail.isfinite().all():
+        _check_kl(z.cuda(), idx.to(torch.int32).cuda(), t.cuda(), tail.cuda(), 2.0)
+    wide = torch.full((n, V + 11), 77.0, dtype=kind)
+    wide[:, 3:3 + V] = z
+    _check_kl(wide.cuda()[:, 3:3 + V], idx.cuda(), t.cuda(), None)
+    _done(nv)
+
+
+@pytest.mark.parametrize("kind,V", [(bf, 470001), (bf, 884720), (f32, 225001), (f32, 442352)])
+def test_top_kl_of_the_longest_rows(nv, kind, V):
+    g = _gen(V)
+    z = (torch.randn(2, V, generator=g) * 2).to(kind)
+    teacher = z.float() + torch.randn(2, V, generator=g)
+    t, idx = torch.topk(teacher, 17, dim=1)
+    tail = torch.logsumexp(teacher.scatter(1, idx, -math.inf), 1)
+    _check_kl(z.cuda(), idx.cuda(), t.cuda(), tail.cuda())
+    _done(nv)
+
+
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("V", [1003, 50277, 200003])
+def test_top_kl_of_awkward_rows(nv, V, kind):
+    """Unused slots (with NaN in them), a column named several times, rows without any slot or any mass, masked student
+    logits (-inf and the type's lowest) beside and under the named ones, a rest far below the named logits and the other
+    way round, a teacher of one certain column."""
+    g = _gen(V)
+    n, K = 12, 6
+    z = torch.randn(n, V, generator=g) * 2
+    idx = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(n)])
+    t = torch.randn(n, K, generator=g)
+    tail = torch.randn(n, generator=g)
+    idx[0, 2:4], t[0, 2:4] = -1, float("nan")
+    idx[1, 1] = idx[1, 4] = idx[1, 5] = idx[1, 0]
+    idx[2, 3] = idx[2, 2]
+    idx[3], tail[3] = -1, -math.inf
+    t[4], tail[4] = -math.inf, -math.inf
+    idx[5] = -1
+    keep = z[6, idx[6]].clone()
+    z[6] = -math.inf
+    z[6, idx[6]] = keep
+    z[6, (int(idx[6, 0]) + 1) % V] = 0.5
+    z[7, 100:] = torch.finfo(kind).min
+    z[7, idx[7]] = 0.25
+    z[8] -= 150.0
+    z[8, idx[8]] = 3.0
+    z[9, idx[9]] = -100.0
+    t[10, 1:], tail[10] = -math.inf, -math.inf
+    z[11] = torch.finfo(kind).min
+    z[11, 5::3] = 1.0
+    z[11, idx[11]] = 2.0
+    z, t = z.to(kind), t.to(kind)
+    _check_kl(z.cuda(), idx.cuda(), t.cuda(), tail.cuda())
+    some = [i for i in range(n) if i != 5]
+    _check_kl(z[some].cuda(), idx[some].cuda(), t[some].cuda(), None, 3.0)
+    _done(nv)
+
+
+def test_top_kl_where_the_loss_is_infinite(nv):
+    """A named column that the student has masked, or a rest that it has masked while the teacher has a tail: the loss is
+    infinite, the gradient is not, and the rows beside it are as without it."""
+    from param_decomp_b200.ops.top_logits import top_kl_rows
+
+    g = _gen(4)
+    z = torch.randn(3, 2000, generator=g)
+    idx, t, tail = torch.tensor([[4, 9], [4, 9], [4, 9]]), torch.randn(3, 2, generator=g), torch.zeros(3)
+    base = top_kl_rows(z.cuda(), idx.cuda(), t.cuda(), tail.cuda())
+    z[0, 4] = -math.inf
+    z[2] = -math.inf
+    z[2, 4:10] = 1.0
+    z[2, 5:9] = -math.inf
+    loss, dz = top_kl_rows(z.cuda(), idx.cuda(), t.cuda(), tail.cuda())
+    assert loss[0].item() == math.inf and loss[2].item() == math.inf and bool(dz.isfinite().all())
+    assert torch.equal(loss[1], base[0][1]) and torch.equal(dz[1], base[1][1])
+    p = torch.softmax(torch.cat([t, tail[:, None]], 1), 1)
+    assert abs(float(dz[0, 4]) + float(p[0, 0])) < 1e-6 and abs(float(dz[2, 9]) - (0.5 - float(p[2, 1]))) < 1e-6
+    assert abs(float(dz[0].double().sum())) < 2000 * U * 4  # a softmax's gradient sums to nothing
+    _done(nv)
+
+
+def test_top_kl_refused_columns_and_empty_batches(nv):
+    from param_decomp_b200.ops.top_logits import next_token_loss, top_kl, top_kl_rows
+
+    g = _gen(8)
+    z, t = torch.randn(5, 600, generator=g).cuda(), torch.randn(5, 3, generator=g).cuda()
+    idx = torch.randint(0, 600, (5, 3), generator=g).cuda()
+    bad, unused = idx.clone(), idx.clone()
+    bad[1, 2], bad[3, 0], unused[1, 2], unused[3, 0] = 600, 2**40, -1, -1
+    want = top_kl_rows(z, unused, t)
+    got = top_kl_rows(z, bad, t)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    torch.cuda.synchronize()
+    with pytest.raises(nv.NativeError, match="column"):
+        top_kl(z, idx, t)
+    top_kl(z, idx, t)
+    loss, dz = top_kl_rows(z[:0], idx[:0], t[:0])
+    assert loss.shape == (0,) and dz.shape == (0, 600)
+    # the mean over the positions that have a target, and its gradient
+    targets = torch.tensor([[3, -1, 599], [-1, 0, 3]])
+    logits = torch.randn(2, 3, 600, generator=g)
+    leaf = logits.cuda().requires_grad_(True)
+    ce = next_token_loss(leaf, targets.cuda())
+    (grad,) = torch.autograd.grad(ce, (leaf,))
+    ref = logits.double().requires_grad_(True)
+    want = torch.nn.functional.cross_entropy(ref.view(-1, 600), targets.view(-1), ignore_index=-1)
+    (want_grad,) = torch.autograd.grad(want, (ref,))
+    assert abs(float(ce) - float(want)) < 600 * U * 8
+    assert float((grad.cpu().double() - want_grad).abs().max()) < 600 * U
+    _done(nv)
+
+
+def test_top_kl_of_top_logits_is_the_whole_divergence(nv):
+    """The two together: at k one short of the row and at the whole row the loss is the divergence over all columns, between
+    it grows with k; and the gradient is that of differences."""
+    from param_decomp_b200.ops.top_logits import top_kl, top_logits
+
+    g = _gen(11)
+    teacher, z = torch.randn(6, 200, generator=g), torch.randn(6, 200, generator=g)
+    p = torch.log_softmax(teacher.double(), 1)
+    whole = (p.exp() * (p - torch.log_softmax(z.double(), 1))).sum(1)
+    before = torch.zeros(6)
+    for k in (1, 10, 100, 199, 200):
+        loss = top_kl(z.cuda(), top_logits(teacher.cuda(), k).indices, top_logits(teacher.cuda(), k).values,
+                      top_logits(teacher.cuda(), k).tail).cpu()
+        assert bool((loss >= before - 1e-6).all())
+        before = loss
+        if k >= 199:
+            assert float((loss.double() - whole).abs().max()) < 600 * U
+    leaf = z.cuda().requires_grad_(True)
+    top = top_logits(teacher.cuda(), 10)
+    (grad,) = torch.autograd.grad(top_kl(leaf, top.indices, top.values, top.tail).sum(), (leaf,))
+    way = torch.randn(6, 200, generator=g, dtype=torch.float64)
+    h = 1e-5
+    args = (top.indices.cpu(), top.values.cpu(), top.tail.cpu(), 1.0)
+    slope = sum(s * _kl_reference(z.double() + s * h * way, *args)[0].sum() for s in (1, -1)) / (2 * h)
+    assert abs(float((grad.cpu().double() * way).sum() - slope)) < 1e-5

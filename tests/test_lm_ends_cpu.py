@@ -1,0 +1,119 @@
+"""Layer norm, token embedding, top logits and the distillation loss without a GPU: what their entry points refuse, and the
+plain statements of the last two."""
+import math
+
+import pytest
+import torch
+
+from param_decomp_b200.ops.elementwise import layer_norm
+from param_decomp_b200.ops.embedding import embedding
+from param_decomp_b200.ops.native import NativeError
+from param_decomp_b200.ops.top_logits import eager_top_kl, eager_top_logits, next_token_loss, top_kl, top_kl_rows, top_logits
+
+F16, BF, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("x,w,b", [
+    (torch.zeros(2, 8, dtype=F16), None, None),  # types the kernels do not have
+    (torch.zeros(2, 8, dtype=torch.float64), None, None),
+    (torch.zeros(2, 8), torch.ones(8, dtype=F16), None),
+    (torch.zeros(2, 8), torch.ones(8, dtype=BF), torch.zeros(8)),  # scale and shift of two types
+    (torch.zeros(2, 8), torch.ones(7), None),
+    (torch.zeros(2, 8), torch.ones(1, 8), None),
+    (torch.zeros(2, 8), None, torch.zeros(9)),
+    (torch.zeros(2, 0), None, None),  # no columns, too many, no axis
+    (torch.zeros(1, 12289), None, None),
+    (torch.zeros(()), None, None),
+])
+def test_layer_norm_refusals(x, w, b):
+    with pytest.raises(ValueError, match="layer_norm"):
+        layer_norm(x, w, b, 1e-5)
+
+
+@pytest.mark.parametrize("tokens,table,out", [
+    (torch.zeros(3, dtype=torch.int16), torch.zeros(4, 8), None),
+    (torch.zeros(3), torch.zeros(4, 8), None),
+    (torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8, dtype=F16), None),
+    (torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8, 2), None),
+    (torch.zeros(3, dtype=torch.int64), torch.zeros(0, 8), None),
+    (torch.zeros(3, dtype=torch.int64), torch.zeros(4, 0), None),
+    (torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), F16),
+    (torch.zeros(1, dtype=torch.int64).expand(1 << 30), torch.zeros(4, 8), None),
+])
+def test_embedding_refusals(tokens, table, out):
+    with pytest.raises(ValueError, match="embedding"):
+        embedding(tokens, table, 1.0, out)
+
+
+@pytest.mark.parametrize("logits,k,T", [
+    (torch.zeros(2, 8, dtype=F16), 1, 1.0), (torch.zeros(2, 8), 0, 1.0), (torch.zeros(2, 8), 9, 1.0), (torch.zeros(2, 300), 257, 1.0),
+    (torch.zeros(2, 8), 1, 0.0), (torch.zeros(2, 8), 1, -1.0), (torch.zeros(2, 8), 1, math.inf), (torch.zeros(2, 8), 1, math.nan),
+    (torch.zeros(2, 0), 1, 1.0), (torch.zeros(()), 1, 1.0),
+])
+def test_top_logits_refusals(logits, k, T):
+    with pytest.raises(ValueError, match="top_logits"):
+        top_logits(logits, k, T)
+
+
+_IDX = torch.zeros(2, 3, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("logits,indices,values,tail,T", [
+    (torch.zeros(2, 8, dtype=F16), _IDX, torch.zeros(2, 3), None, 1.0),
+    (torch.zeros(2, 8), _IDX.to(torch.int16), torch.zeros(2, 3), None, 1.0),
+    (torch.zeros(2, 8), _IDX[:1], torch.zeros(1, 3), None, 1.0),
+    (torch.zeros(2, 8), _IDX[:, 0], torch.zeros(2), None, 1.0),
+    (torch.zeros(2, 8), _IDX, torch.zeros(2, 2), None, 1.0),
+    (torch.zeros(2, 8), _IDX, torch.zeros(2, 3, dtype=F16), None, 1.0),
+    (torch.zeros(2, 8), _IDX[:, :0], torch.zeros(2, 0), None, 1.0),
+    (torch.zeros(2, 8), torch.zeros(2, 257, dtype=torch.int64), torch.zeros(2, 257), None, 1.0),
+    (torch.zeros(2, 8), _IDX, torch.zeros(2, 3), torch.zeros(2, 1), 1.0),
+    (torch.zeros(2, 8), _IDX, torch.zeros(2, 3), torch.zeros(2, dtype=BF), 1.0),
+    (torch.zeros(2, 8), _IDX, torch.zeros(2, 3), None, 0.0),
+])
+def test_top_kl_refusals(logits, indices, values, tail, T):
+    for call in (top_kl, top_kl_rows):
+        with pytest.raises(ValueError, match="top_kl"):
+            call(logits, indices, values, tail, T)
+
+
+def test_tensors_on_the_host_are_refused():
+    z, idx = torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64)
+    for call in (lambda: layer_norm(z, None, None, 1e-5), lambda: embedding(idx, z), lambda: top_logits(z, 1),
+                 lambda: top_kl(z, idx, torch.zeros(2, 3)), lambda: next_token_loss(z, idx[:, 0])):
+        with pytest.raises(NativeError, match="cpu"):
+            call()
+
+
+def test_eager_top_logits_breaks_ties_by_column():
+    z = torch.tensor([[1.0, 3.0, 3.0, 2.0, 3.0], [0.0, -0.0, -1.0, 0.0, float("-inf")]])
+    top = eager_top_logits(z, 2)
+    assert top.indices.tolist() == [[1, 2], [0, 1]] and top.values.tolist() == [[3.0, 3.0], [0.0, 0.0]]
+    want = torch.tensor([math.log(math.exp(1) + math.exp(2) + math.exp(3)), math.log(1 + math.exp(-1))])
+    torch.testing.assert_close(top.tail, want)
+    assert eager_top_logits(z, 5).tail.tolist() == [-math.inf, -math.inf]
+
+
+@pytest.mark.parametrize("k", [1, 4, 19, 20])
+def test_eager_top_kl_is_a_divergence_of_events(k):
+    g = torch.Generator().manual_seed(k)
+    teacher, z = torch.randn(5, 20, generator=g, dtype=torch.float64), torch.randn(5, 20, generator=g, dtype=torch.float64)
+    order = torch.sort(teacher, 1, descending=True)[1]
+    p, q = (torch.softmax(t, 1).gather(1, order) for t in (teacher, z))
+    pe, qe = (torch.cat([t[:, :k], t[:, k:].sum(1, keepdim=True)], 1)[:, :k + (k < 20)] for t in (p, q))
+    want = (pe * (pe / qe).log()).sum(1)
+    top = eager_top_logits(teacher, k)
+    # the tail is kept in fp32: off by 2^-24 of its size
+    torch.testing.assert_close(eager_top_kl(z, top.indices, top.values, top.tail), want, atol=1e-6, rtol=0)
+    leaf = z.requires_grad_(True)
+    assert torch.autograd.gradcheck(lambda t: eager_top_kl(t, top.indices, top.values, top.tail, 2.0), (leaf,))
+
+
+def test_eager_top_kl_of_one_slot_is_cross_entropy():
+    g = torch.Generator().manual_seed(0)
+    z, target = torch.randn(6, 11, generator=g, requires_grad=True), torch.tensor([3, 0, -1, 10, -1, 3])
+    loss = eager_top_kl(z, target[:, None], torch.zeros(6, 1))
+    want = torch.nn.functional.cross_entropy(z, target, ignore_index=-1, reduction="none")
+    torch.testing.assert_close(loss, want)
+    ours, theirs = (torch.autograd.grad(t.sum(), (z,))[0] for t in (loss, want))
+    torch.testing.assert_close(ours, theirs)
