@@ -270,11 +270,15 @@ inline Shape shape_of(int d) {
   return {wpr, (d + 256 * wpr - 1) / (256 * wpr)};
 }
 
-// Blocks that fit the machine at once, at most one a row (or a row group).
+// Blocks that fit the machine at once, at most one a row (or a row group). What fits an SM is asked once a kernel and
+// block size (`fit`, zero at first; the answer is the same whoever writes it).
 template <typename K>
-inline int grid_for(K kern, int threads, size_t smem, long long rows, int rpb) {
-  int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1) return 0;
+inline int grid_for(K kern, int* fit, int threads, size_t smem, long long rows, int rpb) {
+  int& per_sm = fit[threads / 32];
+  if (per_sm == 0 && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1)) {
+    per_sm = 0;
+    return 0;
+  }
   return static_cast<int>(std::min<long long>((rows + rpb - 1) / rpb, 148ll * per_sm));
 }
 
@@ -283,7 +287,8 @@ int fwd(const void* x, const void* w, const void* b, void* y, float* mean, float
         int wpr, int p_fp32, cudaStream_t st) {
   const int threads = wpr == 1 ? 32 * kWarpsPerBlock : 32 * wpr;
   auto kern = layer_norm_fwd_kernel<T, kCh, kVec>;
-  const int grid = grid_for(kern, threads, 0, rows, threads / (32 * wpr));
+  static int fit[kMaxWarps + 1];
+  const int grid = grid_for(kern, fit, threads, 0, rows, threads / (32 * wpr));
   if (grid == 0) return 2;
   kern<<<grid, threads, 0, st>>>(static_cast<const T*>(x), w, b, static_cast<T*>(y), mean, rstd, rows, d, eps, wpr, p_fp32);
   return cudaGetLastError() == cudaSuccess ? 0 : 1;
@@ -295,7 +300,8 @@ int bwd(const void* x, const void* w, const void* dy, const float* mean, const f
   const int threads = wpr == 1 ? 32 * kWarpsPerBlock : 32 * wpr;
   const size_t smem = kParams && wpr == 1 ? static_cast<size_t>(2 * d) * sizeof(float) : 0;
   auto kern = layer_norm_bwd_kernel<T, kCh, kVec, kParams>;
-  int grid = grid_for(kern, threads, smem, rows, threads / (32 * wpr));
+  static int fit[kMaxWarps + 1];
+  int grid = grid_for(kern, fit, threads, smem, rows, threads / (32 * wpr));
   if (grid == 0) return 2;
   grid = std::min(grid, max_blocks);
   kern<<<grid, threads, smem, st>>>(static_cast<const T*>(x), w, static_cast<const T*>(dy), mean, rstd,

@@ -6,68 +6,20 @@
 // Without a tail r = 0: K = 1 is the cross entropy of one target. A slot with a negative column is unused; a row whose
 // teacher has no mass counts zero with a zero gradient.
 //
-// Rows are held in the shared memory of a cluster of 1 to 8 blocks (each a slice of the row, brought in by bulk copies) and
-// read there for the sums and again for the gradient, so a logit crosses HBM once, its gradient once: bound by HBM, beside
-// two exponentials a logit (16 lanes a clock). The named columns are taken out of the row first and written as -inf, so
-// that R is a sum of what it consists of, not a difference; named and other logits have maxima of their own, so a rest far
-// below the named ones keeps its value. The few scalars of a row's loss are formed in 64 bits: it is a small difference of
-// logarithms. Clusters walk the rows; a piece of the next row is requested as soon as the gradient pass has read the
-// present one out of it.
-#include <algorithm>
-
-#include "rows.cuh"
+// Rows are held in the shared memory of a cluster of 1 to 8 blocks (`row_slice.cuh`) and read there for the sums and again
+// for the gradient, so a logit crosses HBM once, its gradient once: bound by HBM, beside two exponentials a logit (16 lanes
+// a clock). The named columns are taken out of the row first and written as -inf, so that R is a sum of what it consists
+// of, not a difference, and relative to a logit that is in it: a rest far below the named logits keeps its value.
+// The teacher's side is a chain of dependent steps on K numbers, and so is a loss, formed in 64 bits because it is a small
+// difference of logarithms: a warp of its own does each, up to two rows ahead of the others and a row behind them.
+#include "row_slice.cuh"
 
 namespace {
 
 using namespace pd;
 
-constexpr int kMaxK = 256;
-constexpr int kMaxPieces = 32;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void store_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
-
-struct MaxSum {  // a maximum and the sum of exp((z - m) / T)
-  float m, s;
-};
-__device__ __forceinline__ MaxSum merge(const MaxSum& x, const MaxSum& y, float c) {
-  MaxSum r;
-  r.m = fmaxf(x.m, y.m);
-  // equal maxima, -inf on both sides among them, are not subtracted
-  r.s = x.s * (x.m == r.m ? 1.0f : ex2((x.m - r.m) * c)) + y.s * (y.m == r.m ? 1.0f : ex2((y.m - r.m) * c));
-  return r;
-}
-__device__ __forceinline__ MaxSum warp_merge(MaxSum t, float c) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    t = merge(t, MaxSum{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o)}, c);
-  return t;
-}
-
-// 16 bytes of shared memory as pairs of fp32.
-template <typename T>
-__device__ __forceinline__ void pairs_of(const uint4& q, f32x2 (&v)[8 / sizeof(T)]) {
-  if constexpr (sizeof(T) == 2) {
-    v[0] = unpack_bf16_2(q.x);
-    v[1] = unpack_bf16_2(q.y);
-    v[2] = unpack_bf16_2(q.z);
-    v[3] = unpack_bf16_2(q.w);
-  } else {
-    v[0] = pk2u(q.x, q.y);
-    v[1] = pk2u(q.z, q.w);
-  }
-}
+constexpr int kWarps = 8;  // that hold a row; as many threads as a row may have slots
+constexpr int kMaxK = 32 * kWarps;
 
 struct Call {
   const void* z;
@@ -87,324 +39,555 @@ struct Call {
   int* refused;
 };
 
+// A sum of exp(z / T) = 2^(c z) is kept as m, one of its z (the largest, or one that is not far below it), and s, the sum
+// relative to a power of two near that z's own term: 2^k, k = c m to the nearest whole number. One fused multiply-add then gives an exponent, c z - k, without the
+// rounding of c m in it, and a change of k is exact. (Where |c m| is so large that whole numbers are no closer than its
+// rounding, as for logits masked with the type's lowest value, s is relative to exp(m / T) itself.)
+struct MaxSum {
+  float m, s;
+};
+constexpr float kLargest = 1.0e6f;
+__device__ __forceinline__ float power_of(float m, float c) { return rintf(m * c); }
+__device__ __forceinline__ bool moderate(float m, float c) { return fabsf(m * c) < kLargest; }
+__device__ __forceinline__ float scaled(const MaxSum& x, float m, float c) {  // the sum as relative to m, not below x.m
+  if (x.m == m) return x.s;  // -inf on both sides among them
+  return x.s * ex2(moderate(x.m, c) && moderate(m, c) ? power_of(x.m, c) - power_of(m, c) : (x.m - m) * c);
+}
+// exp(z / T) as relative to m.
+__device__ __forceinline__ float term(float z, float m, float c) {
+  return ex2(moderate(m, c) ? fmaf(z, c, -power_of(m, c)) : (z - m) * c);
+}
+__device__ __forceinline__ MaxSum merge(const MaxSum& x, const MaxSum& y, float c) {
+  const float m = fmaxf(x.m, y.m);
+  return MaxSum{m, scaled(x, m, c) + scaled(y, m, c)};
+}
+// Logarithm of the sum, in 64 bits.
+__device__ __forceinline__ double log_of(const MaxSum& x, float c) {
+  const double at = moderate(x.m, c) ? power_of(x.m, c) : static_cast<double>(x.m) * c;
+  return at * 0.6931471805599453 + log(static_cast<double>(x.s));
+}
+
+struct Row {  // sums over a row: the columns that are not named, and those that are
+  MaxSum rest, top;
+};
+// Over the `n` (a power of two) neighbouring lanes.
+__device__ __forceinline__ Row merge_lanes(const Row& x, int n, float c) {
+  float m0 = x.rest.m, m1 = x.top.m;
+  for (int o = n / 2; o > 0; o >>= 1) {
+    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+  }
+  float s0 = scaled(x.rest, m0, c), s1 = scaled(x.top, m1, c);
+  for (int o = n / 2; o > 0; o >>= 1) {
+    s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+  }
+  return Row{{m0, s0}, {m1, s1}};
+}
+
+struct Teacher {  // of a row
+  int column[kMaxK];       // of the slots; -1 where a slot is unused, -2 - i where slot i has named the column already
+  float of_column[kMaxK];  // probability of the slot's column, over all slots that name it
+  float edge[16];          // elements at the row's ragged ends, named ones as -inf
+  float r, named;          // probability of the tail; of all slots
+  int row;                 // or -1: there is no further one
+  float top, total, tail;  // largest of the logits over T and the tail; sum of exponentials relative to it
+  bool live;
+};
+
+__device__ __forceinline__ float value_at(const Call& call, long long i) {
+  return call.values_fp32 ? static_cast<const float*>(call.values)[i]
+                          : as_float(static_cast<const __nv_bfloat16*>(call.values)[i]);
+}
+
+// One warp: the teacher's row, kPer slots a lane, and the row's ragged ends.
+template <typename T, int kPer>
+__device__ void prepare(const Call& call, const RowSlice<T>& rows, long long row, Teacher& t, int lane) {
+  const int K = call.K;
+  int col[kPer];
+  float v[kPer];
+  bool bad = false, nan = false;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int k = 32 * i + lane;
+    col[i] = -1;
+    v[i] = -INFINITY;
+    if (k < K) {
+      const long long at = row * K + k;
+      const long long c = call.wide ? static_cast<const long long*>(call.indices)[at] : static_cast<const int*>(call.indices)[at];
+      v[i] = value_at(call, at);
+      bad |= c >= call.V;
+      col[i] = c < 0 || c >= call.V ? -1 : static_cast<int>(c);
+    }
+  }
+  const float tail = call.tail != nullptr ? call.tail[row] : -INFINITY;  // already over T
+  const int shift = rows.shift(row);
+  int edge_col = -1;
+  const int edge_at = lane < 2 * RowSlice<T>::kE ? rows.edge_place(lane, shift, edge_col) : -1;
+  float edge = edge_at >= 0 && edge_col >= 0 && edge_col < call.V ? as_float(rows.row(row)[edge_col]) : -INFINITY;
+  if (bad) {
+    atomicCAS(call.status, 0, kBadColumn);
+    *static_cast<volatile int*>(call.refused) = 1;
+  }
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (col[i] < 0) v[i] = -INFINITY;
+    m = fmaxf(m, v[i]);
+    nan |= v[i] != v[i];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  nan = __any_sync(0xffffffffu, nan) || tail != tail;
+  const float inv_t = static_cast<float>(call.inv_t), over_t = m * inv_t, top = fmaxf(over_t, tail);
+  const bool live = nan || top > -INFINITY;
+  const float below = m > -INFINITY ? over_t - top : 0.0f;
+  float p[kPer], s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    p[i] = v[i] == -INFINITY ? 0.0f : expf((v[i] - m) * inv_t + below);
+    s += p[i];
+  }
+  s = warp_sum(s);
+  const float rest = tail == -INFINITY ? 0.0f : expf(tail - top), total = live ? s + rest : 1.0f, share = 1.0f / total;
+  // does a column come twice?
+  bool twice = false;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const unsigned same = __match_any_sync(0xffffffffu, col[i]);  // every lane, whether its slot is used or not
+    twice |= col[i] >= 0 && __popc(same) > 1;
+    if (32 * (i + 1) >= K) break;
+#pragma unroll 4
+    for (int o = 0; o < 32; ++o) {
+      const int other = __shfl_sync(0xffffffffu, col[i], lane + o);
+#pragma unroll
+      for (int j = i + 1; j < kPer; ++j) twice |= col[j] == other && other >= 0;
+    }
+  }
+  twice = __any_sync(0xffffffffu, twice);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int k = 32 * i + lane;
+    if (k < K) {
+      t.column[k] = col[i];
+      t.of_column[k] = p[i] * share;
+    }
+  }
+  __syncwarp();
+  if (twice) {
+    float sum[kPer];
+    int first[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int k = 32 * i + lane;
+      sum[i] = 0.0f;
+      first[i] = k;
+      if (k < K && col[i] >= 0)
+        for (int j = 0; j < K; ++j)
+          if (t.column[j] == col[i]) {
+            first[i] = min(first[i], j);
+            sum[i] += t.of_column[j];
+          }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (32 * i + lane < K) {
+        if (first[i] != 32 * i + lane) t.column[32 * i + lane] = -2 - first[i];
+        t.of_column[32 * i + lane] = sum[i];
+      }
+  }
+  if (edge_at >= 0)
+    for (int k = 0; k < K; ++k)
+      if (t.column[k] == edge_col) edge = -INFINITY;
+  if (lane < 2 * RowSlice<T>::kE) t.edge[lane] = edge;
+  if (lane == 0) {
+    t.r = live ? rest * share : 0.0f;
+    t.named = live ? s * share : 0.0f;
+    t.live = live;
+    t.top = top;
+    t.total = total;
+    t.tail = tail;
+  }
+}
+
+// One warp: the loss of a row. A logarithm of a sum is that of the sum as it stands: its rounding counts on both sides.
+__device__ float loss_of(const Call& call, long long row, const Teacher& t, const Row& sums, const float* named, float c,
+                         int lane) {
+  const MaxSum all = merge(sums.rest, sums.top, c);
+  const double inv_t = call.inv_t, own_inv_t = static_cast<double>(c) * 0.6931471805599453;  // the sums' own 1 / T
+  const double log_all = log_of(all, c), log_total = log(static_cast<double>(t.total));
+  double sum = 0.0;
+  for (int k0 = 0; k0 < call.K; k0 += 32) {
+    const int k = k0 + lane, column = k < call.K ? t.column[k] : -1;
+    if (column != -1) {
+      const double log_p = value_at(call, row * call.K + k) * inv_t - t.top - log_total;
+      const double log_q = named[column >= 0 ? k : -2 - column] * own_inv_t - log_all;
+      const float p = expf(static_cast<float>(log_p));
+      if (!(p == 0.0f)) sum += p * (log_p - log_q);
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (!(t.r == 0.0f)) {
+    const double log_r = static_cast<double>(t.tail) - t.top - log_total;
+    sum += t.r * (log_r - (log_of(sums.rest, c) - log_all));
+  }
+  return t.live ? static_cast<float>(sum) : 0.0f;
+}
+
+// One object: the address of its barriers goes to inline assembly, so the compiler takes every wait and barrier there for
+// one that may change any part of it.
+struct Shared {
+  RowQueue queue;
+  unsigned long long bars[kWarps + 7];
+  Teacher teacher[3];
+  float named[3][kMaxK];  // student's logits at the columns, in the slots that speak for them
+  Row red[kWarps], xch[3][8], sums[2];
+  float2 part[kWarps];
+  int next;  // the row behind the present one, or -1
+  int rows;  // this cluster has had, once there is no further one
+  int abort_flag;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(512) top_kl_kernel(const Call call, int slice, int cs) {
-  constexpr int kE = 16 / sizeof(T), kP = kE / 2;
+__global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call call, const SlicePlan plan) {
+  constexpr int kE = RowSlice<T>::kE, kP = kE / 2;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) unsigned long long bars[kMaxPieces];
-  __shared__ MaxSum red[16], xch[2][8];
-  __shared__ float named[2][kMaxK];  // student's logits at the columns, in the slots that speak for them
-  __shared__ int column[kMaxK], owner[kMaxK];
-  __shared__ float prob[kMaxK], prob_of_column[kMaxK];
-  __shared__ float teacher[3];  // r, sum of p, 0 or 1: the row counts
-  __shared__ double teacher_log[3];  // maximum (over T), log of the sum, log r
-  __shared__ int abort_flag;
-  const int tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = nt >> 5;
+  __shared__ __align__(16) Shared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cs = plan.cs, warps = kWarps, nt = 32 * kWarps;
   const int rank = cs > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int V = call.V, K = call.K, g0 = rank * slice, pieces = (slice + nt - 1) / nt;
   const float c = static_cast<float>(call.inv_t * 1.4426950408889634);
-  const T* z = static_cast<const T*>(call.z);
+  const RowSlice<T> rows{static_cast<const T*>(call.z), call.ld, call.V, rank * plan.slice, plan.slice, plan.per};
   T* buf = reinterpret_cast<T*>(smem);
-  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t bar0 = smem_u32(sh.bars), ready = bar0 + 8 * kWarps, summed = ready + 16, lost = ready + 32, met = ready + 48;
   if (tid == 0) {
-    for (int i = 0; i < pieces; ++i) mbar_init(bar0 + 8 * i, 1);
-    abort_flag = 0;
+    for (int i = 0; i < warps; ++i) mbar_init(bar0 + 8 * i, 1);
+    for (int i = 0; i < 6; ++i) mbar_init(ready + 8 * i, 1);
+    mbar_init(met, cs);
+    sh.rows = -1;
+    sh.queue.init();
+    sh.abort_flag = 0;
     mbar_fence_init();
   }
   __syncthreads();
-  auto shift_of = [&](long long row) {
-    return static_cast<int>((reinterpret_cast<uintptr_t>(z + row * call.ld) & 15) / sizeof(T));
-  };
-  // Groups of 16 bytes at 16-byte addresses: those that lie in the row whole come by bulk copy, its ragged ends by loads.
-  auto request = [&](long long row, int piece) {  // one thread; nothing new once a wait has run out
-    if (*static_cast<volatile int*>(&abort_flag)) return;
-    const int shift = shift_of(row);
-    const int first = max(g0 + piece * nt, shift > 0 ? 1 : 0);
-    const int stop = min(g0 + min((piece + 1) * nt, slice), (shift + V) / kE);
-    const uint32_t bytes = stop > first ? 16u * (stop - first) : 0u;
-    mbar_expect_tx(bar0 + 8 * piece, bytes);
-    if (bytes > 0)
-      bulk_load(smem_u32(smem + 16ll * (first - g0)), z + row * call.ld - shift + static_cast<long long>(first) * kE, bytes,
-                bar0 + 8 * piece);
-  };
-  const long long first_row = blockIdx.x / cs, step = gridDim.x / cs;
-  if (tid == 0 && first_row < call.rows)
-    for (int i = 0; i < pieces; ++i) request(first_row, i);
   if (cs > 1) cluster_sync_all();  // every block of the cluster runs before another one stores to its shared memory
-  int turn = 0;
-  for (long long row = first_row; row < call.rows; row += step, ++turn) {
-    const int shift = shift_of(row), half = turn & 1;
-    const int groups = min(slice, max(0, (shift + V + kE - 1) / kE - g0));
-    const T* zr = z + row * call.ld;
-    // the ragged ends: thread j < kE an element of the row's first group, the next kE one of its last
-    int end_at = -1;
-    T end_value{};
-    if (tid < 2 * kE) {
-      const int g = tid < kE ? 0 : (shift + V) / kE, at = g * kE + tid % kE, col = at - shift;
-      const bool ragged = tid < kE ? shift > 0 : (shift + V) % kE != 0;
-      if (ragged && g >= g0 && g < g0 + groups) {
-        end_at = at - g0 * kE;
-        if (col >= 0 && col < V)
-          end_value = zr[col];
-        else
-          store1(&end_value, -INFINITY);
+  auto late = [&](bool in_time) {
+    if (!in_time && call.status != nullptr) atomicCAS(call.status, 0, kTimeoutProducer);
+  };
+  // The n-th completion of a pair of barriers that take turns: one that is waited for late is not mistaken for the next.
+  auto wait_pair = [&](uint32_t pair, int n) { return short_wait<false>(pair + 8 * (n & 1), (n >> 1) & 1, &sh.abort_flag); };
+  const bool losses = rank == 0 && call.loss != nullptr;
+  if (warp == warps) {  // the teacher's side, up to two rows ahead
+    auto teach = [&](int row, int n) {
+      Teacher& t = sh.teacher[n % 3];
+      if (row < 0) {
+      } else if (call.K <= 32) {
+        prepare<T, 1>(call, rows, row, t, lane);
+      } else if (call.K <= 64) {
+        prepare<T, 2>(call, rows, row, t, lane);
+      } else {
+        prepare<T, kMaxK / 32>(call, rows, row, t, lane);
       }
+      t.row = row;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ready + 8 * (n & 1));
+      __syncwarp();
+    };
+    // The n-th row, while the one after it is asked for.
+    bool more = true;
+    auto next = [&](int n) {
+      if (!more) return -1;
+      bool in_time = true;
+      const int row = sh.queue.take(n, rank, cs, lane, &sh.abort_flag, in_time);
+      late(in_time);
+      more = row >= 0;
+      if (more && rank == 0 && lane == 0) sh.queue.ask();
+      __syncwarp();
+      return row;
+    };
+    if (rank == 0 && lane == 0) sh.queue.ask();
+    __syncwarp();
+    teach(blockIdx.x / cs, 0);
+    teach(next(1), 1);
+    int ahead = next(2);
+    for (int n = 0; sh.teacher[n % 3].row >= 0; ++n) {
+      late(wait_pair(summed, n));  // the others are done with the row before,
+      if (losses && n > 0) late(wait_pair(lost, n - 1));  // and so is the warp below
+      teach(ahead, n + 2);
+      ahead = next(n + 3);
     }
-    // the teacher's distribution, while the row is on its way
-    if (tid < K) {
-      long long i = call.wide ? static_cast<const long long*>(call.indices)[row * K + tid]
-                              : static_cast<const int*>(call.indices)[row * K + tid];
-      const float t = call.values_fp32 ? static_cast<const float*>(call.values)[row * K + tid]
-                                       : as_float(static_cast<const __nv_bfloat16*>(call.values)[row * K + tid]);
-      if (i >= V) {
-        atomicCAS(call.status, 0, kBadColumn);
-        *static_cast<volatile int*>(call.refused) = 1;
-        i = -1;
-      }
-      column[tid] = i < 0 ? -1 : static_cast<int>(i);
-      prob[tid] = i < 0 ? -INFINITY : t;
-    }
-    __syncthreads();
-    if (warp == 0) {
-      const float tl = call.tail != nullptr ? call.tail[row] : -INFINITY;  // already over T
-      float m = -INFINITY;
-      bool nan = tl != tl;
-      for (int k = lane; k < K; k += 32) {
-        m = fmaxf(m, prob[k]);
-        nan |= prob[k] != prob[k];
-      }
-      nan = __any_sync(0xffffffffu, nan);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const double top = fmax(static_cast<double>(m) * call.inv_t, static_cast<double>(tl));
-      float s = 0.0f;
-      for (int k = lane; k < K; k += 32) s += expf(static_cast<float>(prob[k] * call.inv_t - top));
-      s = warp_sum(s);
-      const float rest = expf(static_cast<float>(tl - top)), total = s + rest;
+  } else if (warp == warps + 1) {  // losses, a row behind
+    // What a loss reads is written again three rows on, by whichever block, and not before the teacher of that row is
+    // there, which waits for this warp.
+    for (int n = 0; losses; ++n) {
+      late(wait_pair(summed, n));
+      if (n == *static_cast<volatile int*>(&sh.rows) || *static_cast<volatile int*>(&sh.abort_flag)) break;
+      const Teacher& t = sh.teacher[n % 3];
+      const float loss = loss_of(call, t.row, t, sh.sums[n & 1], sh.named[n % 3], c, lane);
       if (lane == 0) {
-        const bool live = nan || top > -INFINITY;
-        teacher[0] = live ? rest / total : 0.0f;
-        teacher[1] = live ? s / total : 0.0f;
-        teacher[2] = live ? 1.0f : 0.0f;
-        teacher_log[0] = top;
-        teacher_log[1] = log(static_cast<double>(total));
-        teacher_log[2] = tl - top - teacher_log[1];
+        call.loss[t.row] = loss;
+        mbar_arrive(lost + 8 * (n & 1));
       }
+      __syncwarp();
     }
-    __syncthreads();
-    // Every slot learns which slot speaks for its column (the first that names it) and the column's whole probability.
-    const bool live = teacher[2] != 0.0f;
-    if (tid < K) {
-      const double top = teacher_log[0], log_total = teacher_log[1];
-      const int mine = column[tid];
-      int speaker = tid;
-      float p = 0.0f;
-      if (mine >= 0 && live)
-        for (int k = 0; k < K; ++k)
-          if (column[k] == mine) {
-            speaker = min(speaker, k);
-            p += expf(static_cast<float>(prob[k] * call.inv_t - top - log_total));
+  } else {
+    if (lane == 0) rows.request(blockIdx.x / cs, warp, smem, bar0 + 8 * warp, false);
+    __syncwarp();
+    late(wait_pair(ready, 0));
+    const uint32_t per_inverse = plan.per > 1 ? 0xFFFFFFFFu / plan.per + 1 : 0;  // x / per = x per_inverse >> 32, x per < 2^32
+    int n = 0;
+    for (int row = blockIdx.x / cs; row >= 0; ++n) {
+      const Teacher& t = sh.teacher[n % 3];
+      const int shift = rows.shift(row), groups = rows.groups(shift);
+      const int begin = warp * plan.per + lane, stop = min(groups, (warp + 1) * plan.per);
+      float* zk = sh.named[n % 3];
+      const float up =  // on its way while the row is waited for
+          (call.scale != nullptr ? call.scale[row] : 1.0f) * static_cast<float>(call.inv_t);
+      late(short_wait<false>(bar0 + 8 * warp, n & 1, &sh.abort_flag));
+      if (tid < 2 * kE) {
+        int col;
+        const int at = rows.edge_place(tid, shift, col);
+        if (at >= 0) store1(buf + at, t.edge[tid]);
+      }
+      // Named columns leave the row: their logits go to every block of the cluster.
+      int mine = -1;  // the column whose gradient this thread writes
+      float mine_logit = 0.0f;
+      if (tid < call.K && t.column[tid] >= 0 && t.column[tid] < call.V) {
+        const int place = shift + t.column[tid], g = place / kE, at = place - rows.g0 * kE;
+        if (at >= 0 && at < groups * kE) {
+          mine = t.column[tid];
+          if (g >= rows.whole_first(shift) && g < rows.whole_stop(shift)) {
+            const uint32_t x = g - rows.g0, holder = plan.per > 1 ? __umulhi(x, per_inverse) : x;  // the warp that holds it
+            late(short_wait<false>(bar0 + 8 * holder, n & 1, &sh.abort_flag));
+            mine_logit = as_float(buf[at]);
+            store1(buf + at, -INFINITY);
+          } else {
+            mine_logit = as_float(rows.row(row)[mine]);  // at a ragged end, which is already without it
           }
-      owner[tid] = speaker;
-      prob_of_column[tid] = p;
-    }
-    for (int i = 0; i < pieces; ++i)
-      if (!mbar_wait(bar0 + 8 * i, turn & 1, &abort_flag) && call.status != nullptr)
-        atomicCAS(call.status, 0, kTimeoutProducer);
-    if (end_at >= 0) buf[end_at] = end_value;
-    __syncthreads();
-    // Named columns leave the row: their logits go to every block of the cluster.
-    const int at = tid < K && column[tid] >= 0 && owner[tid] == tid ? shift + column[tid] - g0 * kE : -1;
-    const bool here = at >= 0 && at < groups * kE;
-    if (here) {
-      const float v = as_float(buf[at]);
-      const uint32_t local = smem_u32(&named[half][tid]);
-      if (cs > 1)
-        for (int b = 0; b < cs; ++b) store_cluster_f32(mapa_shared(local, b), v);
-      else
-        named[half][tid] = v;
-      store1(buf + at, -INFINITY);
-    }
-    fence_proxy_async_smem();  // before the next row's bulk copies write where this row's ends and marks are
-    __syncthreads();
-    float m = -INFINITY;
-    for (int g = tid; g < groups; g += nt) {
-      f32x2 v[kP];
-      pairs_of<T>(*reinterpret_cast<const uint4*>(smem + 16 * g), v);
-#pragma unroll
-      for (int j = 0; j < kP; ++j) {
-        const float2 x = unpack2(v[j]);
-        m = fmaxf(m, fmaxf(x.x, x.y));
-      }
-    }
-    MaxSum t{m, 0.0f};
-    if (m > -INFINITY) {
-      const f32x2 neg = pk2(-m, -m), c2 = pk2(c, c);
-      f32x2 s = 0ull;
-      for (int g = tid; g < groups; g += nt) {
-        f32x2 v[kP];
-        pairs_of<T>(*reinterpret_cast<const uint4*>(smem + 16 * g), v);
-#pragma unroll
-        for (int j = 0; j < kP; ++j) {
-          const float2 x = unpack2(mul2(add2(v[j], neg), c2));
-          s = add2(s, pk2(ex2(x.x), ex2(x.y)));
+          const uint32_t local = smem_u32(zk + tid);
+          if (cs > 1)
+            for (int b = 0; b < cs; ++b) store_cluster_f32(mapa_shared(local, b), mine_logit);
+          else
+            zk[tid] = mine_logit;
         }
       }
-      const float2 s2 = unpack2(s);
-      t.s = s2.x + s2.y;
-    }
-    t = warp_merge(t, c);
-    if (lane == 0) red[warp] = t;
-    __syncthreads();
-    if (warp == 0) {
-      t = lane < warps ? red[lane] : MaxSum{-INFINITY, 0.0f};
-      t = warp_merge(t, c);
-      if (lane < cs) {
-        const uint32_t local = smem_u32(&xch[half][rank]);
-        const uint32_t to = cs > 1 ? mapa_shared(local, lane) : local;
-        store_cluster_f32(to, t.m);
-        store_cluster_f32(to + 4, t.s);
-      }
-    }
-    if (cs > 1)
-      cluster_sync_all();
-    else
-      __syncthreads();
-    MaxSum rest = xch[half][0];
-    for (int b = 1; b < cs; ++b) rest = merge(rest, xch[half][b], c);
-    MaxSum top{-INFINITY, 0.0f};  // of the named columns; every warp forms it for itself
-    for (int k = lane; k < K; k += 32)
-      if (column[k] >= 0 && owner[k] == k) top = merge(top, MaxSum{named[half][k], 1.0f}, c);
-    top = warp_merge(top, c);
-    const MaxSum all = merge(rest, top, c);
-    const float r = teacher[0], p_named = teacher[1];
-    if (warp == 0 && rank == 0 && call.loss != nullptr) {
-      const double log_all = log(static_cast<double>(all.s)), inv_t = call.inv_t;
-      double sum = 0.0;
-      for (int k = lane; k < K; k += 32) {
-        if (column[k] < 0) continue;
-        const double log_p = prob[k] * inv_t - teacher_log[0] - teacher_log[1];
-        const double log_q = (static_cast<double>(named[half][owner[k]]) - all.m) * inv_t - log_all;
-        const float p = expf(static_cast<float>(log_p));
-        if (!(p == 0.0f)) sum += p * (log_p - log_q);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) {
-        if (!(r == 0.0f)) {
-          const double log_rest = (static_cast<double>(rest.m) - all.m) * inv_t + log(static_cast<double>(rest.s)) - log_all;
-          sum += r * (teacher_log[2] - log_rest);
-        }
-        call.loss[row] = live ? static_cast<float>(sum) : 0.0f;
-      }
-    }
-    const bool more = row + step < call.rows;
-    if (call.dz != nullptr) {
-      const float up = (call.scale != nullptr ? call.scale[row] : 1.0f) * static_cast<float>(call.inv_t);
-      // q of the named columns and of the rest; the difference R - r from whichever side is small
-      const float q_top = top.s * (top.m == all.m ? 1.0f : ex2((top.m - all.m) * c)) / all.s;
-      const float q_rest = rest.s * (rest.m == all.m ? 1.0f : ex2((rest.m - all.m) * c)) / all.s;
-      const float gap = r > 0.5f ? p_named - q_top : q_rest - r;
-      const float f = live && rest.s > 0.0f ? gap / rest.s * up : (rest.s == rest.s ? 0.0f : rest.s);
-      const float ref = rest.m > -INFINITY ? rest.m : 0.0f;
-      const f32x2 neg = pk2(-ref, -ref), c2 = pk2(c, c), f2 = pk2(f, f);
-      T* out = static_cast<T*>(call.dz) + row * call.ldo;
-      for (int i = 0; i < pieces; ++i) {
-        const int g = i * nt + tid;
-        if (g < groups) {
+      fence_proxy_async_smem();  // before bulk copies of the next row write where this row's ends and marks are
+      sync_first(nt);
+      // The slice's sums relative to one of its own logits: they serve as they are unless another one is larger by 2^100.
+      GroupMax<T> gm;
+      if (groups > 0) gm.add(*reinterpret_cast<const uint4*>(smem));
+      if (groups > 1) gm.add(*reinterpret_cast<const uint4*>(smem + 16));
+      const float ref = gm.value();
+      const f32x2 c2 = pk2(c, c);
+      auto add_up = [&](auto exponent) {  // of a pair of logits
+        f32x2 s0 = 0ull, s1 = 0ull;
+#pragma unroll 4
+        for (int g = begin; g < stop; g += 32) {
           f32x2 v[kP];
           pairs_of<T>(*reinterpret_cast<const uint4*>(smem + 16 * g), v);
 #pragma unroll
           for (int j = 0; j < kP; ++j) {
-            const float2 x = unpack2(mul2(add2(v[j], neg), c2));
-            v[j] = live ? mul2(pk2(ex2(x.x), ex2(x.y)), f2) : 0ull;
-          }
-          const int col = (g0 + g) * kE - shift;
-          if (col >= 0 && col + kE <= V) {
-            uint4 q;
-            if constexpr (sizeof(T) == 2) {
-              q = make_uint4(pack_bf16_2(v[0]), pack_bf16_2(v[1]), pack_bf16_2(v[2]), pack_bf16_2(v[3]));
-            } else {
-              const float2 a = unpack2(v[0]), b = unpack2(v[1]);
-              q = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
-            }
-            *reinterpret_cast<uint4*>(out + col) = q;
-          } else {
-#pragma unroll
-            for (int j = 0; j < kP; ++j) {
-              const float2 a = unpack2(v[j]);
-              if (col + 2 * j >= 0 && col + 2 * j < V) store1(out + col + 2 * j, a.x);
-              if (col + 2 * j + 1 >= 0 && col + 2 * j + 1 < V) store1(out + col + 2 * j + 1, a.y);
-            }
+            const float2 x = unpack2(exponent(v[j]));
+            const f32x2 e = pk2(ex2(x.x), ex2(x.y));
+            if (j & 1)
+              s1 = add2(s1, e);
+            else
+              s0 = add2(s0, e);
           }
         }
-        __syncthreads();  // the piece has been read; behind the last one, the row's stores are in order before the named
-        if (more && tid == 0) request(row + step, i);
+        const float2 a = unpack2(add2(s0, s1));
+        return a.x + a.y;
+      };
+      float2 part = make_float2(INFINITY, 0.0f);
+      if (moderate(ref, c)) {
+        const float k = -power_of(ref, c);
+        const f32x2 k2 = pk2(k, k);
+        part = make_float2(add_up([&](f32x2 v) { return fma2(v, c2, k2); }), mine >= 0 ? term(mine_logit, ref, c) : 0.0f);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          part.x += __shfl_xor_sync(0xffffffffu, part.x, o);
+          part.y += __shfl_xor_sync(0xffffffffu, part.y, o);
+        }
       }
-      if (here) {
-        const float q = ex2((named[half][tid] - all.m) * c) / all.s;
-        store1(out + column[tid], live ? (q - prob_of_column[tid]) * up : 0.0f);
+      if (lane == 0) sh.part[warp] = part;
+      if (tid == 0) {  // all warps go on together, or none does: what the barrier below shows them decides
+        late(wait_pair(ready, n + 1));
+        sh.next = *static_cast<volatile int*>(&sh.abort_flag) ? -1 : sh.teacher[(n + 1) % 3].row;
       }
-      __syncthreads();  // before the next row's slots overwrite this one's
-    } else {
-      __syncthreads();
-      if (more && tid == 0)
-        for (int i = 0; i < pieces; ++i) request(row + step, i);
+      sync_first(nt);
+      const int next = sh.next;
+      part = sh.part[lane & 7];
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        part.x += __shfl_xor_sync(0xffffffffu, part.x, o);
+        part.y += __shfl_xor_sync(0xffffffffu, part.y, o);
+      }
+      Row sums{{ref, part.x}, {ref, part.y}};
+      if (!(part.x < 1e30f && part.y < 1e30f)) {  // the same in every thread: sums relative to true maxima
+        GroupMax<T> all;
+        for (int g = begin; g < stop; g += 32) all.add(*reinterpret_cast<const uint4*>(smem + 16 * g));
+        const float own = all.value();
+        sums = Row{{own, 0.0f}, {-INFINITY, 0.0f}};
+        if (mine >= 0 && mine_logit > -INFINITY) sums.top = MaxSum{mine_logit, term(mine_logit, mine_logit, c)};
+        if (moderate(own, c)) {
+          const float k = -power_of(own, c);
+          const f32x2 k2 = pk2(k, k);
+          sums.rest.s = add_up([&](f32x2 v) { return fma2(v, c2, k2); });
+        } else if (own > -INFINITY) {
+          const f32x2 neg = pk2(-own, -own);
+          sums.rest.s = add_up([&](f32x2 v) { return mul2(add2(v, neg), c2); });
+        }
+        sums = merge_lanes(sums, 32, c);
+        if (lane == 0) sh.red[warp] = sums;
+        sync_first(nt);
+        sums = merge_lanes(sh.red[lane & 7], 8, c);
+      }
+      if (cs > 1) {
+        if (warp == 0 && lane < cs) {
+          const uint32_t to = mapa_shared(smem_u32(&sh.xch[n % 3][rank]), lane);
+          store_cluster_f32(to, sums.rest.m);
+          store_cluster_f32(to + 4, sums.rest.s);
+          store_cluster_f32(to + 8, sums.top.m);
+          store_cluster_f32(to + 12, sums.top.s);
+          mbar_arrive_cluster(mapa_shared(met, lane));  // with it, the named logits that were stored before the barriers
+        }
+        __syncwarp();
+        late(short_wait<true>(met, n & 1, &sh.abort_flag));
+        const Row none{{-INFINITY, 0.0f}, {-INFINITY, 0.0f}};
+        sums = (lane & 7) < cs ? sh.xch[n % 3][lane & 7] : none;
+        sums = merge_lanes(sums, 8, c);
+      }
+      if (tid == 0) {
+        sh.sums[n & 1] = sums;
+        mbar_arrive(summed + 8 * (n & 1));
+      }
+      __syncwarp();
+      auto ask_for_next = [&] {  // the warp's part of it
+        __syncwarp();
+        if (lane == 0 && next >= 0) {
+          fence_proxy_async_smem();
+          rows.request(next, warp, smem, bar0 + 8 * warp, false);
+        }
+        __syncwarp();
+      };
+      if (call.dz != nullptr) {
+        const MaxSum all = merge(sums.rest, sums.top, c), rest = sums.rest;
+        const bool live = t.live;
+        // the difference R - r from whichever side is small
+        const float gap = t.r > 0.5f ? t.named - scaled(sums.top, all.m, c) / all.s : scaled(rest, all.m, c) / all.s - t.r;
+        float f = rest.s == 0.0f ? 0.0f : gap / rest.s * up;  // of an exponential as relative to rest.m
+        T* const out = static_cast<T*>(call.dz) + static_cast<long long>(row) * call.ldo;  // column 0
+        T* const slice_out = out + (rows.g0 * kE - shift);
+        const int inner_first = rows.whole_first(shift) - rows.g0, inner_stop = rows.whole_stop(shift) - rows.g0;
+        auto put = [&](auto gradient) {  // words of gradients from words of the row
+          auto ragged = [&](int g) {
+            const uint4 q = gradient(*reinterpret_cast<const uint4*>(smem + 16 * g));
+            const T* each = reinterpret_cast<const T*>(&q);
+            const int col = (rows.g0 + g) * kE - shift;
+#pragma unroll
+            for (int j = 0; j < kE; ++j)
+              if (col + j >= 0 && col + j < call.V) out[col + j] = each[j];
+          };
+          int g = begin;
+          if (g < inner_first && g < stop) {  // no more than the row's first group
+            ragged(g);
+            g += 32;
+          }
+          const int inner = min(stop, inner_stop);
+          uint4* to = reinterpret_cast<uint4*>(slice_out + g * kE);
+#pragma unroll 4
+          for (; g < inner; g += 32, to += 32) *to = gradient(*reinterpret_cast<const uint4*>(smem + 16 * g));
+          if (g < stop) ragged(g);  // no more than its last
+        };
+        if (!live || f == 0.0f) {
+          put([&](const uint4&) { return make_uint4(0u, 0u, 0u, 0u); });
+        } else if constexpr (sizeof(T) == 4) {
+          const float k = moderate(rest.m, c) ? -power_of(rest.m, c) : 0.0f;
+          const f32x2 k2 = pk2(k, k), neg = pk2(-rest.m, -rest.m), f2 = pk2(f, f);
+          auto words = [&](const uint4& w, auto exponent) {
+            f32x2 v[kP];
+            pairs_of<T>(w, v);
+#pragma unroll
+            for (int j = 0; j < kP; ++j) {
+              const float2 x = unpack2(exponent(v[j])), e = unpack2(mul2(pk2(ex2(x.x), ex2(x.y)), f2));
+              v[j] = pk2(e.x, e.y);
+            }
+            const float2 a = unpack2(v[0]), b = unpack2(v[1]);
+            return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+          };
+          if (moderate(rest.m, c))
+            put([&](const uint4& w) { return words(w, [&](f32x2 v) { return fma2(v, c2, k2); }); });
+          else
+            put([&](const uint4& w) { return words(w, [&](f32x2 v) { return mul2(add2(v, neg), c2); }); });
+        } else {
+          // f goes into the exponent, its sign into the word: what the exponent's rounding costs (below 2^-18 of the value)
+          // is far below the result's half step
+          const float lf = log2f(fabsf(f)), k = moderate(rest.m, c) ? lf - power_of(rest.m, c) : 0.0f;
+          const f32x2 k2 = pk2(k, k), neg = pk2(-rest.m, -rest.m), lf2 = pk2(lf, lf);
+          const uint32_t sign = f < 0.0f ? 0x80008000u : 0u;
+          auto words = [&](const uint4& w, auto exponent) {
+            f32x2 v[kP];
+            pairs_of<T>(w, v);
+            uint32_t o[kP];
+#pragma unroll
+            for (int j = 0; j < kP; ++j) {
+              const float2 x = unpack2(exponent(v[j]));
+              o[j] = pack_bf16_2(pk2(ex2(x.x), ex2(x.y))) ^ sign;
+            }
+            return make_uint4(o[0], o[1], o[2], o[3]);
+          };
+          if (moderate(rest.m, c))
+            put([&](const uint4& w) { return words(w, [&](f32x2 v) { return fma2(v, c2, k2); }); });
+          else
+            put([&](const uint4& w) { return words(w, [&](f32x2 v) { return fma2(add2(v, neg), c2, lf2); }); });
+        }
+        ask_for_next();
+        sync_first(nt);  // the row's stores are in order before those of the named columns
+        if (mine >= 0) {
+          const float q = term(zk[tid], all.m, c) / all.s;
+          store1(out + mine, live ? (q - t.of_column[tid]) * up : 0.0f);
+        }
+      } else {
+        ask_for_next();
+      }
+      row = next;
+    }
+    if (tid == 0) {
+      *static_cast<volatile int*>(&sh.rows) = n;
+      mbar_arrive(summed + 8 * (n & 1));
     }
   }
+  __syncwarp();
+  if (cs > 1) cluster_sync_all();  // no block leaves while another one may still store to it
 }
 
-// Slices (16-byte groups a block) and the cluster that holds a row of V columns; 0 where none does.
-struct Plan {
-  int cs, slice;
-};
-template <typename T>
-Plan plan_for(long long V) {
-  // the smallest cluster that leaves room for two blocks an SM; past that, up to one block an SM
-  constexpr long long kHalfSm = 104 * 1024, kWholeSm = 216 * 1024, kE = 16 / sizeof(T);
-  const long long groups = (V + 2 * kE - 2) / kE;  // wherever a row starts
-  int cs = 1;
-  while (cs < 8 && (groups + cs - 1) / cs * 16 > kHalfSm) cs *= 2;
-  const long long slice = (groups + cs - 1) / cs;
-  return slice * 16 > kWholeSm ? Plan{0, 0} : Plan{cs, static_cast<int>(slice)};
-}
+// Beside a slice, 10 KB of fixed shared memory and 1 KB of the system's: two blocks an SM, or one.
+constexpr long long kHalfSm = 102 * 1024, kWholeSm = 216 * 1024;
 
 template <typename T>
 int launch(const Call& call, cudaStream_t st) {
-  const Plan plan = plan_for<T>(call.V);
+  const SlicePlan plan = slice_plan<T>(call.V, kWarps, kHalfSm, kWholeSm);
   if (plan.cs == 0) return 5;
-  const int smem = plan.slice * 16;
-  // short rows: fewer threads, so that every thread has a group and more rows share an SM; a slot needs a thread
-  const int nt = plan.slice >= 1024 ? 512 : 256;
+  const int smem = plan.slice * 16, threads = 32 * (kWarps + 2);
   auto kern = top_kl_kernel<T>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024) != cudaSuccess) return 2;
-  const int per_sm = std::max(1, std::min(1024 / nt, 227 * 1024 / (smem + 8 * 1024)));
-  const long long clusters = std::min<long long>(call.rows, std::max(1, 148 * per_sm / plan.cs));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(clusters * plan.cs));
-  cfg.blockDim = dim3(nt);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = plan.cs;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, call, plan.slice, plan.cs);
-  return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : 1;
+  static bool sized = false;  // the same answer whoever asks first
+  if (!sized && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kWholeSm) != cudaSuccess) return 2;
+  sized = true;
+  return launch_clusters(kern, call.rows, plan.cs, threads, smem, st, call, plan);
 }
 
 }  // namespace
 
 // Widest row that a cluster holds.
-extern "C" long long pd_top_kl_max_columns(int z_fp32) { return 8ll * 216 * 1024 / (z_fp32 ? 4 : 2) - 16; }
+extern "C" long long pd_top_kl_max_columns(int z_fp32) { return 8 * kWholeSm / (z_fp32 ? 4 : 2) - 16; }
 
 extern "C" int pd_top_kl(const void* z, long long rows, int V, long long ld, const void* indices, int wide,
                          const void* values, int values_fp32, int K, const float* tail, double inv_t, float* loss, void* dz,
                          long long ldo, const float* scale, int z_fp32, int* status, int* refused, void* stream) {
-  if (rows <= 0 || V <= 0 || K <= 0 || K > kMaxK || !(inv_t > 0.0)) return 5;
+  if (rows <= 0 || rows >= (1ll << 28) || V <= 0 || K <= 0 || K > kMaxK || !(inv_t > 0.0)) return 5;
   const Call call{z, rows, ld, V, indices, wide, values, values_fp32, K, tail, inv_t, loss, dz, ldo, scale, status, refused};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return z_fp32 ? launch<float>(call, st) : launch<__nv_bfloat16>(call, st);

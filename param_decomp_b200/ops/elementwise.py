@@ -3,12 +3,14 @@
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 
 import torch
 from torch import Tensor
 
 from param_decomp_b200.ops import native as nv
 
+_FLOAT = (torch.bfloat16, torch.float32)
 _configured = False
 
 
@@ -29,6 +31,9 @@ def _lib():
         lib.pd_swiglu_bwd.argtypes = [P, P, P, P, P, LL, P]
         lib.pd_rowscale.argtypes = [P, P, P, LL, I, P]
         lib.pd_ci_squash.argtypes = [P, P, P, LL, F, P]
+        lib.pd_layer_norm_partial_rows.argtypes = [LL, I]
+        lib.pd_layer_norm_fwd.argtypes = [P, P, P, P, P, P, LL, I, F, I, I, P]
+        lib.pd_layer_norm_bwd.argtypes = [P, P, P, P, P, P, P, P, P, LL, I, I, I, P]
         _configured = True
     return lib
 
@@ -158,65 +163,83 @@ def rms_norm(x: Tensor, w: Tensor | None, eps: float) -> Tensor:
 
 def _on_current_device(what: str, *tensors: Tensor | None) -> None:
     """Kernels launch on the current device's stream: a tensor that lies elsewhere is refused."""
+    current = -1
     for t in tensors:
-        if t is not None and not t.is_cuda:
+        if t is None:
+            continue
+        where = t.get_device()
+        if where < 0:
             raise nv.NativeError(f"{what}: a tensor on {t.device}: the kernels run on a GPU")
-        if t is not None and t.device.index != torch._C._cuda_getDevice():
-            raise nv.NativeError(f"{what}: a tensor on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+        if current < 0:
+            current = torch._C._cuda_getDevice()
+        if where != current:
+            raise nv.NativeError(f"{what}: a tensor on {t.device}, the current device is cuda:{current}")
 
 
 def _dense(t: Tensor) -> Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _flat_rows(t: Tensor, columns: int) -> Tensor:
+    """`[rows, columns]`, contiguous."""
+    t = t if t.dim() == 2 else t.reshape(-1, columns)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+LAYER_NORM_MAX_COLUMNS = 12288
+_layer_norm_partial_rows = lru_cache(maxsize=256)(lambda rows, d: _lib().pd_layer_norm_partial_rows(rows, d))
+
+
+def _layer_norm_fwd(x: Tensor, w: Tensor | None, b: Tensor | None, eps: float, stats: Tensor | None) -> Tensor:
+    """`x [rows, d]` -> y; `stats [2, rows]` (or None) receives the rows' means and reciprocal deviations."""
+    rows, d = x.shape
+    y = torch.empty_like(x)
+    if rows > 0:
+        at = None if stats is None else stats.data_ptr()
+        p = w if w is not None else b
+        _check(_lib().pd_layer_norm_fwd(x.data_ptr(), None if w is None else w.data_ptr(), None if b is None else b.data_ptr(),
+                                        y.data_ptr(), at, None if at is None else at + 4 * rows, rows, d, eps,
+                                        x.dtype is torch.float32, p is not None and p.dtype is torch.float32, _s()),
+               "layer_norm_fwd")
+    return y
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Tensor:  # type: ignore[override]
-        d = x.shape[-1]
-        x2 = _dense(x.reshape(-1, d))
-        w, b = (None if p is None else _dense(p) for p in (w, b))
-        p_fp32 = any(p is not None and p.dtype == torch.float32 for p in (w, b))
-        rows = x2.shape[0]
-        y = torch.empty_like(x2)
-        stats = torch.empty(2, rows, device=x.device, dtype=torch.float32) if any(ctx.needs_input_grad) else None
-        if rows > 0:
-            lib = _lib()
-            lib.pd_layer_norm_fwd.argtypes = [C.c_void_p] * 6 + [C.c_longlong, C.c_int, C.c_float, C.c_int, C.c_int, C.c_void_p]
-            mean, rstd = (None, None) if stats is None else (stats[0].data_ptr(), stats[1].data_ptr())
-            _check(lib.pd_layer_norm_fwd(x2.data_ptr(), None if w is None else w.data_ptr(),
-                                         None if b is None else b.data_ptr(), y.data_ptr(), mean, rstd, rows, d, eps,
-                                         int(x.dtype == torch.float32), int(p_fp32), _s()), "layer_norm_fwd")
+        x2 = _flat_rows(x, x.shape[-1])
+        w, b = None if w is None else _dense(w), None if b is None else _dense(b)
+        stats = torch.empty(2, x2.shape[0], device=x.device, dtype=torch.float32)
+        y = _layer_norm_fwd(x2, w, b, eps, stats)
         ctx.save_for_backward(x2, w, stats)
-        ctx.p_dtype = torch.float32 if p_fp32 else torch.bfloat16
-        return y.view(x.shape)
+        ctx.p_dtype = b.dtype if w is None and b is not None else torch.float32 if w is None else w.dtype
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     def backward(ctx, dy: Tensor):  # type: ignore[override]
         x2, w, stats = ctx.saved_tensors
         rows, d = x2.shape
-        dy2 = _dense(dy.reshape(x2.shape))
         want_x, want_w, want_b, _ = ctx.needs_input_grad
+        dev, p_dtype = x2.device, ctx.p_dtype
         dx = torch.empty_like(x2) if want_x else None
-        new = torch.zeros if rows == 0 else torch.empty
-        dw = new(d, device=x2.device, dtype=ctx.p_dtype) if want_w else None
-        db = new(d, device=x2.device, dtype=ctx.p_dtype) if want_b else None
+        dw = torch.empty(d, device=dev, dtype=p_dtype) if want_w else None
+        db = torch.empty(d, device=dev, dtype=p_dtype) if want_b else None
         if rows > 0:
-            lib = _lib()
+            dy2 = _flat_rows(dy, d)
             partial = None
             if want_w or want_b:
-                lib.pd_layer_norm_partial_rows.argtypes = [C.c_longlong, C.c_int]
-                partial = torch.empty(lib.pd_layer_norm_partial_rows(rows, d), 2, d, device=x2.device, dtype=torch.float32)
+                partial = torch.empty(_layer_norm_partial_rows(rows, d), 2, d, device=dev, dtype=torch.float32)
                 nv.count_launch()
-            lib.pd_layer_norm_bwd.argtypes = [C.c_void_p] * 9 + [C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p]
-            ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-            _check(lib.pd_layer_norm_bwd(x2.data_ptr(), ptr(w), dy2.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(),
-                                         ptr(dx), ptr(dw), ptr(db), ptr(partial), rows, d,
-                                         int(x2.dtype == torch.float32), int(ctx.p_dtype == torch.float32), _s()),
-                   "layer_norm_bwd")
-        return None if dx is None else dx.view(dy.shape), dw, db, None
-
-
-LAYER_NORM_MAX_COLUMNS = 12288
+            at = stats.data_ptr()
+            _check(_lib().pd_layer_norm_bwd(x2.data_ptr(), None if w is None else w.data_ptr(), dy2.data_ptr(), at, at + 4 * rows,
+                                            None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                                            None if db is None else db.data_ptr(), None if partial is None else partial.data_ptr(),
+                                            rows, d, x2.dtype is torch.float32, p_dtype is torch.float32, _s()), "layer_norm_bwd")
+        else:
+            for grad in (dw, db):
+                if grad is not None:
+                    grad.zero_()
+        return None if dx is None else dx if dy.dim() == 2 else dx.view(dy.shape), dw, db, None
 
 
 def layer_norm(x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Tensor:
@@ -224,17 +247,21 @@ def layer_norm(x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Ten
 
     `x [..., d]` bf16 or fp32 with `1 <= d <= 12288`; `w`, `b` `[d]` (or None), bf16 or fp32 and of one type. Statistics and
     weight gradients are summed in fp32, in an order that depends on the sizes alone; each output is rounded once."""
-    if x.dtype not in (torch.bfloat16, torch.float32):
+    if x.dtype not in _FLOAT:
         raise ValueError(f"layer_norm: {x.dtype} is not bf16 or fp32")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= LAYER_NORM_MAX_COLUMNS:
         raise ValueError(f"layer_norm: rows of 1 to {LAYER_NORM_MAX_COLUMNS} columns, not {tuple(x.shape)}")
-    given = [p for p in (w, b) if p is not None]
-    for p in given:
-        if p.shape != x.shape[-1:] or p.dtype not in (torch.bfloat16, torch.float32) or p.dtype != given[0].dtype:
-            raise ValueError(f"layer_norm: scale and shift are [{x.shape[-1]}] in bf16 or fp32 and of one type, "
-                             f"not {[(tuple(q.shape), q.dtype) for q in given]}")
+    for p in (w, b):
+        if p is not None and (p.dim() != 1 or p.shape[0] != x.shape[-1] or p.dtype not in _FLOAT):
+            raise ValueError(f"layer_norm: scale and shift are [{x.shape[-1]}] in bf16 or fp32, not {tuple(p.shape)} {p.dtype}")
+    if w is not None and b is not None and w.dtype is not b.dtype:
+        raise ValueError(f"layer_norm: scale and shift are of one type, not {w.dtype} and {b.dtype}")
     _on_current_device("layer_norm", x, w, b)
-    return _LayerNorm.apply(x, w, b, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad) or (b is not None and b.requires_grad)):
+        return _LayerNorm.apply(x, w, b, eps)
+    x2 = _flat_rows(x, x.shape[-1])
+    y = _layer_norm_fwd(x2, None if w is None else _dense(w), None if b is None else _dense(b), eps, None)
+    return y if x.dim() == 2 else y.view(x.shape)
 
 
 class _Rope(torch.autograd.Function):

@@ -8,16 +8,16 @@ run, and rounded once to the table's type. Every row of the gradient is written:
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 
 import torch
 from torch import Tensor
 
 from param_decomp_b200.ops import native as nv
-from param_decomp_b200.ops.elementwise import _check, _dense, _on_current_device, _s
-
-_FLOAT = (torch.bfloat16, torch.float32)
+from param_decomp_b200.ops.elementwise import _FLOAT, _check, _dense, _flat_rows, _on_current_device, _s
 
 
+@lru_cache(maxsize=1)
 def _lib():
     lib = nv.lib()
     P, LL, I, F = C.c_void_p, C.c_longlong, C.c_int, C.c_float
@@ -28,15 +28,31 @@ def _lib():
     return lib
 
 
+@lru_cache(maxsize=256)
+def _scratch(n: int, d: int) -> tuple[int, int]:
+    """Ints and floats of the gradient's scratch."""
+    return _lib().pd_embedding_grad_ints(n), _lib().pd_embedding_grad_floats(n, d)
+
+
+def _lookup(table: Tensor, tokens: Tensor, scale: float, out_dtype: torch.dtype) -> Tensor:
+    n, (rows, d) = tokens.numel(), table.shape
+    y = torch.empty(n, d, device=table.device, dtype=out_dtype)
+    if n > 0:
+        _check(_lib().pd_embedding(tokens.data_ptr(), tokens.dtype is torch.int64, table.data_ptr(), y.data_ptr(), n, rows, d,
+                                   scale, table.dtype is torch.float32, out_dtype is torch.float32,
+                                   nv.status_word().data_ptr(), nv.refused_ptr(), _s()), "embedding")
+    return y
+
+
 def _grad(tokens: Tensor, dy: Tensor, rows: int, scale: float, dtype: torch.dtype) -> Tensor:
     n, d = dy.shape
     lib = _lib()
     dE = torch.empty(rows, d, device=dy.device, dtype=dtype)
-    ints = torch.empty(lib.pd_embedding_grad_ints(n), device=dy.device, dtype=torch.int32)
-    partial = torch.empty(lib.pd_embedding_grad_floats(n, d), device=dy.device, dtype=torch.float32)
-    _check(lib.pd_embedding_grad(tokens.data_ptr(), int(tokens.dtype == torch.int64), dy.data_ptr(), dE.data_ptr(), n, rows,
-                                 d, scale, int(dy.dtype == torch.float32), int(dtype == torch.float32), ints.data_ptr(),
-                                 partial.data_ptr(), _s()), "embedding_grad")
+    ints, floats = _scratch(n, d)
+    scratch = torch.empty(ints + floats, device=dy.device, dtype=torch.float32)
+    _check(lib.pd_embedding_grad(tokens.data_ptr(), tokens.dtype is torch.int64, dy.data_ptr(), dE.data_ptr(), n, rows,
+                                 d, scale, dy.dtype is torch.float32, dtype is torch.float32, scratch.data_ptr() + 4 * floats,
+                                 scratch.data_ptr(), _s()), "embedding_grad")
     nv.count_launch()
     return dE
 
@@ -44,24 +60,14 @@ def _grad(tokens: Tensor, dy: Tensor, rows: int, scale: float, dtype: torch.dtyp
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table: Tensor, tokens: Tensor, scale: float, out_dtype: torch.dtype) -> Tensor:  # type: ignore[override]
-        table = _dense(table)
-        flat = _dense(tokens.reshape(-1))
-        rows, d = table.shape
-        y = torch.empty(flat.numel(), d, device=table.device, dtype=out_dtype)
-        if flat.numel() > 0:
-            _check(_lib().pd_embedding(flat.data_ptr(), int(flat.dtype == torch.int64), table.data_ptr(), y.data_ptr(),
-                                       flat.numel(), rows, d, scale, int(table.dtype == torch.float32),
-                                       int(out_dtype == torch.float32), nv.status_word().data_ptr(), nv.refused_ptr(),
-                                       _s()), "embedding")
-        ctx.save_for_backward(flat)
-        ctx.cfg = (rows, scale, table.dtype)
-        return y.view(*tokens.shape, d)
+        ctx.save_for_backward(tokens)
+        ctx.cfg = (table.shape[0], scale, table.dtype)
+        return _lookup(_dense(table), tokens, scale, out_dtype)
 
     @staticmethod
     def backward(ctx, dy: Tensor):  # type: ignore[override]
-        (flat,) = ctx.saved_tensors
         rows, scale, dtype = ctx.cfg
-        return _grad(flat, _dense(dy.reshape(flat.numel(), dy.shape[-1])), rows, scale, dtype), None, None, None
+        return _grad(ctx.saved_tensors[0], _flat_rows(dy, dy.shape[-1]), rows, scale, dtype), None, None, None
 
 
 def embedding(tokens: Tensor, table: Tensor, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> Tensor:
@@ -81,4 +87,10 @@ def embedding(tokens: Tensor, table: Tensor, scale: float = 1.0, out_dtype: torc
         raise ValueError(f"embedding: fewer than 2^30 tokens and 2^31 rows, not {tokens.numel()} and {table.shape[0]}")
     _on_current_device("embedding", tokens, table)
     nv.raise_refused()
-    return _Embedding.apply(table, tokens, float(scale), out_dtype)
+    flat = tokens if tokens.dim() == 1 else tokens.reshape(-1)
+    flat = _dense(flat)
+    if table.requires_grad and torch.is_grad_enabled():
+        y = _Embedding.apply(table, flat, scale, out_dtype)
+    else:
+        y = _lookup(_dense(table), flat, scale, out_dtype)
+    return y if tokens.dim() == 1 else y.view(*tokens.shape, table.shape[1])

@@ -13,16 +13,16 @@ The `eager_*` functions are the same definitions in plain torch, for any device.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
 from torch import Tensor
 
 from param_decomp_b200.ops import native as nv
-from param_decomp_b200.ops.elementwise import _check, _dense, _on_current_device, _s
+from param_decomp_b200.ops.elementwise import _FLOAT, _check, _dense, _flat_rows, _on_current_device, _s
 
 MAX_K = 256
-_FLOAT = (torch.bfloat16, torch.float32)
 
 
 class TopLogits(NamedTuple):
@@ -31,6 +31,7 @@ class TopLogits(NamedTuple):
     tail: Tensor  # [...] fp32 logsumexp of all other logits over the temperature (-inf where k is the whole row)
 
 
+@lru_cache(maxsize=1)
 def _lib():
     lib = nv.lib()
     P, LL, I, F, D = C.c_void_p, C.c_longlong, C.c_int, C.c_float, C.c_double
@@ -40,11 +41,16 @@ def _lib():
     return lib
 
 
+@lru_cache(maxsize=2)
+def _max_columns(fp32: bool) -> int:
+    return _lib().pd_top_kl_max_columns(fp32)
+
+
 def _rows_of(logits: Tensor) -> Tensor:
     """`[rows, V]` view with neighbouring columns and rows that do not overlap (a copy where there is none)."""
-    z = logits.reshape(-1, logits.shape[-1])
-    V = z.shape[1]
-    if (V > 1 and z.stride(1) != 1) or (z.shape[0] > 1 and z.stride(0) < V):
+    V = logits.shape[-1]
+    z = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if not z.is_contiguous() and ((V > 1 and z.stride(1) != 1) or (z.shape[0] > 1 and z.stride(0) < V)):
         z = z.contiguous()
     return z
 
@@ -58,8 +64,8 @@ def _check_logits(what: str, logits: Tensor, temperature: float) -> None:
         raise ValueError(f"{what}: logits are bf16 or fp32, not {logits.dtype}")
     if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 31:
         raise ValueError(f"{what}: logits of shape {tuple(logits.shape)}")
-    if logits.numel() // logits.shape[-1] >= 1 << 31:
-        raise ValueError(f"{what}: fewer than 2^31 rows")
+    if logits.numel() // logits.shape[-1] >= 1 << 28:
+        raise ValueError(f"{what}: fewer than 2^28 rows")
     if not 0.0 < temperature < float("inf"):
         raise ValueError(f"{what}: the temperature is positive, not {temperature}")
 
@@ -80,19 +86,19 @@ def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     tail = torch.empty(rows, device=z.device, dtype=torch.float32)
     if rows > 0:
         _check(_lib().pd_top_logits(z.data_ptr(), rows, V, _pitch(z), k, 1.0 / temperature, values.data_ptr(),
-                                    indices.data_ptr(), tail.data_ptr(), int(z.dtype == torch.float32), _s()), "top_logits")
+                                    indices.data_ptr(), tail.data_ptr(), z.dtype is torch.float32, _s()), "top_logits")
     return TopLogits(values.view(*lead, k), indices.view(*lead, k), tail.view(lead))
 
 
 def _launch(z: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None, temperature: float, loss: Tensor | None,
             dz: Tensor | None, scale: Tensor | None) -> None:
     rows, V = z.shape
-    _check(_lib().pd_top_kl(z.data_ptr(), rows, V, _pitch(z), indices.data_ptr(), int(indices.dtype == torch.int64),
-                            values.data_ptr(), int(values.dtype == torch.float32), indices.shape[1],
+    _check(_lib().pd_top_kl(z.data_ptr(), rows, V, _pitch(z), indices.data_ptr(), indices.dtype is torch.int64,
+                            values.data_ptr(), values.dtype is torch.float32, indices.shape[1],
                             None if tail is None else tail.data_ptr(), 1.0 / temperature,
                             None if loss is None else loss.data_ptr(), None if dz is None else dz.data_ptr(),
                             0 if dz is None else dz.stride(0), None if scale is None else scale.data_ptr(),
-                            int(z.dtype == torch.float32), nv.status_word().data_ptr(), nv.refused_ptr(), _s()), "top_kl")
+                            z.dtype is torch.float32, nv.status_word().data_ptr(), nv.refused_ptr(), _s()), "top_kl")
 
 
 def _grad_like(z: Tensor) -> Tensor:
@@ -122,7 +128,7 @@ class _TopKL(torch.autograd.Function):
         z, indices, values, tail = ctx.saved_tensors
         dz = _grad_like(z)
         if z.shape[0] > 0:
-            _launch(z, indices, values, tail, ctx.temperature, None, dz, _dense(dloss.float()))
+            _launch(z, indices, values, tail, ctx.temperature, None, dz, _dense(dloss))
         return dz, None, None, None, None
 
 
@@ -141,11 +147,11 @@ def _arguments(what: str, logits: Tensor, indices: Tensor, values: Tensor, tail:
     if tail is not None and (tail.dtype != torch.float32 or tail.shape != lead):
         raise ValueError(f"{what}: the tail is fp32 of shape {tuple(lead)}, not {tail.dtype} {tuple(tail.shape)}")
     _on_current_device(what, logits, indices, values, tail)
-    limit = _lib().pd_top_kl_max_columns(int(logits.dtype == torch.float32))
+    limit = _max_columns(logits.dtype is torch.float32)
     if V > limit:
         raise ValueError(f"{what}: rows of at most {limit} {logits.dtype} logits, not {V}")
     nv.raise_refused()
-    return (_rows_of(logits), _dense(indices.reshape(-1, k)), _dense(values.detach().reshape(-1, k)),
+    return (_rows_of(logits), _flat_rows(indices, k), _flat_rows(values.detach(), k),
             None if tail is None else _dense(tail.detach().reshape(-1)))
 
 
@@ -158,7 +164,13 @@ def top_kl(logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None 
     logsumexp of all other logits over the temperature; without it the teacher has its `k` slots alone. Both sides are taken
     at `temperature`. A row whose teacher has no mass counts zero, with a zero gradient."""
     z, indices, values, tail = _arguments("top_kl", logits, indices, values, tail, temperature)
-    return _TopKL.apply(z, indices, values, tail, temperature).view(logits.shape[:-1])
+    if z.requires_grad and torch.is_grad_enabled():
+        loss = _TopKL.apply(z, indices, values, tail, temperature)
+    else:
+        loss = torch.empty(z.shape[0], device=z.device, dtype=torch.float32)
+        if z.shape[0] > 0:
+            _launch(z, indices, values, tail, temperature, loss, None, None)
+    return loss if logits.dim() == 2 else loss.view(logits.shape[:-1])
 
 
 def top_kl_rows(logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None = None, temperature: float = 1.0,
