@@ -1,16 +1,19 @@
 // The k largest logits of every row (descending, equal logits in the order of their columns), their columns, and the
 // logarithm of the sum of exp(z / T) over the rest of the row.
 //
-// One block a row, two passes. First: every thread keeps the maximum of its own columns; the k-th largest T_0 of those
-// maxima is a lower bound of the k-th largest logit, and a tight one (k = 64 of 512 threads: about 68 logits reach it).
-// Second, out of L2: logits that reach T_0 are collected with their columns, all others go into the sum of
-// exponentials relative to T_0. The collected ones are ranked by counting, with (logit, column) as one number, so the
-// order in which they arrived does not matter. A row that defeats the bound (fewer than 2 k groups of 16 bytes, ties in
-// masses, rows of -inf) is selected by its keys' digits instead, exactly and at any number of ties.
-// HBM is read once; what bounds a row is its first pass.
+// Rows are held in the shared memory of a cluster of 1 to 8 blocks (`row_slice.cuh`) and read there twice, so a logit
+// crosses HBM once, and that bounds it. First pass: every thread keeps the maxima of two halves of its own columns; the k-th
+// largest T_0 of those (over the cluster's blocks, of the threads of one number taken together) is a lower bound of the k-th
+// largest logit, and a tight one (k = 64 of 512 maxima: about 68 logits reach it). Second: logits that reach T_0 are
+// collected with their columns, and exponentials are summed with every logit cut off at T_0, whose term is taken off again
+// once a collected logit. The cluster's first block ranks the collected ones by counting, with (logit, column) as one
+// number, so the order in which they arrived does not matter.
+// A row that defeats the bound (fewer than 2 k groups of 16 bytes, ties in masses, rows of -inf) is selected out of global
+// memory by its keys' digits instead, exactly and at any number of ties, and a rest that is small beside what was taken off
+// is summed by itself.
 #include <algorithm>
 
-#include "rows.cuh"
+#include "row_slice.cuh"
 
 namespace {
 
@@ -18,12 +21,20 @@ using namespace pd;
 
 constexpr int kMaxK = 256;
 constexpr int kRoom = 512;  // logits collected
+constexpr int kWarps = 8, kThreads = 32 * kWarps;  // that hold a row; one more warp deals rows
+constexpr int kMaxima = 2 * kThreads;
+constexpr int kBins = 512;
 constexpr float kLog2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+__device__ __forceinline__ uint32_t load_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long load_cluster_u64(uint32_t addr) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
 }
 // Whole numbers in the order of the values: -0 equals +0, NaN above everything.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -34,12 +45,66 @@ __device__ __forceinline__ uint32_t key_of(float v) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
-// (logit, column) as one number: larger logits first, then lower columns.
+// (logit, column) as one number: larger logits first, then lower columns; the last bit keeps a zero's sign.
 __device__ __forceinline__ unsigned long long place_of(float v, int col) {
-  return (static_cast<unsigned long long>(key_of(v)) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(col));
+  return (static_cast<unsigned long long>(key_of(v)) << 32) | ((0x7FFFFFFFu - static_cast<uint32_t>(col)) << 1) |
+         (__float_as_uint(v) == 0x80000000u);
+}
+__device__ __forceinline__ int column_of(unsigned long long place) {
+  return static_cast<int>(0x7FFFFFFFu - (static_cast<uint32_t>(place) >> 1));
+}
+__device__ __forceinline__ float logit_of(unsigned long long place) {
+  const float v = value_of(static_cast<uint32_t>(place >> 32));
+  return v == 0.0f && (place & 1) ? -0.0f : v;
+}
+// The larger of two words' values, NaN before everything; and a word cut off at `low`, NaN too.
+template <typename T>
+__device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat162 r =
+        __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+    return __float_as_uint(r);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t most(const uint4& q) {
+  return most<T>(most<T>(q.x, q.y), most<T>(q.z, q.w));
+}
+template <typename T>
+__device__ __forceinline__ bool below(uint32_t w, float low) {
+  if constexpr (sizeof(T) == 2)
+    return __uint_as_float(w << 16) < low && __uint_as_float(w & 0xFFFF0000u) < low;
+  else
+    return __uint_as_float(w) < low;
+}
+// One bit a value of the group that is not below `low`.
+template <typename T>
+__device__ __forceinline__ uint32_t reached(const uint4& q, float low) {
+  f32x2 v[8 / sizeof(T)];
+  pairs_of<T>(q, v);
+  uint32_t bits = 0;
+#pragma unroll
+  for (int j = 0; j < static_cast<int>(8 / sizeof(T)); ++j) {
+    const float2 x = unpack2(v[j]);
+    bits |= (x.x < low ? 0u : 1u << 2 * j) | (x.y < low ? 0u : 2u << 2 * j);
+  }
+  return bits;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t cut_off(uint32_t w, uint32_t low) {
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat162 r = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&low));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    return __float_as_uint(fminf(__uint_as_float(w), __uint_as_float(low)));
+  }
 }
 
-// 16 bytes of a row at a time, at 16-byte addresses wherever the row starts: group g holds columns g kE - shift + j.
+// A row in global memory, 16 bytes at a time, at 16-byte addresses wherever it starts: group g holds columns g kE - shift + j.
 template <typename T>
 struct Row {
   static constexpr int kE = 16 / sizeof(T);
@@ -49,39 +114,45 @@ struct Row {
     shift = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
     groups = (shift + V + kE - 1) / kE;
   }
-  // The group's values; columns outside the row hold -inf.
-  __device__ __forceinline__ void load(int g, float (&v)[kE]) const {
+  // A group as it lies in memory; columns outside the row hold -inf.
+  __device__ __forceinline__ uint4 load(int g) const {
     const int c0 = g * kE - shift;
-    if (c0 >= 0 && c0 + kE <= V) {
-      const uint4 q = *reinterpret_cast<const uint4*>(base + c0);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if (c0 >= 0 && c0 + kE <= V) return *reinterpret_cast<const uint4*>(base + c0);
+    T each[kE];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 2) {
-          v[2 * j] = __uint_as_float(w[j] << 16);
-          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        } else {
-          v[j] = __uint_as_float(w[j]);
-        }
-      }
-    } else {
+    for (int j = 0; j < kE; ++j) {
+      if (c0 + j >= 0 && c0 + j < V)
+        each[j] = base[c0 + j];
+      else
+        store1(each + j, -INFINITY);
+    }
+    uint4 q;
+    memcpy(&q, each, 16);
+    return q;
+  }
+  __device__ __forceinline__ static void values(const uint4& q, float (&v)[kE]) {
+    f32x2 pair[kE / 2];
+    pairs_of<T>(q, pair);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) v[j] = c0 + j >= 0 && c0 + j < V ? as_float(base[c0 + j]) : -INFINITY;
+    for (int j = 0; j < kE / 2; ++j) {
+      const float2 x = unpack2(pair[j]);
+      v[2 * j] = x.x;
+      v[2 * j + 1] = x.y;
     }
   }
   __device__ __forceinline__ bool inside(int col) const { return col >= 0 && col < V; }
 };
 
-// log of the sum of exp(z / T) over the columns behind the place `last` of the k-th, relative to their own maximum.
+// The columns behind the place `last` of the k-th: their maximum m, and the sum of exp((z - m) / T).
 template <typename T>
-__device__ float rest_logsumexp(const Row<T>& row, unsigned long long last, float inv_t, float (*red)[32]) {
+__device__ float2 rest_of(const Row<T>& row, unsigned long long last, float inv_t, float (*red)[32]) {
   constexpr int kE = Row<T>::kE;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kWarps;
   float m = -INFINITY;
   bool nan = false;
-  for (int g = threadIdx.x; g < row.groups; g += blockDim.x) {
+  for (int g = threadIdx.x; g < row.groups; g += kThreads) {
     float v[kE];
-    row.load(g, v);
+    Row<T>::values(row.load(g), v);
 #pragma unroll
     for (int j = 0; j < kE; ++j) {
       const int col = g * kE - row.shift + j;
@@ -93,15 +164,20 @@ __device__ float rest_logsumexp(const Row<T>& row, unsigned long long last, floa
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  nan = __syncthreads_or(nan);
-  if (lane == 0) red[0][warp] = m;
-  __syncthreads();
-  for (int w = 0; w < warps; ++w) m = fmaxf(m, red[0][w]);
+  nan = __any_sync(0xffffffffu, nan);
+  sync_first(kThreads);
+  if (lane == 0) red[0][warp] = nan ? NAN : m;
+  sync_first(kThreads);
+  nan = false;
+  for (int w = 0; w < warps; ++w) {
+    nan |= red[0][w] != red[0][w];
+    m = fmaxf(m, red[0][w]);
+  }
   float s = 0.0f;
   if (m > -INFINITY && m < INFINITY) {
-    for (int g = threadIdx.x; g < row.groups; g += blockDim.x) {
+    for (int g = threadIdx.x; g < row.groups; g += kThreads) {
       float v[kE];
-      row.load(g, v);
+      Row<T>::values(row.load(g), v);
 #pragma unroll
       for (int j = 0; j < kE; ++j) {
         const int col = g * kE - row.shift + j;
@@ -111,12 +187,12 @@ __device__ float rest_logsumexp(const Row<T>& row, unsigned long long last, floa
   }
   s = warp_sum(s);
   if (lane == 0) red[1][warp] = s;
-  __syncthreads();
+  sync_first(kThreads);
   s = 0.0f;
   for (int w = 0; w < warps; ++w) s += red[1][w];
-  __syncthreads();
-  if (nan) return NAN;
-  return m > -INFINITY && m < INFINITY ? m * inv_t + logf(s) : m;
+  sync_first(kThreads);
+  if (nan) return make_float2(INFINITY, NAN);
+  return make_float2(m, m == INFINITY ? 1.0f : s);
 }
 
 // The k-th largest (value, column) place by the keys' digits from the top; leaves the k best in `kept` (any order).
@@ -130,11 +206,11 @@ __device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* k
 #pragma unroll 1
   for (int digit = 0; digit < kDigits; ++digit) {
     const int down = 24 - 8 * digit;
-    for (int i = tid; i < 256; i += blockDim.x) hist[i] = 0;
-    __syncthreads();
-    for (int g = tid; g < row.groups; g += blockDim.x) {
+    for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
+    sync_first(kThreads);
+    for (int g = tid; g < row.groups; g += kThreads) {
       float v[kE];
-      row.load(g, v);
+      Row<T>::values(row.load(g), v);
 #pragma unroll
       for (int j = 0; j < kE; ++j) {
         const uint32_t key = key_of(v[j]);
@@ -142,7 +218,7 @@ __device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* k
           atomicAdd(hist + ((key >> down) & 255), 1);
       }
     }
-    __syncthreads();
+    sync_first(kThreads);
     if (warp == 0) {  // lane l holds the eight bins 255 - 8 l and below: from the largest digit down
       int sum = 0;
 #pragma unroll
@@ -166,21 +242,21 @@ __device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* k
         }
       }
     }
-    __syncthreads();
+    sync_first(kThreads);
     prefix = prefix << 8 | static_cast<uint32_t>(shared[0]);
     need = shared[1];
-    __syncthreads();
+    sync_first(kThreads);
   }
   // everything above the k-th key, and the first `need` columns that hold it
   if (tid == 0) shared[0] = shared[1] = 0;
-  __syncthreads();
+  sync_first(kThreads);
   constexpr int kDown = 32 - 8 * kDigits;
-  for (int g0 = 0; g0 < row.groups; g0 += blockDim.x) {
+  for (int g0 = 0; g0 < row.groups; g0 += kThreads) {
     const int g = g0 + tid;
     float v[kE];
     int equal = 0;
     if (g < row.groups) {
-      row.load(g, v);
+      Row<T>::values(row.load(g), v);
 #pragma unroll
       for (int j = 0; j < kE; ++j) {
         const int col = g * kE - row.shift + j;
@@ -197,9 +273,9 @@ __device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* k
       if (lane >= o) upto += u;
     }
     if (lane == 31) hist[warp] = upto;
-    __syncthreads();
+    sync_first(kThreads);
     int before = shared[1] + upto - equal, all = 0;
-    for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) before += hist[w];
       all += hist[w];
     }
@@ -212,125 +288,368 @@ __device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* k
         ++before;
       }
     }
-    __syncthreads();
+    sync_first(kThreads);
     if (tid == 0) shared[1] += all;
-    __syncthreads();
+    sync_first(kThreads);
   }
 }
 
+// log of s exp(m / T); s = 0 for nothing, and for an infinite m whatever it is (NaN stays NaN).
+__device__ __forceinline__ float log_sum(float2 r, float inv_t) { return r.x > -INFINITY && r.x < INFINITY ? r.x * inv_t + logf(r.y) : r.x + 0.0f * r.y; }
+
+struct Shared {  // one object, whose address inline assembly gets: waits there may change any part of it
+  RowQueue queue;
+  unsigned long long bars[kWarps + 6];
+  unsigned long long kept[kRoom], last;
+  float red[2][32], sums[kWarps], sum;
+  alignas(16) int hist[kBins];
+  int pair[2];
+  struct {
+    int row;
+    float edge[16];
+  } ahead[3];  // rows to come, with the elements at their ragged ends
+  uint32_t top;  // the largest key
+  int found, next, abort_flag;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(512) top_logits_kernel(const T* __restrict__ z, long long ld, int V, int k, float inv_t,
-                                                         T* __restrict__ values, int* __restrict__ indices,
-                                                         float* __restrict__ tail) {
+__global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* __restrict__ z, long long ld, int V, int k,
+                                                                      float inv_t, SlicePlan plan, T* __restrict__ values,
+                                                                      int* __restrict__ indices, float* __restrict__ tail,
+                                                                      int* __restrict__ status) {
   constexpr int kE = Row<T>::kE;
-  __shared__ unsigned long long kept[kRoom];
-  __shared__ float red[2][32];
-  __shared__ int hist[256], shared[2], found;
-  __shared__ unsigned long long last;
-  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
-  const long long r = blockIdx.x;
-  const Row<T> row(z + r * ld, V);
-  bool by_digits = min(nt, row.groups) < 2 * k;
-  int n = 0;
-  float low = 0.0f, sum = 0.0f;
-  if (!by_digits) {
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int g = tid; g < row.groups; g += nt) {
-      float v[kE];
-      row.load(g, v);
-#pragma unroll
-      for (int j = 0; j < kE; ++j) m = fmaxf(m, v[j]);
+  extern __shared__ __align__(128) uint8_t smem[];  // the slice; behind it, in a cluster, [cs][kMaxima] maxima
+  __shared__ __align__(16) Shared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cs = plan.cs;
+  const int rank = cs > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const RowSlice<T> rows{z, ld, V, rank * plan.slice, plan.slice, plan.per};
+  unsigned short* maxima = reinterpret_cast<unsigned short*>(smem + 16ll * plan.slice);
+  T* buf = reinterpret_cast<T*>(smem);
+  const float c = inv_t * kLog2E;
+  const uint32_t bar0 = smem_u32(sh.bars), ready = bar0 + 8 * kWarps, done = ready + 16, met = ready + 32;
+  if (tid == 0) {
+    for (int i = 0; i < kWarps + 4; ++i) mbar_init(bar0 + 8 * i, 1);
+    mbar_init(met, cs);
+    mbar_init(met + 8, cs);
+    sh.queue.init();
+    sh.abort_flag = 0;
+    sh.top = 0;
+    mbar_fence_init();
+  }
+  __syncthreads();
+  if (cs > 1) cluster_sync_all();  // every block of the cluster runs before another one stores to its shared memory
+  auto late = [&](bool in_time) {
+    if (!in_time && status != nullptr) atomicCAS(status, 0, kTimeoutProducer);
+  };
+  // The n-th completion of a pair of barriers that take turns.
+  auto wait_pair = [&](uint32_t pair, int n) { return short_wait<false>(pair + 8 * (n & 1), (n >> 1) & 1, &sh.abort_flag); };
+  if (warp == kWarps) {  // rows to come, two ahead
+    bool more = true;
+    if (rank == 0 && lane == 0) sh.queue.ask();
+    __syncwarp();
+    for (int n = 0;; ++n) {
+      int row = -1;
+      if (n == 0) {
+        row = blockIdx.x / cs;
+      } else if (more) {
+        bool in_time = true;
+        row = sh.queue.take(n, rank, cs, lane, &sh.abort_flag, in_time);
+        late(in_time);
+        if (row >= 0 && rank == 0 && lane == 0) sh.queue.ask();
+        __syncwarp();
+      }
+      more = row >= 0;
+      float edge = -INFINITY;
+      if (more && lane < 2 * kE) {
+        int col;
+        if (rows.edge_place(lane, rows.shift(row), col) >= 0 && col >= 0 && col < V) edge = as_float(rows.row(row)[col]);
+      }
+      if (n >= 2) late(wait_pair(done, n - 2));  // the row before the present one has been left
+      if (lane < 2 * kE) sh.ahead[n % 3].edge[lane] = edge;
+      if (lane == 0) sh.ahead[n % 3].row = row;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ready + 8 * (n & 1));
+      __syncwarp();
+      if (!more) break;
     }
-    if (tid == 0) found = 0;
-    // the k-th largest of the threads' maxima, in the upper 16 bits of its key (rounded down: still a lower bound)
-    const uint32_t mine = key_of(m) >> 16;
-    uint32_t bound = 0;
-#pragma unroll 1
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t trial = bound | 1u << bit;
-      if (__syncthreads_count(mine >= trial) >= k) bound = trial;
-    }
-    low = value_of(bound << 16);
-    by_digits = !(low > -INFINITY && low < INFINITY);
-    if (!by_digits) {
-      const float c = inv_t * kLog2E;
-#pragma unroll 4
-      for (int g = tid; g < row.groups; g += nt) {
-        float v[kE];
-        row.load(g, v);
+  } else {
+    if (lane == 0) rows.request(blockIdx.x / cs, warp, smem, bar0 + 8 * warp, false);
+    __syncwarp();
+    late(wait_pair(ready, 0));
+    int n = 0;
+    for (int r = blockIdx.x / cs; r >= 0; ++n) {
+      const int shift = rows.shift(r), groups = rows.groups(shift);
+      const int begin = warp * plan.per + lane, stop = min(groups, (warp + 1) * plan.per);
+      const Row<T> row(rows.row(r), V);
+      late(short_wait<false>(bar0 + 8 * warp, n & 1, &sh.abort_flag));
+      // a ragged end is written by the warp that reads it
+      if (warp == 0 || stop == groups) {
+        int col;
+        const int at = lane < 2 * kE ? rows.edge_place(lane, shift, col) : -1;
+        if (at >= 0 && at / kE >= warp * plan.per && at / kE < stop) store1(buf + at, sh.ahead[n % 3].edge[lane]);
+        fence_proxy_async_smem();  // before bulk copies of the next row write there
+        __syncwarp();
+      }
+      bool by_digits = min(kMaxima, row.groups) < 2 * k;  // from sizes alone: the same in every block
+      float low = 0.0f, sum = 0.0f, over = 0.0f, power = 0.0f;
+      uint32_t keys = 0;
+      int collected = 0;
+      if (!by_digits) {
+        GroupMax<T> m0, m1;
+        int g = begin;
+#pragma unroll 2
+        for (; g + 32 < stop; g += 64) {
+          m0.add(*reinterpret_cast<const uint4*>(smem + 16 * g));
+          m1.add(*reinterpret_cast<const uint4*>(smem + 16 * (g + 32)));
+        }
+        if (g < stop) m0.add(*reinterpret_cast<const uint4*>(smem + 16 * g));
+        keys = key_of(m0.value()) >> 16 | (key_of(m1.value()) & 0xFFFF0000u);
+        if (cs > 1) {
+          const uint32_t local = smem_u32(maxima + rank * kMaxima + 2 * tid);
+          for (int b = 0; b < cs; ++b)
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(local, b)), "r"(keys) : "memory");
+        } else {
+          const uint32_t most = __reduce_max_sync(0xffffffffu, max(keys >> 16, keys & 0xFFFFu));
+          if (lane == 0) atomicMax(&sh.top, most);
+          if (tid == 0) sh.found = 0;
+        }
+        sh.hist[tid] = sh.hist[tid + kThreads] = 0;
+      }
+      if (tid == 0) {  // all warps go on together, or none does: what the barrier below shows them decides
+        late(wait_pair(ready, n + 1));
+        sh.next = *static_cast<volatile int*>(&sh.abort_flag) ? -1 : sh.ahead[(n + 1) % 3].row;
+      }
+      sync_first(kThreads);
+      const int next = sh.next;
+      if (!by_digits) {
+        if (cs > 1) {
+          if (warp == 0 && lane < cs) mbar_arrive_cluster(mapa_shared(met, lane));
+          __syncwarp();
+          late(short_wait<true>(met, n & 1, &sh.abort_flag));
+          for (int b = 0; b < cs; ++b) keys = __vmaxu2(keys, reinterpret_cast<const uint32_t*>(maxima + b * kMaxima)[tid]);
+          const uint32_t most = __reduce_max_sync(0xffffffffu, max(keys >> 16, keys & 0xFFFFu));
+          if (lane == 0) atomicMax(&sh.top, most);
+          if (tid == 0) sh.found = 0;  // the first block has come to this row: it is done with the last one's list
+          sync_first(kThreads);
+        }
+        // The k-th largest of the maxima in the upper 16 bits of its key, rounded down: by a histogram of their distances
+        // from the largest, 128 bins an octave; where that does not reach far enough, of 16 and then of one.
+        const uint32_t top = sh.top;
+        uint32_t bound;
+        for (int coarse = 0;; coarse = coarse == 0 ? 3 : 7) {
+          atomicAdd(sh.hist + min(kBins - 1, (top - (keys >> 16)) >> coarse), 1);
+          atomicAdd(sh.hist + min(kBins - 1, (top - (keys & 0xFFFFu)) >> coarse), 1);
+          sync_first(kThreads);
+          int count[kBins / 32], total = 0;  // every warp for itself
 #pragma unroll
-        for (int j = 0; j < kE; ++j) {
-          if (v[j] < low) {
-            sum += ex2((v[j] - low) * c);
-          } else {
-            const int at = atomicAdd(&found, 1);
-            if (at < kRoom) kept[at] = place_of(v[j], g * kE - row.shift + j);
+          for (int i = 0; i < kBins / 128; ++i) {
+            const int4 q = reinterpret_cast<const int4*>(sh.hist)[kBins / 128 * lane + i];
+            count[4 * i] = q.x, count[4 * i + 1] = q.y, count[4 * i + 2] = q.z, count[4 * i + 3] = q.w;
+            total += q.x + q.y + q.z + q.w;
           }
+          int upto = total;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+          }
+          const int holder = __ffs(__ballot_sync(0xffffffffu, upto >= k)) - 1;  // kMaxima >= 2 k: there is one
+          int before = upto - total, bin = 0;
+#pragma unroll
+          for (int i = 0; i < kBins / 32; ++i) {
+            bin += before + count[i] < k;
+            before += count[i];
+          }
+          bin = __shfl_sync(0xffffffffu, kBins / 32 * lane + min(bin, kBins / 32 - 1), holder);
+          if (bin < kBins - 1 || coarse == 7) {
+            const uint32_t reach = (static_cast<uint32_t>(bin + 1) << coarse) - 1;
+            bound = bin < kBins - 1 && reach < top ? top - reach : 0;
+            break;
+          }
+          sync_first(kThreads);
+          sh.hist[tid] = sh.hist[tid + kThreads] = 0;
+          sync_first(kThreads);
+        }
+        if (tid == 0) sh.top = 0;
+        low = value_of(bound << 16);
+        if (sizeof(T) == 2) low = __uint_as_float(__float_as_uint(low) & 0xFFFF0000u);  // the bf16 number of that key
+        // Sums are relative to 2^power, so that one fused multiply-add gives an exponent.
+        power = rintf(low * c);
+        by_digits = !(fabsf(power) < 1.0e6f);
+        if (!by_digits) {
+          const f32x2 c2 = pk2(c, c), k2 = pk2(-power, -power);
+          const uint32_t low_bits = __float_as_uint(low), low_word = sizeof(T) == 2 ? low_bits >> 16 | low_bits : low_bits;
+          f32x2 s0 = 0ull, s1 = 0ull;
+          // groups that hold a logit to collect are noted, and looked into when the sums are done
+          unsigned long long noted = 0ull, bit = 1ull;
+#pragma unroll 4
+          for (int g = begin; g < stop; g += 32) {
+            const uint4 q = *reinterpret_cast<const uint4*>(smem + 16 * g);
+            if (!below<T>(most<T>(q), low)) noted |= bit;
+            bit <<= 1;
+            f32x2 v[kE / 2];
+            pairs_of<T>(make_uint4(cut_off<T>(q.x, low_word), cut_off<T>(q.y, low_word), cut_off<T>(q.z, low_word),
+                                   cut_off<T>(q.w, low_word)),
+                        v);
+#pragma unroll
+            for (int j = 0; j < kE / 2; ++j) {
+              const float2 x = unpack2(fma2(v[j], c2, k2));
+              const f32x2 e = pk2(ex2(x.x), ex2(x.y));
+              if (j & 1)
+                s1 = add2(s1, e);
+              else
+                s0 = add2(s0, e);
+            }
+          }
+          for (; noted != 0; noted &= noted - 1) {
+            const int g = begin + 32 * (__ffsll(noted) - 1);
+            for (uint32_t bits = reached<T>(*reinterpret_cast<const uint4*>(smem + 16 * g), low); bits != 0; bits &= bits - 1) {
+              const int j = __ffs(bits) - 1, col = (rows.g0 + g) * kE - shift + j;
+              const int at = col >= 0 && col < V ? atomicAdd(&sh.found, 1) : kRoom;
+              if (at < kRoom) sh.kept[at] = place_of(as_float(buf[g * kE + j]), col);
+            }
+          }
+          const float2 a = unpack2(add2(s0, s1));
+          sum = warp_sum(a.x + a.y);
+          if (lane == 0) sh.sums[warp] = sum;
         }
       }
-      sum = warp_sum(sum);
-      if (lane == 0) red[0][warp] = sum;
-      __syncthreads();
+      __syncwarp();
+      if (lane == 0 && next >= 0) {  // the warp's part of the next row
+        fence_proxy_async_smem();
+        rows.request(next, warp, smem, bar0 + 8 * warp, false);
+      }
+      __syncwarp();
+      sync_first(kThreads);
       sum = 0.0f;
-      for (int w = 0; w < nt / 32; ++w) sum += red[0][w];
-      n = found;
-      by_digits = n > kRoom;
-    }
-    __syncthreads();
-  }
-  if (by_digits) {
-    select_by_digits(row, k, kept, hist, shared);
-    n = k;
-  }
-  // rank by counting; every place differs from every other
-  float over = 0.0f;  // collected, but not among the k
-  for (int i = tid; i < n; i += nt) {
-    const unsigned long long own = kept[i];
-    int rank = 0;
+      for (int w = 0; w < kWarps; ++w) sum += sh.sums[w];
+      collected = sh.found;
+      if (cs > 1) {  // the first block takes over; the others write to their lists again when it has come to the next row
+        if (tid == 0) {
+          sh.sum = sum;
+          mbar_arrive_cluster(mapa_shared(met + 8, 0));
+        }
+        __syncwarp();
+        if (rank == 0) {
+          late(short_wait<true>(met + 8, n & 1, &sh.abort_flag));
+          if (!by_digits) {
+            // warp b copies block b's list; every warp reads all counts and sums for itself
+            const int count = lane < cs ? static_cast<int>(load_cluster_u32(mapa_shared(smem_u32(&sh.found), lane))) : 0;
+            sum = lane < cs ? __uint_as_float(load_cluster_u32(mapa_shared(smem_u32(&sh.sum), lane))) : 0.0f;
+            int upto = count;
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) {
+              const int v = __shfl_up_sync(0xffffffffu, upto, o);
+              if (lane >= o) upto += v;
+            }
+            sum = warp_sum(sum);
+            const int mine = __shfl_sync(0xffffffffu, count, warp), at = __shfl_sync(0xffffffffu, upto, warp) - mine;
+            collected = __shfl_sync(0xffffffffu, upto, 7);
+            if (warp > 0 && warp < cs) {
+              const uint32_t list = mapa_shared(smem_u32(sh.kept), warp);
+              for (int i = lane; i < mine && at + i < kRoom; i += 32) sh.kept[at + i] = load_cluster_u64(list + 8 * i);
+            }
+          }
+          sync_first(kThreads);
+        }
+      }
+      if (rank == 0) {
+        by_digits |= collected > kRoom;
+        if (by_digits) {
+          select_by_digits(row, k, sh.kept, sh.hist, sh.pair);
+          collected = k;
+        } else {
+          const float taken = static_cast<float>(collected) * ex2(fmaf(low, c, -power));
+          over = sum < 1.0625f * taken ? INFINITY : 0.0f;  // too little is left of it
+          sum = (sum - taken) * ex2(fmaf(-low, c, power));  // relative to exp(low / T) from here on
+        }
+        T* const row_values = values + static_cast<long long>(r) * k;
+        int* const row_indices = indices + static_cast<long long>(r) * k;
+        auto put = [&](unsigned long long own, int place) {
+          if (place < k) {
+            store1(row_values + place, logit_of(own));
+            row_indices[place] = column_of(own);
+            if (place == k - 1) sh.last = own;
+          } else {
+            over += ex2((logit_of(own) - low) * c);  // collected, but not among the k
+          }
+        };
+        if (collected <= kThreads / 2) {
+          // rank by counting, two threads a place; every place differs from every other
+          const int i = tid >> 1;
+          const unsigned long long own = i < collected ? sh.kept[i] : 0ull;
+          int place = 0;
+          if (i < collected) {
 #pragma unroll 8
-    for (int j = 0; j < n; ++j) rank += kept[j] > own;
-    const int col = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(own));
-    if (rank < k) {
-      values[r * k + rank] = row.base[col];
-      indices[r * k + rank] = col;
-      if (rank == k - 1) last = own;
-    } else {
-      over += ex2((as_float(row.base[col]) - low) * (inv_t * kLog2E));
+            for (int j = tid & 1; j < collected; j += 2) place += sh.kept[j] > own;
+          }
+          place += __shfl_xor_sync(0xffffffffu, place, 1);
+          if (i < collected && !(tid & 1)) put(own, place);
+        } else {
+          // sort all of them, descending, in 512 places: a warp's 64 by itself, wider steps over the block
+          for (int i = collected + tid; i < kRoom; i += kThreads) sh.kept[i] = 0ull;
+          sync_first(kThreads);
+          for (int size = 2; size <= kRoom; size *= 2)
+            for (int step = size / 2; step > 0; step /= 2) {
+              const int i = 2 * tid - (tid & (step - 1));  // the lower one of the pair
+              const unsigned long long x = sh.kept[i], y = sh.kept[i + step];
+              if ((x < y) == ((i & size) == 0)) {
+                sh.kept[i] = y;
+                sh.kept[i + step] = x;
+              }
+              if (step > 32 || (step == 1 && size >= 64))
+                sync_first(kThreads);
+              else
+                __syncwarp();
+            }
+          for (int i = tid; i < collected; i += kThreads) put(sh.kept[i], i);
+        }
+        // What is left: the sum relative to the bound with the collected ones that did not make it.
+        over = warp_sum(over);
+        if (lane == 0) sh.red[0][warp] = over;
+        sync_first(kThreads);
+        over = 0.0f;
+        for (int w = 0; w < kWarps; ++w) over += sh.red[0][w];
+        float2 result = make_float2(low, sum + over);
+        if (by_digits || !(over < 1e30f)) result = rest_of(row, sh.last, inv_t, sh.red);
+        if (tid == 0) tail[r] = log_sum(result, inv_t);
+        sync_first(kThreads);  // before the next row collects
+      }
+      if (tid == 0) mbar_arrive(done + 8 * (n & 1));
+      __syncwarp();
+      r = next;
     }
   }
-  // What is left: the sum relative to the bound with the collected ones that did not make it. Sums that are tiny have lost
-  // what lies far below the bound, and take the exact way; so do rows selected by digits.
-  const bool exact = __syncthreads_or(by_digits || !(over < 1e30f));
-  float result;
-  if (!exact) {
-    const float s = warp_sum(over);
-    if (lane == 0) red[1][warp] = s;
-    __syncthreads();
-    for (int w = 0; w < nt / 32; ++w) sum += red[1][w];
-    result = low * inv_t + logf(sum);
-  }
-  if (exact || !(sum > 1e-20f)) result = rest_logsumexp(row, last, inv_t, red);
-  if (tid == 0) tail[r] = result;
+  __syncwarp();
+  if (cs > 1) cluster_sync_all();  // no block leaves while another one may still read from it or store to it
 }
 
 template <typename T>
 int top(const void* z, long long rows, int V, long long ld, int k, float inv_t, void* values, int* indices, float* tail,
-        cudaStream_t st) {
-  const int groups = (V + Row<T>::kE - 1) / Row<T>::kE;
-  const int threads = groups > 1024 || k > 64 ? 512 : 256;
-  top_logits_kernel<T><<<static_cast<unsigned>(rows), threads, 0, st>>>(static_cast<const T*>(z), ld, V, k, inv_t,
-                                                                        static_cast<T*>(values), indices, tail);
-  return cudaGetLastError() == cudaSuccess ? 0 : 1;
+        int* status, cudaStream_t st) {
+  // Beside a slice, 7 KB of fixed shared memory and 1 KB of the system's: two blocks an SM, or one.
+  constexpr long long kHalfSm = 104 * 1024, kWholeSm = 208 * 1024;
+  const SlicePlan plan = slice_plan<T>(V, kWarps, kHalfSm, kWholeSm);
+  if (plan.cs == 0) return 5;
+  const int smem = plan.slice * 16 + (plan.cs > 1 ? plan.cs * kMaxima * 2 : 0);
+  auto kern = top_logits_kernel<T>;
+  static bool sized = false;  // the same answer whoever asks first
+  if (!sized && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 217 * 1024) != cudaSuccess) return 2;
+  sized = true;
+  return launch_clusters(kern, rows, plan.cs, kThreads + 32, smem, st, static_cast<const T*>(z), ld, V, k, inv_t, plan,
+                         static_cast<T*>(values), indices, tail, status);
 }
 
 }  // namespace
 
+// Widest row that a cluster holds.
+extern "C" long long pd_top_logits_max_columns(int z_fp32) { return 8ll * 208 * 1024 / (z_fp32 ? 4 : 2) - 16; }
+
 // z [rows, V] in bf16 or fp32, rows ld elements apart; values, indices [rows, k], tail [rows].
 extern "C" int pd_top_logits(const void* z, long long rows, int V, long long ld, int k, float inv_t, void* values,
-                             int* indices, float* tail, int z_fp32, void* stream) {
-  if (rows <= 0 || rows >= (1ll << 31) || V <= 0 || k <= 0 || k > kMaxK || k > V || !(inv_t > 0.0f)) return 5;
+                             int* indices, float* tail, int z_fp32, int* status, void* stream) {
+  if (rows <= 0 || rows >= (1ll << 28) || V <= 0 || k <= 0 || k > kMaxK || k > V || !(inv_t > 0.0f)) return 5;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return z_fp32 ? top<float>(z, rows, V, ld, k, inv_t, values, indices, tail, st)
-                : top<__nv_bfloat16>(z, rows, V, ld, k, inv_t, values, indices, tail, st);
+  return z_fp32 ? top<float>(z, rows, V, ld, k, inv_t, values, indices, tail, status, st)
+                : top<__nv_bfloat16>(z, rows, V, ld, k, inv_t, values, indices, tail, status, st);
 }

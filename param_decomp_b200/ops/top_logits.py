@@ -35,15 +35,23 @@ class TopLogits(NamedTuple):
 def _lib():
     lib = nv.lib()
     P, LL, I, F, D = C.c_void_p, C.c_longlong, C.c_int, C.c_float, C.c_double
-    lib.pd_top_logits.argtypes = [P, LL, I, LL, I, F, P, P, P, I, P]
+    lib.pd_top_logits.argtypes = [P, LL, I, LL, I, F, P, P, P, I, P, P]
+    lib.pd_top_logits_max_columns.argtypes, lib.pd_top_logits_max_columns.restype = [I], LL
     lib.pd_top_kl.argtypes = [P, LL, I, LL, P, I, P, I, I, P, D, P, P, LL, P, I, P, P, P]
     lib.pd_top_kl_max_columns.argtypes, lib.pd_top_kl_max_columns.restype = [I], LL
     return lib
 
 
-@lru_cache(maxsize=2)
-def _max_columns(fp32: bool) -> int:
-    return _lib().pd_top_kl_max_columns(fp32)
+@lru_cache(maxsize=4)
+def _max_columns(what: str, fp32: bool) -> int:
+    """The widest row that a cluster's shared memory holds."""
+    return (_lib().pd_top_logits_max_columns if what == "top_logits" else _lib().pd_top_kl_max_columns)(fp32)
+
+
+def _check_width(what: str, logits: Tensor) -> None:
+    limit = _max_columns(what, logits.dtype is torch.float32)
+    if logits.shape[-1] > limit:
+        raise ValueError(f"{what}: rows of at most {limit} {logits.dtype} logits, not {logits.shape[-1]}")
 
 
 def _rows_of(logits: Tensor) -> Tensor:
@@ -78,6 +86,7 @@ def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     if not 1 <= k <= min(V, MAX_K):
         raise ValueError(f"top_logits: k from 1 to {min(V, MAX_K)}, not {k}")
     _on_current_device("top_logits", logits)
+    _check_width("top_logits", logits)
     lead = logits.shape[:-1]
     z = _rows_of(logits.detach())
     rows = z.shape[0]
@@ -86,7 +95,8 @@ def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     tail = torch.empty(rows, device=z.device, dtype=torch.float32)
     if rows > 0:
         _check(_lib().pd_top_logits(z.data_ptr(), rows, V, _pitch(z), k, 1.0 / temperature, values.data_ptr(),
-                                    indices.data_ptr(), tail.data_ptr(), z.dtype is torch.float32, _s()), "top_logits")
+                                    indices.data_ptr(), tail.data_ptr(), z.dtype is torch.float32,
+                                    nv.status_word().data_ptr(), _s()), "top_logits")
     return TopLogits(values.view(*lead, k), indices.view(*lead, k), tail.view(lead))
 
 
@@ -134,7 +144,7 @@ class _TopKL(torch.autograd.Function):
 
 def _arguments(what: str, logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None, temperature: float):
     _check_logits(what, logits, temperature)
-    lead, V = logits.shape[:-1], logits.shape[-1]
+    lead = logits.shape[:-1]
     if indices.dtype not in (torch.int32, torch.int64) or indices.shape[:-1] != lead or indices.dim() != logits.dim():
         raise ValueError(f"{what}: columns are int32 or int64 of shape {tuple(lead)} + [k], not {indices.dtype} "
                          f"{tuple(indices.shape)}")
@@ -147,9 +157,7 @@ def _arguments(what: str, logits: Tensor, indices: Tensor, values: Tensor, tail:
     if tail is not None and (tail.dtype != torch.float32 or tail.shape != lead):
         raise ValueError(f"{what}: the tail is fp32 of shape {tuple(lead)}, not {tail.dtype} {tuple(tail.shape)}")
     _on_current_device(what, logits, indices, values, tail)
-    limit = _max_columns(logits.dtype is torch.float32)
-    if V > limit:
-        raise ValueError(f"{what}: rows of at most {limit} {logits.dtype} logits, not {V}")
+    _check_width(what, logits)
     nv.raise_refused()
     return (_rows_of(logits), _flat_rows(indices, k), _flat_rows(values.detach(), k),
             None if tail is None else _dense(tail.detach().reshape(-1)))
