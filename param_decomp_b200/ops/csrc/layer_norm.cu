@@ -1,10 +1,13 @@
 // Layer norm over rows of `d` columns:
 //   mean = sum x / d, var = sum (x - mean)^2 / d, xh = (x - mean) rstd, rstd = 1 / sqrt(var + eps), y = xh w + b
 //   dx = rstd (g - mean(g) - xh mean(g xh)) with g = dy w;  dw = sum over rows of dy xh;  db = sum over rows of dy
-// A row is held in the registers of one warp (up to 768 columns) or of one block, so x (and dy) cross HBM once and the
-// variance is summed around the mean that was just formed, not from sums of squares. All sums are in fp32; what is stored
-// is rounded once. Bound by HBM: 2 (forward) and 3 (backward) passes of the row data.
-// The weight gradients: every thread keeps the sums of its own columns over all rows that its block walks; blocks write
+// Bound by HBM: 2 (forward) and 3 (backward) passes of the row data. A group of warps holds a few rows at a time in
+// registers as they lie in memory, 8 columns a thread (up to 4096 columns; two or three times 8 beyond), so x and dy cross
+// HBM once, and one barrier serves the sums of all those rows. The handfuls to come are copied into shared memory meanwhile
+// (every thread's own columns, so no barrier but the thread's own wait): 60 to 90 KB an SM are on their way at any time,
+// more than registers could wait for. The variance is summed around the mean that was just formed, not from sums of
+// squares. All sums are in fp32; what is stored is rounded once.
+// The weight gradients: every thread keeps the sums of its own columns over all rows that its group walks; blocks write
 // those to scratch and a second kernel adds them in a fixed order, so a result does not change from run to run.
 #include <algorithm>
 
@@ -15,8 +18,20 @@ namespace {
 using namespace pd;
 
 constexpr int kMaxWarps = 16;  // of a row
-constexpr int kMaxChunks = 3;  // of 8 columns a thread: the backward holds 4 x 8 values a chunk
-constexpr int kWarpsPerBlock = 8;  // where a warp takes whole rows
+constexpr int kMaxChunks = 3;  // of 8 columns a thread
+constexpr int kMaxGroups = 8;  // of a block
+
+// Eight elements as they lie in memory.
+template <typename T>
+struct Words {
+  uint32_t w[2 * sizeof(T)];
+  __device__ __forceinline__ f32x2 pair(int i) const {  // elements 2 i and 2 i + 1
+    if constexpr (sizeof(T) == 2)
+      return unpack_bf16_2(w[i]);
+    else
+      return pk2u(w[2 * i], w[2 * i + 1]);
+  }
+};
 
 // Which column element j of chunk c is, for thread t of `tpr` that share a row. Rows of 16-byte pieces: eight
 // neighbours a thread; any other row: threads side by side, one element each.
@@ -24,217 +39,405 @@ template <bool kVec>
 __device__ __forceinline__ int column(int c, int j, int t, int tpr) {
   return kVec ? (c * tpr + t) * 8 + j : (c * 8 + j) * tpr + t;
 }
-
-// Eight neighbouring parameters, or one, in either type (a branch every thread takes alike).
-__device__ __forceinline__ void params8(const void* p, int fp32, int col, float (&v)[8]) {
-  if (fp32)
-    unpack8(load8(static_cast<const float*>(p) + col), v);
-  else
-    unpack8(load8(static_cast<const __nv_bfloat16*>(p) + col), v);
-}
-__device__ __forceinline__ float param1(const void* p, int fp32, int col) {
-  return fp32 ? static_cast<const float*>(p)[col] : as_float(static_cast<const __nv_bfloat16*>(p)[col]);
-}
-
-template <typename T, int kCh, bool kVec>
-__device__ __forceinline__ void load_row(const T* __restrict__ row, int d, int t, int tpr, float (&v)[kCh][8]) {
-  if (kVec) {
-    Raw8<T> raw[kCh];
+// Columns outside the row read as zero.
+template <typename T, bool kVec>
+__device__ __forceinline__ Words<T> load_words(const T* __restrict__ row, int c, int d, int t, int tpr, bool there) {
+  Words<T> r;
 #pragma unroll
-    for (int c = 0; c < kCh; ++c)
-      if (column<kVec>(c, 0, t, tpr) < d) raw[c] = load8(row + column<kVec>(c, 0, t, tpr));
+  for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) r.w[i] = 0u;
+  if constexpr (kVec) {
+    const int col = column<true>(c, 0, t, tpr);
+    if (there && col < d) {
 #pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      if (column<kVec>(c, 0, t, tpr) < d) {
-        unpack8(raw[c], v[c]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[c][j] = 0.0f;
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(row + col)[i];
+        r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
       }
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < kCh; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int col = column<kVec>(c, j, t, tpr);
-        v[c][j] = col < d ? as_float(row[col]) : 0.0f;
+    for (int j = 0; j < 8; ++j) {
+      const int col = column<false>(c, j, t, tpr);
+      if (there && col < d) {
+        if constexpr (sizeof(T) == 2)
+          r.w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(row)[col]) << 16 * (j % 2);
+        else
+          r.w[j] = reinterpret_cast<const uint32_t*>(row)[col];
       }
+    }
   }
+  return r;
+}
+// Rows of 16-byte pieces are copied ahead; in pieces of 4 bytes that does not gain (35 and 42 us against 31 and 36 on 6151
+// rows of 2047 fp32 columns), so other rows are loaded when their turn comes.
+__device__ __forceinline__ void copy_async_16(uint32_t to, const void* from, bool there) {  // zeros where not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+// The handfuls of rows that a thread's group walks, kTensors rows of kCh chunks of 8 columns each.
+template <typename T, int kCh, int kRows, int kTensors>
+struct Ahead {
+  static constexpr int kParts = sizeof(T) / 2;  // 16-byte pieces of 8 elements
+  static constexpr int kPieces = kRows * kTensors * kCh * kParts;
+  static constexpr int kStages = kPieces <= 4 ? 4 : kPieces <= 8 ? 3 : 2;  // up to 192 KB with 512 threads
+  const T* from[kTensors];  // this thread's first column
+  int rows, d, stride;      // columns between chunks
+  int inside;               // chunks that lie in the row
+  uint32_t slot;            // this thread's piece 0 of stage 0; pieces lie blockDim.x * 16 bytes apart
+
+  // Ask for the handful at r0 (nothing but an empty group of copies past the last row).
+  __device__ __forceinline__ void ask(int stage, int r0) const {
+    uint32_t to = slot + stage * (kPieces * 16) * blockDim.x;
+    if (r0 < rows) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const bool row = r0 + k < rows;
+        const long long at = static_cast<long long>(row ? r0 + k : r0) * d;
+#pragma unroll
+        for (int n = 0; n < kTensors; ++n)
+#pragma unroll
+          for (int c = 0; c < kCh; ++c) {
+            const T* p = from[n] + (c < inside ? at + c * stride : 0);
+#pragma unroll
+            for (int part = 0; part < kParts; ++part, to += 16 * blockDim.x)
+              copy_async_16(to, p + part * (16 / sizeof(T)), row && c < inside);
+          }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ Words<T> get(int stage, int k, int n, int c) const {
+    Words<T> r;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const uint32_t at = slot + (stage * kPieces + ((k * kTensors + n) * kCh + c) * kParts + part) * 16 * blockDim.x;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(r.w[4 * part]), "=r"(r.w[4 * part + 1]), "=r"(r.w[4 * part + 2]), "=r"(r.w[4 * part + 3])
+                   : "r"(at)
+                   : "memory");
+    }
+    return r;
+  }
+};
+template <typename T, int kCh, int kRows, int kTensors>
+__device__ __forceinline__ Ahead<T, kCh, kRows, kTensors> ahead_of(const T* a, const T* b, int rows, int d, int t, int tpr,
+                                                                   void* slots) {
+  Ahead<T, kCh, kRows, kTensors> r;
+  int inside = 0;
+  for (int c = 0; c < kCh; ++c) inside += column<true>(c, 0, t, tpr) < d;
+  const int col = inside > 0 ? column<true>(0, 0, t, tpr) : 0;
+  r.from[0] = a + col;
+  if constexpr (kTensors > 1) r.from[1] = b + col;
+  r.rows = rows, r.d = d, r.stride = 8 * tpr, r.inside = inside;
+  r.slot = smem_u32(slots) + threadIdx.x * 16;
+  return r;
 }
 
-template <typename T, int kCh, bool kVec>
-__device__ __forceinline__ void store_row(T* __restrict__ row, int d, int t, int tpr, const float (&v)[kCh][8]) {
-#pragma unroll
-  for (int c = 0; c < kCh; ++c) {
-    if (kVec) {
-      if (column<kVec>(c, 0, t, tpr) < d) store8(row + column<kVec>(c, 0, t, tpr), v[c]);
+template <typename T, bool kVec>
+__device__ __forceinline__ void store_pairs(T* __restrict__ row, int c, int d, int t, int tpr, const f32x2 (&v)[4]) {
+  if constexpr (kVec) {
+    const int col = column<true>(c, 0, t, tpr);
+    if (col >= d) return;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(row + col) = make_uint4(pack_bf16_2(v[0]), pack_bf16_2(v[1]), pack_bf16_2(v[2]), pack_bf16_2(v[3]));
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int col = column<kVec>(c, j, t, tpr);
-        if (col < d) store1(row + col, v[c][j]);
+      for (int i = 0; i < 2; ++i) {
+        const float2 a = unpack2(v[2 * i]), b = unpack2(v[2 * i + 1]);
+        reinterpret_cast<float4*>(row + col)[i] = make_float4(a.x, a.y, b.x, b.y);
       }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = unpack2(v[i]);
+      const int c0 = column<false>(c, 2 * i, t, tpr), c1 = column<false>(c, 2 * i + 1, t, tpr);
+      if (c0 < d) store1(row + c0, a.x);
+      if (c1 < d) store1(row + c1, a.y);
     }
   }
 }
+// Eight parameters in either type (a branch every thread takes alike), `none` where there are none.
+template <bool kVec>
+__device__ __forceinline__ void load_params(const void* p, int fp32, float none, int c, int d, int t, int tpr, f32x2 (&v)[4]) {
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int col = column<kVec>(c, j, t, tpr);
+    x[j] = p == nullptr ? none : 0.0f;
+    if (p != nullptr && col < d)
+      x[j] = fp32 ? static_cast<const float*>(p)[col] : as_float(static_cast<const __nv_bfloat16*>(p)[col]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pk2(x[2 * i], x[2 * i + 1]);
+}
+__device__ __forceinline__ float total_of(f32x2 v) {
+  const float2 a = unpack2(v);
+  return a.x + a.y;
+}
 
-// Sums over the threads of a row; `red` is used in turn (two halves), so one barrier a sum is enough.
-__device__ __forceinline__ float2 row_sum(float2 s, int wpr, float2 (*red)[32], int& turn) {
-  s.x = warp_sum(s.x);
-  s.y = warp_sum(s.y);
-  if (wpr > 1) {
-    float2* r = red[turn & 1];
-    ++turn;
-    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = s;
-    __syncthreads();
-    s = r[0];
-    for (int w = 1; w < wpr; ++w) {
-      s.x += r[w].x;
-      s.y += r[w].y;
+// N sums over the 32 lanes with as few shuffles as there are halves to exchange; lane (j << (5 - log2 N)) ends with sum j.
+template <int N>
+__device__ __forceinline__ float lane_sums(float (&v)[N], int lane) {
+  int o = 16;
+#pragma unroll
+  for (int n = N; n > 1; n /= 2, o /= 2) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float send = upper ? v[i] : v[i + n / 2], keep = upper ? v[i + n / 2] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
     }
   }
+  float s = v[0];
+#pragma unroll
+  for (; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 
-template <typename T, int kCh, bool kVec>
-__global__ void __launch_bounds__(32 * kMaxWarps) layer_norm_fwd_kernel(const T* __restrict__ x, const void* __restrict__ w,
-                                                              const void* __restrict__ b, T* __restrict__ y,
-                                                              float* __restrict__ mean_out, float* __restrict__ rstd_out,
-                                                              long long rows, int d, float eps, int wpr, int p_fp32) {
-  __shared__ float2 red[2][32];
-  const int tpr = 32 * wpr, rpb = blockDim.x / tpr, t = threadIdx.x % tpr;
+// The threads that share rows: `wpr` warps, group `g` of the block.
+struct Group {
+  int wpr, g, t, tpr, lane, warp;  // warp: of the group
+  float* red;                      // [2][wpr][8], used in turn, so one barrier a sum is enough
+  int turn;
+  // v[j] becomes its sum over the group's threads.
+  template <int N>
+  __device__ __forceinline__ void sum(float (&v)[N]) {
+    constexpr int kShift = N == 8 ? 2 : N == 4 ? 3 : N == 2 ? 4 : 5;
+    const float s = lane_sums(v, lane);
+    if (wpr == 1) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = __shfl_sync(0xffffffffu, s, j << kShift);
+      return;
+    }
+    float* r = red + turn * wpr * 8;
+    turn ^= 1;
+    if ((lane & ((1 << kShift) - 1)) == 0) r[warp * 8 + (lane >> kShift)] = s;
+    asm volatile("barrier.sync %0, %1;" ::"r"(g + 1), "r"(tpr) : "memory");
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = r[j];
+    for (int w = 1; w < wpr; ++w) {
+      float e[N];
+      if constexpr (N >= 4) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(r + w * 8 + j);
+          e[j] = q.x, e[j + 1] = q.y, e[j + 2] = q.z, e[j + 3] = q.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) e[j] = r[w * 8 + j];
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] += e[j];
+    }
+  }
+};
+__device__ __forceinline__ Group group_of(int wpr, float* red) {
+  const int warp = threadIdx.x >> 5, g = warp / wpr;
+  return Group{wpr, g, static_cast<int>(threadIdx.x) - g * 32 * wpr, 32 * wpr, static_cast<int>(threadIdx.x & 31), warp - g * wpr,
+               red + g * 2 * wpr * 8, 0};
+}
+
+// kRows rows a group at a time.
+template <typename T, int kCh, int kRows, bool kVec>
+__global__ void __launch_bounds__(32 * kMaxWarps) layer_norm_fwd_kernel(
+    const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, T* __restrict__ y,
+    float* __restrict__ mean_out, float* __restrict__ rstd_out, int rows, int d, float eps, int wpr, int p_fp32) {
+  extern __shared__ __align__(16) uint8_t slots[];
+  __shared__ __align__(16) float red[kMaxWarps * 16];
+  Group group = group_of(wpr, red);
+  const int t = group.t, tpr = group.tpr, groups = blockDim.x / tpr;
   const float inv_d = 1.0f / static_cast<float>(d);
-  int turn = 0;
-  for (long long r = static_cast<long long>(blockIdx.x) * rpb + threadIdx.x / tpr; r < rows;
-       r += static_cast<long long>(gridDim.x) * rpb) {
-    float v[kCh][8];
-    load_row<T, kCh, kVec>(x + r * d, d, t, tpr, v);
-    float2 s = make_float2(0.0f, 0.0f);
+  const int first = (blockIdx.x * groups + group.g) * kRows, step = gridDim.x * groups * kRows;
+  using Copies = Ahead<T, kCh, kRows, 1>;
+  constexpr int kStages = Copies::kStages;
+  const Copies ahead = ahead_of<T, kCh, kRows, 1>(x, nullptr, rows, d, t, tpr, slots);
+  if constexpr (kVec)
+    for (int i = 0; i < kStages - 1; ++i) ahead.ask(i, first + i * step);
+  f32x2 scale[kCh][4], shift[kCh][4];
 #pragma unroll
-    for (int c = 0; c < kCh; ++c)
+  for (int c = 0; c < kCh; ++c) {
+    load_params<kVec>(w, p_fp32, 1.0f, c, d, t, tpr, scale[c]);
+    load_params<kVec>(b, p_fp32, 0.0f, c, d, t, tpr, shift[c]);
+  }
+  int stage = 0;
+  for (int r0 = first; r0 < rows; r0 += step) {
+    f32x2 v[kRows][kCh][4];
+    float s[kRows];
+    if constexpr (kVec) asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s.x += v[c][j];
-    const float mean = row_sum(s, wpr, red, turn).x * inv_d;
-    s = make_float2(0.0f, 0.0f);
+    for (int k = 0; k < kRows; ++k) {
+      f32x2 a = 0ull;
 #pragma unroll
-    for (int c = 0; c < kCh; ++c)
+      for (int c = 0; c < kCh; ++c) {
+        const Words<T> words = kVec ? ahead.get(stage, k, 0, c)
+                                    : load_words<T, kVec>(x + static_cast<long long>(r0 + k) * d, c, d, t, tpr, r0 + k < rows);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (column<kVec>(c, j, t, tpr) < d) {
-          v[c][j] -= mean;
-          s.x += v[c][j] * v[c][j];
-        }
-    const float rstd = rsqrtf(row_sum(s, wpr, red, turn).x * inv_d + eps);
-    if (t == 0 && mean_out != nullptr) {
-      mean_out[r] = mean;
-      rstd_out[r] = rstd;
-    }
-#pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      float wv[8], bv[8];
-      // the parameters are read again for every row: they stay in L1
-      if (kVec) {
-        const int col = column<kVec>(c, 0, t, tpr);
-        if (col < d) {
-          if (w != nullptr) params8(w, p_fp32, col, wv);
-          if (b != nullptr) params8(b, p_fp32, col, bv);
+        for (int i = 0; i < 4; ++i) {
+          v[k][c][i] = words.pair(i);
+          a = add2(a, v[k][c][i]);
         }
       }
+      s[k] = total_of(a);
+    }
+    if constexpr (kVec) {
+      ahead.ask((stage + kStages - 1) % kStages, r0 + (kStages - 1) * step);
+      stage = (stage + 1) % kStages;
+    }
+    group.sum(s);
+    float mean[kRows];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int col = column<kVec>(c, j, t, tpr);
-        if (col >= d) continue;
-        const float scale = w == nullptr ? 1.0f : kVec ? wv[j] : param1(w, p_fp32, col);
-        const float shift = b == nullptr ? 0.0f : kVec ? bv[j] : param1(b, p_fp32, col);
-        v[c][j] = v[c][j] * rstd * scale + shift;
+    for (int k = 0; k < kRows; ++k) {
+      mean[k] = s[k] * inv_d;
+      const f32x2 neg = pk2(-mean[k], -mean[k]);
+      s[k] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kCh; ++c) {
+        f32x2 a = 0ull;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[k][c][i] = add2(v[k][c][i], neg);
+          if constexpr (!kVec) {
+            const float2 e = unpack2(v[k][c][i]);
+            v[k][c][i] = pk2(column<kVec>(c, 2 * i, t, tpr) < d ? e.x : 0.0f, column<kVec>(c, 2 * i + 1, t, tpr) < d ? e.y : 0.0f);
+          }
+          a = fma2(v[k][c][i], v[k][c][i], a);
+        }
+        s[k] += !kVec || column<kVec>(c, 0, t, tpr) < d ? total_of(a) : 0.0f;
       }
     }
-    store_row<T, kCh, kVec>(y + r * d, d, t, tpr, v);
+    group.sum(s);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (r0 + k >= rows) break;
+      const float rstd = rsqrtf(s[k] * inv_d + eps);
+      if (t == 0 && mean_out != nullptr) {
+        mean_out[r0 + k] = mean[k];
+        rstd_out[r0 + k] = rstd;
+      }
+      const f32x2 r2 = pk2(rstd, rstd);
+#pragma unroll
+      for (int c = 0; c < kCh; ++c) {
+        f32x2 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = fma2(mul2(v[k][c][i], r2), scale[c][i], shift[c][i]);
+        store_pairs<T, kVec>(y + static_cast<long long>(r0 + k) * d, c, d, t, tpr, o);
+      }
+    }
   }
 }
 
-template <typename T, int kCh, bool kVec, bool kParams>
+template <typename T, int kCh, int kRows, bool kVec, bool kParams>
 __global__ void __launch_bounds__(32 * kMaxWarps) layer_norm_bwd_kernel(
     const T* __restrict__ x, const void* __restrict__ w, const T* __restrict__ dy, const float* __restrict__ mean_in,
-    const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ partial, long long rows, int d, int wpr,
-    int p_fp32) {
-  extern __shared__ float sums[];  // [2][d], where warps of a block share columns
-  __shared__ float2 red[2][32];
-  const int tpr = 32 * wpr, rpb = blockDim.x / tpr, t = threadIdx.x % tpr;
+    const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ partial, int rows, int d, int wpr, int p_fp32) {
+  extern __shared__ __align__(16) uint8_t slots[];
+  float* sums = reinterpret_cast<float*>(slots);  // at the end: [2][d], where groups of a block share columns
+  __shared__ __align__(16) float red[kMaxWarps * 16];
+  Group group = group_of(wpr, red);
+  const int t = group.t, tpr = group.tpr, groups = blockDim.x / tpr;
   const float inv_d = 1.0f / static_cast<float>(d);
-  float dw[kCh][8], db[kCh][8];
+  const int first = (blockIdx.x * groups + group.g) * kRows, step = gridDim.x * groups * kRows;
+  using Copies = Ahead<T, kCh, kRows, 2>;
+  constexpr int kStages = Copies::kStages;
+  const Copies ahead = ahead_of<T, kCh, kRows, 2>(x, dy, rows, d, t, tpr, slots);
+  if constexpr (kVec)
+    for (int i = 0; i < kStages - 1; ++i) ahead.ask(i, first + i * step);
+  f32x2 scale[kCh][4], dw[kCh][4], db[kCh][4];
 #pragma unroll
-  for (int c = 0; c < kCh; ++c)
+  for (int c = 0; c < kCh; ++c) {
+    load_params<kVec>(w, p_fp32, 1.0f, c, d, t, tpr, scale[c]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[c][j] = db[c][j] = 0.0f;
-  int turn = 0;
-  for (long long r = static_cast<long long>(blockIdx.x) * rpb + threadIdx.x / tpr; r < rows;
-       r += static_cast<long long>(gridDim.x) * rpb) {
-    float xh[kCh][8], g[kCh][8];
-    load_row<T, kCh, kVec>(x + r * d, d, t, tpr, xh);
-    load_row<T, kCh, kVec>(dy + r * d, d, t, tpr, g);
-    const float mean = mean_in[r], rstd = rstd_in[r];
-    float2 s = make_float2(0.0f, 0.0f);
+    for (int i = 0; i < 4; ++i) dw[c][i] = db[c][i] = 0ull;
+  }
+  int stage = 0;
+  float next_mean[kRows], next_rstd[kRows];
+  auto ask_stats = [&](int r0) {
 #pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      float wv[8];
-      if (kVec && w != nullptr && column<kVec>(c, 0, t, tpr) < d) params8(w, p_fp32, column<kVec>(c, 0, t, tpr), wv);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int col = column<kVec>(c, j, t, tpr);
-        if (col >= d) continue;
-        xh[c][j] = (xh[c][j] - mean) * rstd;
-        if (kParams) {
-          dw[c][j] += g[c][j] * xh[c][j];
-          db[c][j] += g[c][j];
-        }
-        g[c][j] *= w == nullptr ? 1.0f : kVec ? wv[j] : param1(w, p_fp32, col);
-        s.x += g[c][j];
-        s.y += g[c][j] * xh[c][j];
-      }
+    for (int k = 0; k < kRows; ++k) {
+      next_mean[k] = r0 + k < rows ? mean_in[r0 + k] : 0.0f;
+      next_rstd[k] = r0 + k < rows ? rstd_in[r0 + k] : 0.0f;
     }
-    s = row_sum(s, wpr, red, turn);
-    if (dx != nullptr) {
-      const float m1 = s.x * inv_d, m2 = s.y * inv_d;
+  };
+  ask_stats(first);
+  for (int r0 = first; r0 < rows; r0 += step) {
+    f32x2 xh[kRows][kCh][4], g[kRows][kCh][4];
+    float rstd[kRows], s[2 * kRows];
+    if constexpr (kVec) asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    // outside the row dy reads as zero, and with it all that is summed
 #pragma unroll
-      for (int c = 0; c < kCh; ++c)
+    for (int k = 0; k < kRows; ++k) {
+      rstd[k] = next_rstd[k];
+      const f32x2 neg = pk2(-next_mean[k], -next_mean[k]), r2 = pk2(rstd[k], rstd[k]);
+      f32x2 s1 = 0ull, s2 = 0ull;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[c][j] = rstd * (g[c][j] - m1 - xh[c][j] * m2);
-      store_row<T, kCh, kVec>(dx + r * d, d, t, tpr, g);
+      for (int c = 0; c < kCh; ++c) {
+        const long long at = static_cast<long long>(r0 + k) * d;
+        const Words<T> vx = kVec ? ahead.get(stage, k, 0, c) : load_words<T, kVec>(x + at, c, d, t, tpr, r0 + k < rows);
+        const Words<T> vy = kVec ? ahead.get(stage, k, 1, c) : load_words<T, kVec>(dy + at, c, d, t, tpr, r0 + k < rows);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x2 e = vy.pair(i);
+          xh[k][c][i] = mul2(add2(vx.pair(i), neg), r2);
+          g[k][c][i] = mul2(e, scale[c][i]);
+          if (kParams) {
+            dw[c][i] = fma2(e, xh[k][c][i], dw[c][i]);
+            db[c][i] = add2(db[c][i], e);
+          }
+          s1 = add2(s1, g[k][c][i]);
+          s2 = fma2(g[k][c][i], xh[k][c][i], s2);
+        }
+      }
+      s[2 * k] = total_of(s1);
+      s[2 * k + 1] = total_of(s2);
+    }
+    ask_stats(r0 + step);
+    if constexpr (kVec) {
+      ahead.ask((stage + kStages - 1) % kStages, r0 + (kStages - 1) * step);
+      stage = (stage + 1) % kStages;
+    }
+    if (dx == nullptr) continue;
+    group.sum(s);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (r0 + k >= rows) break;
+      const float m1 = -s[2 * k] * inv_d, m2 = -s[2 * k + 1] * inv_d;
+      const f32x2 r2 = pk2(rstd[k], rstd[k]), m1_2 = pk2(m1, m1), m2_2 = pk2(m2, m2);
+#pragma unroll
+      for (int c = 0; c < kCh; ++c) {
+        f32x2 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = mul2(r2, fma2(xh[k][c][i], m2_2, add2(g[k][c][i], m1_2)));
+        store_pairs<T, kVec>(dx + static_cast<long long>(r0 + k) * d, c, d, t, tpr, o);
+      }
     }
   }
   if (kParams) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // nothing is on its way to the slots, which the sums take over
     float* out = partial + static_cast<long long>(blockIdx.x) * 2 * d;
-    if (wpr > 1) {
+    float* to = groups > 1 ? sums : out;
+    for (int turn = 0; turn < groups; ++turn) {  // the groups add their sums in order
+      if (group.g == turn) {
 #pragma unroll
-      for (int c = 0; c < kCh; ++c)
+        for (int c = 0; c < kCh; ++c)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int col = column<kVec>(c, j, t, tpr);
-          if (col < d) {
-            out[col] = dw[c][j];
-            out[d + col] = db[c][j];
-          }
-        }
-    } else {
-      for (int turn_of = 0; turn_of < rpb; ++turn_of) {  // the warps add their sums in order
-        if (static_cast<int>(threadIdx.x >> 5) == turn_of) {
+          for (int i = 0; i < 4; ++i) {
+            const float2 a = unpack2(dw[c][i]), e = unpack2(db[c][i]);
 #pragma unroll
-          for (int c = 0; c < kCh; ++c)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int col = column<kVec>(c, j, t, tpr);
+            for (int h = 0; h < 2; ++h) {
+              const int col = column<kVec>(c, 2 * i + h, t, tpr);
               if (col < d) {
-                sums[col] = (turn_of ? sums[col] : 0.0f) + dw[c][j];
-                sums[d + col] = (turn_of ? sums[d + col] : 0.0f) + db[c][j];
+                to[col] = (turn ? to[col] : 0.0f) + (h ? a.y : a.x);
+                to[d + col] = (turn ? to[d + col] : 0.0f) + (h ? e.y : e.x);
               }
             }
-        }
-        __syncthreads();
+          }
       }
-      for (int i = threadIdx.x; i < 2 * d; i += blockDim.x) out[i] = sums[i];
+      if (groups > 1) __syncthreads();
     }
+    if (groups > 1)
+      for (int i = threadIdx.x; i < 2 * d; i += blockDim.x) out[i] = sums[i];
   }
 }
 
@@ -259,19 +462,24 @@ __global__ void __launch_bounds__(1024) layer_norm_params_kernel(const float* __
   }
 }
 
+// How rows are spread: the fewest warps whose threads hold a row of up to 4096 columns 8 a thread, or of up to 8192 and
+// 12,288 in two and three chunks; as many groups as make 256 to 512 threads a block.
 struct Shape {
-  int wpr, ch;
+  int wpr, ch, groups;
 };
-// A warp a row up to 768 columns; then the fewest warps whose threads hold the row in two chunks, or three at the most warps.
 inline Shape shape_of(int d) {
-  int wpr = 1;
-  if (d > 256 * kMaxChunks)
-    while (wpr < kMaxWarps && d > 512 * wpr) wpr *= 2;
-  return {wpr, (d + 256 * wpr - 1) / (256 * wpr)};
+  const int ch = (d + 256 * kMaxWarps - 1) / (256 * kMaxWarps);
+  const int wpr = (d + 256 * ch - 1) / (256 * ch);
+  return {wpr, ch, std::max(1, std::min(kMaxGroups, kMaxWarps / wpr))};
+}
+// Rows a group at a time: fewer where they would not fit registers or the room for copies, or with so many warps a row that
+// their sums cost more than the barriers saved.
+inline int rows_of(const Shape& s, bool fp32, bool backward) {
+  return s.ch > 1 ? 1 : s.wpr > 8 || (fp32 && backward) ? 2 : 4;
 }
 
-// Blocks that fit the machine at once, at most one a row (or a row group). What fits an SM is asked once a kernel and
-// block size (`fit`, zero at first; the answer is the same whoever writes it).
+// Blocks that fit the machine at once, at most one a handful of rows. What fits an SM is asked once a kernel and block
+// size (`fit`, zero at first; the answer is the same whoever writes it).
 template <typename K>
 inline int grid_for(K kern, int* fit, int threads, size_t smem, long long rows, int rpb) {
   int& per_sm = fit[threads / 32];
@@ -282,30 +490,47 @@ inline int grid_for(K kern, int* fit, int threads, size_t smem, long long rows, 
   return static_cast<int>(std::min<long long>((rows + rpb - 1) / rpb, 148ll * per_sm));
 }
 
-template <typename T, int kCh, bool kVec>
+template <typename T, int kCh, int kRows, int kTensors, bool kVec>
+inline size_t slots_bytes(int threads) {
+  using Copies = Ahead<T, kCh, kRows, kTensors>;
+  return kVec ? static_cast<size_t>(Copies::kStages) * Copies::kPieces * threads * 16 : 0;
+}
+// The blocks of a kernel that walks rows, or 0; `fit` as for grid_for.
+template <typename K>
+inline int prepare(K kern, int* fit, int threads, size_t smem, long long rows, int rpb) {
+  if (fit[threads / 32] == 0 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024) != cudaSuccess)
+    return 0;
+  return grid_for(kern, fit, threads, smem, rows, rpb);
+}
+
+template <typename T, int kCh, int kRows, bool kVec>
 int fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, long long rows, int d, float eps,
-        int wpr, int p_fp32, cudaStream_t st) {
-  const int threads = wpr == 1 ? 32 * kWarpsPerBlock : 32 * wpr;
-  auto kern = layer_norm_fwd_kernel<T, kCh, kVec>;
+        Shape s, int p_fp32, cudaStream_t st) {
+  const int threads = 32 * s.wpr * s.groups;
+  const size_t smem = slots_bytes<T, kCh, kRows, 1, kVec>(threads);
+  auto kern = layer_norm_fwd_kernel<T, kCh, kRows, kVec>;
   static int fit[kMaxWarps + 1];
-  const int grid = grid_for(kern, fit, threads, 0, rows, threads / (32 * wpr));
+  const int grid = prepare(kern, fit, threads, smem, rows, kRows * s.groups);
   if (grid == 0) return 2;
-  kern<<<grid, threads, 0, st>>>(static_cast<const T*>(x), w, b, static_cast<T*>(y), mean, rstd, rows, d, eps, wpr, p_fp32);
+  kern<<<grid, threads, smem, st>>>(static_cast<const T*>(x), w, b, static_cast<T*>(y), mean, rstd, static_cast<int>(rows), d, eps, s.wpr,
+                                    p_fp32);
   return cudaGetLastError() == cudaSuccess ? 0 : 1;
 }
 
-template <typename T, int kCh, bool kVec, bool kParams>
+template <typename T, int kCh, int kRows, bool kVec, bool kParams>
 int bwd(const void* x, const void* w, const void* dy, const float* mean, const float* rstd, void* dx, void* dw, void* db,
-        float* partial, int max_blocks, long long rows, int d, int wpr, int p_fp32, cudaStream_t st) {
-  const int threads = wpr == 1 ? 32 * kWarpsPerBlock : 32 * wpr;
-  const size_t smem = kParams && wpr == 1 ? static_cast<size_t>(2 * d) * sizeof(float) : 0;
-  auto kern = layer_norm_bwd_kernel<T, kCh, kVec, kParams>;
+        float* partial, int max_blocks, long long rows, int d, Shape s, int p_fp32, cudaStream_t st) {
+  const int threads = 32 * s.wpr * s.groups;
+  const size_t sums = kParams && s.groups > 1 ? static_cast<size_t>(16 * s.wpr * 256) : 0;  // 2 d floats and more
+  const size_t smem = std::max(sums, slots_bytes<T, kCh, kRows, 2, kVec>(threads));
+  auto kern = layer_norm_bwd_kernel<T, kCh, kRows, kVec, kParams>;
   static int fit[kMaxWarps + 1];
-  int grid = grid_for(kern, fit, threads, smem, rows, threads / (32 * wpr));
+  int grid = prepare(kern, fit, threads, smem, rows, kRows * s.groups);
   if (grid == 0) return 2;
-  grid = std::min(grid, max_blocks);
+  if (kParams) grid = std::min(grid, max_blocks);
   kern<<<grid, threads, smem, st>>>(static_cast<const T*>(x), w, static_cast<const T*>(dy), mean, rstd,
-                                    static_cast<T*>(dx), partial, rows, d, wpr, p_fp32);
+                                    static_cast<T*>(dx), partial, static_cast<int>(rows), d, s.wpr, p_fp32);
   if (cudaGetLastError() != cudaSuccess) return 1;
   if (!kParams) return 0;
   const dim3 blocks((2 * d + 31) / 32);
@@ -319,20 +544,25 @@ int bwd(const void* x, const void* w, const void* dy, const float* mean, const f
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// The kernel for (chunks, rows at a time).
 template <typename T, bool kVec, typename... A>
-int fwd_ch(int ch, A... a) {
-  return ch == 1 ? fwd<T, 1, kVec>(a...) : ch == 2 ? fwd<T, 2, kVec>(a...) : fwd<T, 3, kVec>(a...);
+int fwd_rows(int ch, int n, A... a) {
+  if (ch == 2) return fwd<T, 2, 1, kVec>(a...);
+  if (ch == 3) return fwd<T, 3, 1, kVec>(a...);
+  return n == 4 ? fwd<T, 1, 4, kVec>(a...) : fwd<T, 1, 2, kVec>(a...);
 }
 template <typename T, bool kVec, bool kParams, typename... A>
-int bwd_ch(int ch, A... a) {
-  return ch == 1   ? bwd<T, 1, kVec, kParams>(a...)
-         : ch == 2 ? bwd<T, 2, kVec, kParams>(a...)
-                   : bwd<T, 3, kVec, kParams>(a...);
+int bwd_rows(int ch, int n, A... a) {
+  if (ch == 2) return bwd<T, 2, 1, kVec, kParams>(a...);
+  if (ch == 3) return bwd<T, 3, 1, kVec, kParams>(a...);
+  if constexpr (sizeof(T) == 2)
+    if (n == 4) return bwd<T, 1, 4, kVec, kParams>(a...);
+  return bwd<T, 1, 2, kVec, kParams>(a...);
 }
 template <typename T, typename... A>
-int bwd_all(bool vec, bool params, int ch, A... a) {
-  if (params) return vec ? bwd_ch<T, true, true>(ch, a...) : bwd_ch<T, false, true>(ch, a...);
-  return vec ? bwd_ch<T, true, false>(ch, a...) : bwd_ch<T, false, false>(ch, a...);
+int bwd_all(bool vec, bool params, int ch, int n, A... a) {
+  if (params) return vec ? bwd_rows<T, true, true>(ch, n, a...) : bwd_rows<T, false, true>(ch, n, a...);
+  return vec ? bwd_rows<T, true, false>(ch, n, a...) : bwd_rows<T, false, false>(ch, n, a...);
 }
 
 }  // namespace
@@ -341,21 +571,21 @@ int bwd_all(bool vec, bool params, int ch, A... a) {
 extern "C" int pd_layer_norm_max_columns() { return 256 * kMaxWarps * kMaxChunks; }
 extern "C" int pd_layer_norm_partial_rows(long long rows, int d) {
   const Shape s = shape_of(d);
-  const int rpb = s.wpr == 1 ? kWarpsPerBlock : 1;
-  return static_cast<int>(std::min<long long>((rows + rpb - 1) / rpb, 148ll * std::max(1, 16 / std::max(8, s.wpr))));
+  return static_cast<int>(std::min<long long>((rows + s.groups - 1) / s.groups, 148ll * 4));
 }
 
 // x, y [rows, d] contiguous in bf16 or fp32 (x_fp32); w, b [d] or null, of one type (p_fp32). mean, rstd [rows] or null.
 extern "C" int pd_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd,
                                  long long rows, int d, float eps, int x_fp32, int p_fp32, void* stream) {
-  if (rows <= 0 || d <= 0 || d > pd_layer_norm_max_columns() || (mean == nullptr) != (rstd == nullptr)) return 5;
+  if (rows <= 0 || rows >= (1ll << 30) || d <= 0 || d > pd_layer_norm_max_columns() || (mean == nullptr) != (rstd == nullptr)) return 5;
   const Shape s = shape_of(d);
-  const bool vec = d % 8 == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
+  const bool vec = d % 8 == 0 && aligned16(x) && aligned16(y);
+  const int n = rows_of(s, x_fp32, false);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = [&](auto t) {
     using T = decltype(t);
-    return vec ? fwd_ch<T, true>(s.ch, x, w, b, y, mean, rstd, rows, d, eps, s.wpr, p_fp32, st)
-               : fwd_ch<T, false>(s.ch, x, w, b, y, mean, rstd, rows, d, eps, s.wpr, p_fp32, st);
+    return vec ? fwd_rows<T, true>(s.ch, n, x, w, b, y, mean, rstd, rows, d, eps, s, p_fp32, st)
+               : fwd_rows<T, false>(s.ch, n, x, w, b, y, mean, rstd, rows, d, eps, s, p_fp32, st);
   };
   return x_fp32 ? go(float()) : go(__nv_bfloat16());
 }
@@ -365,16 +595,15 @@ extern "C" int pd_layer_norm_fwd(const void* x, const void* w, const void* b, vo
 extern "C" int pd_layer_norm_bwd(const void* x, const void* w, const void* dy, const float* mean, const float* rstd,
                                  void* dx, void* dw, void* db, float* partial, long long rows, int d, int x_fp32,
                                  int p_fp32, void* stream) {
-  if (rows <= 0 || d <= 0 || d > pd_layer_norm_max_columns()) return 5;
+  if (rows <= 0 || rows >= (1ll << 30) || d <= 0 || d > pd_layer_norm_max_columns()) return 5;
   const bool params = dw != nullptr || db != nullptr;
   if (params && partial == nullptr) return 5;
   const Shape s = shape_of(d);
-  const bool vec = d % 8 == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(w);
-  const int blocks = pd_layer_norm_partial_rows(rows, d);
+  const bool vec = d % 8 == 0 && aligned16(x) && aligned16(dy) && aligned16(dx);
+  const int n = rows_of(s, x_fp32, true), blocks = pd_layer_norm_partial_rows(rows, d);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = [&](auto t) {
-    return bwd_all<decltype(t)>(vec, params, s.ch, x, w, dy, mean, rstd, dx, dw, db, partial, blocks, rows, d, s.wpr,
-                                p_fp32, st);
+    return bwd_all<decltype(t)>(vec, params, s.ch, n, x, w, dy, mean, rstd, dx, dw, db, partial, blocks, rows, d, s, p_fp32, st);
   };
   return x_fp32 ? go(float()) : go(__nv_bfloat16());
 }

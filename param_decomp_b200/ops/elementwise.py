@@ -251,6 +251,8 @@ def layer_norm(x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Ten
         raise ValueError(f"layer_norm: {x.dtype} is not bf16 or fp32")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= LAYER_NORM_MAX_COLUMNS:
         raise ValueError(f"layer_norm: rows of 1 to {LAYER_NORM_MAX_COLUMNS} columns, not {tuple(x.shape)}")
+    if x.numel() >= x.shape[-1] << 30:
+        raise ValueError(f"layer_norm: fewer than 2^30 rows, not {tuple(x.shape)}")
     for p in (w, b):
         if p is not None and (p.dim() != 1 or p.shape[0] != x.shape[-1] or p.dtype not in _FLOAT):
             raise ValueError(f"layer_norm: scale and shift are [{x.shape[-1]}] in bf16 or fp32, not {tuple(p.shape)} {p.dtype}")
