@@ -3,13 +3,15 @@
 // rows once and writes every row of the table (most of them zeros).
 //
 // The gradient sums each row in fp32 over its tokens in ascending order and rounds once, with two launches and no float
-// atomics. First kernel: block b owns a span of the vocabulary. Its 32 warps walk all tokens, each its own consecutive
-// part: once to count the block's tokens by id and warp (and the valid tokens of lower ids, which gives the block's place
-// in the sorted order without asking the other blocks), once more to write each token's place in that order (a stable
-// counting sort: id, then warp, then position). All blocks read all tokens, from L2. The block then writes the zero rows
-// of its span and sums the rows of ids with up to kSlab tokens. Second kernel: ids with more tokens, in slabs of kSlab
-// places of the sorted order, so a token that fills a tenth of the batch is shared by many blocks; a slab's sum goes to
-// scratch and the block that finishes a run last adds its slabs in their order.
+// atomics. First kernel: block b owns a span of the vocabulary. Its 32 warps read all tokens (from L2, as the lookup left
+// them in 32 bits), each its own consecutive part, note those of the block and count the valid tokens of lower ids, which
+// gives the block's place in the sorted order without asking the other blocks. The noted ones are sorted by counting: id,
+// then warp, then position, and rows of up to kSlab tokens are summed. Second kernel: ids with more tokens, in slabs of
+// kSlab places of the sorted order, so a token that fills a tenth of the batch is shared by many blocks; a slab's sum goes
+// to scratch and the block that finishes a run last adds its slabs in their order. Rows of dy come in no order that a cache
+// could guess, so the block that finds a token asks for its row in L2 at once, long before it is summed. The rows without a token, most of the
+// bytes, are written by blocks of the second kernel too: zeros at the full rate in the first one made the loads of its sums
+// wait for several microseconds each (32,768 tokens in 50,277 rows of 768: 77 us).
 #include <algorithm>
 
 #include "rows.cuh"
@@ -22,6 +24,8 @@ constexpr int kSlab = 32;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxSpan = 1280;  // ids a block: 32 counts of 4 bytes each in shared memory
+constexpr int kNoted = 128;     // tokens a warp notes; where there are more, it reads its part again
+constexpr int kRunThreads = 384;
 
 __device__ __forceinline__ long long token_at(const void* tokens, int wide, long long i) {
   return wide ? static_cast<const long long*>(tokens)[i] : static_cast<const int*>(tokens)[i];
@@ -32,8 +36,9 @@ __device__ __forceinline__ long long token_at(const void* tokens, int wide, long
 template <typename P, typename T, bool kVec>
 __global__ void __launch_bounds__(256) embedding_lookup_kernel(const void* __restrict__ tokens, int wide,
                                                                const P* __restrict__ table, T* __restrict__ y,
-                                                               long long n, long long V, int d, float scale,
-                                                               int* __restrict__ status, int* __restrict__ refused) {
+                                                               int* __restrict__ ids, long long n, long long V, int d,
+                                                               float scale, int* __restrict__ status,
+                                                               int* __restrict__ refused) {
   constexpr int kRowsAhead = 4;
   const int lane = threadIdx.x & 31;
   const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x / 32);
@@ -46,6 +51,7 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const void* __res
       const bool known = t >= 0 && t < V;
       bad |= !known && r0 + k < n;
       src[k] = known ? table + t * d : nullptr;
+      if (lane == 0 && ids != nullptr && r0 + k < n) ids[r0 + k] = known ? static_cast<int>(t) : -1;
     }
     if (bad && lane == 0) {
       atomicCAS(status, 0, kBadToken);
@@ -85,46 +91,190 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const void* __res
 
 // ---- gradient ----------------------------------------------------------------------------------------------------
 struct Runs {        // what the first kernel tells the second
-  int* order;        // [n] position of the token at each place of the sorted order
+  int* order;        // [n] position of the token at each place of the sorted order, where its id has more than kSlab
   int* run_start;    // [n] place where the run of an id with more than kSlab tokens starts, at each of its places; else -1
   int* id;           // [slabs] of the run that starts in the slab (a longer run than a slab: at most one does)
   int* end;          // [slabs] place behind it
   int* done;         // [slabs] slabs of it that are summed
+  uint8_t* empty;    // [V] the id has no token
 };
 
+// Zeros in a row, by one warp: whole 16-byte pieces, the ends element by element.
+template <typename P>
+__device__ __forceinline__ void write_zeros(P* to, int count, int lane) {
+  const int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(to) & 15)) % 16 / sizeof(P));
+  const int first = min(head, count), pieces = (count - first) * static_cast<int>(sizeof(P)) / 16;
+  const int rest = first + pieces * 16 / static_cast<int>(sizeof(P));
+  if (lane < first) store1(to + lane, 0.0f);
+  if (rest + lane < count) store1(to + rest + lane, 0.0f);  // fewer than 16 bytes
+  uint4* p = reinterpret_cast<uint4*>(to + first);
+  for (int i = lane; i < pieces; i += 32) p[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// One warp: scale times rows of dy, each in one piece of 256 columns; lane u names the u-th row, its place in the table and
+// its first column (d: none). All of their loads are in flight together.
+constexpr int kItems = 4;
 template <typename T, typename P, bool kVec>
-__global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const void* __restrict__ tokens, int wide,
-                                                                      const T* __restrict__ dy, P* __restrict__ dE,
-                                                                      int n, long long V, int d, float scale, int span,
-                                                                      Runs runs) {
-  extern __shared__ int hist[];  // [kSortWarps][span] counts, then next places; behind it [span] counts of the ids
-  int* count = hist + kSortWarps * span;
-  __shared__ int warp_total[kSortWarps], below_of[kSortWarps];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long lo = static_cast<long long>(blockIdx.x) * span;
-  const int ids = static_cast<int>(min(static_cast<long long>(span), V - lo));
-  for (int i = tid; i < kSortWarps * span; i += kSortThreads) hist[i] = 0;
-  __syncthreads();
-  const int part = (n + kSortThreads - 1) / kSortThreads * 32;  // tokens a warp
-  const int from = min(n, warp * part), to = min(n, from + part);
-  int* mine = hist + warp * span;
-  int below = 0;
-#pragma unroll 8
-  for (int i = from + lane; i < to; i += 32) {
-    const long long t = token_at(tokens, wide, i);
-    below += t >= 0 && t < lo;
-    if (t >= lo && t < lo + ids) atomicAdd(mine + (t - lo), 1);
+__device__ __forceinline__ void copy_rows(const T* __restrict__ dy, P* __restrict__ dE, int from, int to, int c0, int d,
+                                          float scale, int lane) {
+  Raw8<T> raw[kVec ? kItems : 1];
+  float v[kVec ? 1 : kItems][8];
+#pragma unroll
+  for (int u = 0; u < kItems; ++u) {
+    const T* row = dy + static_cast<long long>(__shfl_sync(0xffffffffu, from, u)) * d;
+    const int col = __shfl_sync(0xffffffffu, c0, u) + (kVec ? 8 * lane : lane);
+    if constexpr (kVec) {
+      if (col < d) raw[u] = load8(row + col);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[u][j] = col + 32 * j < d ? as_float(row[col + 32 * j]) : 0.0f;
+    }
   }
+#pragma unroll
+  for (int u = 0; u < kItems; ++u) {
+    P* out = dE + static_cast<long long>(__shfl_sync(0xffffffffu, to, u)) * d;
+    const int col = __shfl_sync(0xffffffffu, c0, u) + (kVec ? 8 * lane : lane);
+    if constexpr (kVec) {
+      float e[8];
+      if (col < d) {
+        unpack8(raw[u], e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] *= scale;
+        store8(out + col, e);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + 32 * j < d) store1(out + col + 32 * j, v[u][j] * scale);
+    }
+  }
+}
+
+// One warp: scale times the sum of k rows of dy, the r-th at lane r's `row_of`, over 256 columns from c0; the loads of eight
+// bf16 rows or four fp32 rows are in flight (two, element by element, where rows are not of 16-byte pieces).
+template <typename T, typename P, bool kVec>
+__device__ __forceinline__ void sum_rows(const T* __restrict__ dy, int row_of, int k, P* out, int c0, int d, float scale,
+                                         int lane) {
+  constexpr int kRows = kVec ? 16 / sizeof(T) : 2;
+  const int col = kVec ? c0 + 8 * lane : c0 + lane;
+  float acc[8] = {};
+#pragma unroll 1
+  for (int r = 0; r < k; r += kRows) {
+    Raw8<T> raw[kVec ? kRows : 1];
+    float v[kVec ? 1 : kRows][8];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const T* row = dy + static_cast<long long>(__shfl_sync(0xffffffffu, row_of, min(r + u, k - 1))) * d;
+      if constexpr (kVec) {
+        if (col < d && r + u < k) raw[u] = load8(row + col);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u][j] = col + 32 * j < d && r + u < k ? as_float(row[col + 32 * j]) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      if constexpr (kVec) {
+        if (col < d && r + u < k) {
+          float e[8];
+          unpack8(raw[u], e);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += e[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += v[u][j];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] *= scale;
+  if constexpr (kVec) {
+    if (col < d) store8(out + col, acc);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (col + 32 * j < d) store1(out + col + 32 * j, acc[j]);
+  }
+}
+
+// Asks for a row's whole 16-byte pieces in L2.
+template <typename T>
+__device__ __forceinline__ void fetch_to_l2(const T* row, int d) {
+  const uintptr_t from = (reinterpret_cast<uintptr_t>(row) + 15) & ~static_cast<uintptr_t>(15);
+  const uintptr_t to = reinterpret_cast<uintptr_t>(row + d) & ~static_cast<uintptr_t>(15);
+  if (to > from)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(static_cast<uint32_t>(to - from)) : "memory");
+}
+
+template <typename T, typename P, bool kVec>
+__global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const int* __restrict__ ids_of,
+                                                                         const T* __restrict__ dy, P* __restrict__ dE,
+                                                                         int n, int V, int d, float scale, int span,
+                                                                         int ahead, Runs runs) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  int* noted = reinterpret_cast<int*>(smem);  // [kSortWarps][kNoted] positions
+  int* sorted = noted + kSortWarps * kNoted;               // [kSortWarps * kNoted] positions in the sorted order
+  int* hist = sorted + kSortWarps * kNoted;                // [kSortWarps][span] counts, then next places
+  int* count = hist + kSortWarps * span;                   // [span] of the ids
+  int* listed = count + span;  // [span] from the front ids with 2 to kSlab tokens, from the back those with more, in any order
+  int* single = listed + span;  // [span] ids with one token
+  __shared__ int warp_total[kSortWarps], below_of[kSortWarps], n_few, n_many, n_single;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lo = blockIdx.x * span, ids = min(span, V - lo);
+  for (int i = tid; i < kSortWarps * span; i += kSortThreads) hist[i] = 0;
+  if (tid == 0) n_few = n_many = n_single = 0;
+  __syncthreads();
+  const int part = (n + 128 * kSortWarps - 1) / (128 * kSortWarps) * 128;  // tokens a warp
+  const int from = min(n, warp * part), to = min(n, from + part);
+  int *mine = hist + warp * span, *my_noted = noted + warp * kNoted;
+  int below = 0, found = 0;
+  // four tokens a lane; f(position, in order over the lanes, belongs to the block) by every lane, or not at all
+  auto scan = [&](auto f) {
+    const int4* p = reinterpret_cast<const int4*>(ids_of + from) + lane;
+#pragma unroll 4
+    for (int i = from + 4 * lane; i - 4 * lane < to; i += 128, p += 32) {
+      int4 q = make_int4(-1, -1, -1, -1);
+      if (i + 3 < n)
+        q = *p;
+      else if (i < n)
+        q = make_int4(ids_of[i], i + 1 < n ? ids_of[i + 1] : -1, i + 2 < n ? ids_of[i + 2] : -1, -1);
+      f(i, q);
+    }
+  };
+  auto in_block = [&](int t) { return static_cast<unsigned>(t - lo) < static_cast<unsigned>(ids); };
+  scan([&](int i, const int4& q) {
+    const unsigned first = static_cast<unsigned>(lo);  // ids out of the table are -1: never below
+    below += (static_cast<unsigned>(q.x) < first) + (static_cast<unsigned>(q.y) < first) + (static_cast<unsigned>(q.z) < first) +
+             (static_cast<unsigned>(q.w) < first);
+    const bool o0 = in_block(q.x), o1 = in_block(q.y), o2 = in_block(q.z), o3 = in_block(q.w);
+    if (!__any_sync(0xffffffffu, o0 | o1 | o2 | o3)) return;
+    const unsigned b0 = __ballot_sync(0xffffffffu, o0), b1 = __ballot_sync(0xffffffffu, o1),
+                   b2 = __ballot_sync(0xffffffffu, o2), b3 = __ballot_sync(0xffffffffu, o3), under = (1u << lane) - 1;
+    int at = found + __popc(b0 & under) + __popc(b1 & under) + __popc(b2 & under) + __popc(b3 & under);
+    auto note = [&](bool own, int t, int position) {
+      if (!own) return;
+      atomicAdd(mine + (t - lo), 1);
+      if (ahead) fetch_to_l2(dy + static_cast<long long>(position) * d, d);
+      if (at < kNoted) my_noted[at] = position;
+      ++at;
+    };
+    note(o0, q.x, i), note(o1, q.y, i + 1), note(o2, q.z, i + 2), note(o3, q.w, i + 3);
+    found += __popc(b0) + __popc(b1) + __popc(b2) + __popc(b3);
+  });
   below = __reduce_add_sync(0xffffffffu, below);
   if (lane == 0) below_of[warp] = below;
   __syncthreads();
-  // exclusive sums over (id, warp); a thread takes two neighbouring ids
-  int c[2] = {0, 0};
+  // exclusive sums over (id, warp); a thread takes an id, or two neighbouring ones
+  const int each = ids <= kSortThreads ? 1 : 2;
+  int totals[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    if (2 * tid + k < ids)
-      for (int w = 0; w < kSortWarps; ++w) c[k] += hist[w * span + 2 * tid + k];
-  int incl = c[0] + c[1];
+    if (k < each && each * tid + k < ids) {
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) totals[k] += hist[w * span + each * tid + k];
+    }
+  int incl = totals[0] + totals[1];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -132,22 +282,25 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const v
   }
   if (lane == 31) warp_total[warp] = incl;
   __syncthreads();
-  int at = incl - c[0] - c[1];
-  for (int w = 0; w < kSortWarps; ++w) {
-    at += below_of[w];
-    if (w < warp) at += warp_total[w];
-  }
+  const int base = __reduce_add_sync(0xffffffffu, below_of[lane]);
+  const int block_total = __reduce_add_sync(0xffffffffu, warp_total[lane]);
+  int at = base + __reduce_add_sync(0xffffffffu, lane < warp ? warp_total[lane] : 0) + incl - totals[0] - totals[1];
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    if (2 * tid + k < ids) {
-      const int i = 2 * tid + k;
-      count[i] = c[k];
-      if (c[k] > kSlab) {
+    if (k < each && each * tid + k < ids) {
+      const int i = each * tid + k;
+      count[i] = totals[k];
+      runs.empty[lo + i] = totals[k] == 0;
+      if (totals[k] == 1) single[atomicAdd(&n_single, 1)] = i;
+      if (totals[k] > 1 && totals[k] <= kSlab) listed[atomicAdd(&n_few, 1)] = i;
+      if (totals[k] > kSlab) {
+        listed[span - 1 - atomicAdd(&n_many, 1)] = i;
         const int slab = at / kSlab;
-        runs.id[slab] = static_cast<int>(lo) + i;
-        runs.end[slab] = at + c[k];
+        runs.id[slab] = lo + i;
+        runs.end[slab] = at + totals[k];
         runs.done[slab] = 0;
       }
+#pragma unroll 8
       for (int w = 0; w < kSortWarps; ++w) {
         const int v = hist[w * span + i];
         hist[w * span + i] = at;
@@ -155,90 +308,62 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const v
       }
     }
   __syncthreads();
-  // zero rows first: the stores drain while the tokens are placed
-  const int step = kVec ? 8 : 1;
-  for (int i = warp; i < ids; i += kSortWarps) {
-    if (count[i] != 0) continue;
-    P* out = dE + (lo + i) * d;
-    const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int col = step * lane; col < d; col += 32 * step) {
-      if (kVec)
-        store8(out + col, zero);
-      else
-        store1(out + col, 0.0f);
-    }
-  }
-#pragma unroll 4
-  for (int i = from + lane; i - lane < to; i += 32) {
-    const long long t = i < to ? token_at(tokens, wide, i) : -1;
-    const bool own = t >= lo && t < lo + ids;
+  const bool local = block_total <= kSortWarps * kNoted;  // the sorted order fits shared memory
+  auto place = [&](bool own, int bin, int position) {     // by every lane of the warp, positions ascending with the lane
     const unsigned all = __ballot_sync(0xffffffffu, own);
     if (own) {
-      const int bin = static_cast<int>(t - lo);
       const unsigned same = __match_any_sync(all, bin);
       const int first = mine[bin], rank = __popc(same & ((1u << lane) - 1));
       __syncwarp(all);
       if (rank == 0) mine[bin] = first + __popc(same);
-      runs.order[first + rank] = i;
+      if (local) sorted[first + rank - base] = position;
+      if (!local || count[bin] > kSlab) runs.order[first + rank] = position;
     }
     __syncwarp();
+  };
+  if (found <= kNoted) {
+    for (int e = lane; e - lane < found; e += 32) {
+      const int position = e < found ? my_noted[e] : -1;
+      place(e < found, e < found ? ids_of[position] - lo : 0, position);
+    }
+  } else {
+    for (int i = from + lane; i - lane < to; i += 32) {
+      const int t = i < to ? ids_of[i] : -1;
+      place(in_block(t), t - lo, i);
+    }
   }
   __syncthreads();
   let_next_start();
   // place of an id's first token: where the last warp's part of the id before it ended
-  int base = 0;
-  for (int w = 0; w < kSortWarps; ++w) base += below_of[w];
-  const int* ends = hist + (kSortWarps - 1) * span;
-  if (lo + ids == V)  // places behind the last valid token
-    for (int i = ends[ids - 1] + tid; i < n; i += kSortThreads) runs.run_start[i] = -1;
-  for (int i = warp; i < ids; i += kSortWarps) {
-    const int k = count[i], start = i == 0 ? base : ends[i - 1];
-    for (int j = lane; j < k; j += 32) runs.run_start[start + j] = k > kSlab ? start : -1;
-    if (k == 0 || k > kSlab) continue;
-    const int row_of = lane < k ? runs.order[start + lane] : 0;
-    P* out = dE + (lo + i) * d;
-    if (kVec) {
-      constexpr int kCh = 3;
-      for (int c0 = 8 * lane; c0 - 8 * lane < d; c0 += 256 * kCh) {
-        float acc[kCh][8] = {};
-        for (int r = 0; r < k; ++r) {
-          const T* row = dy + static_cast<long long>(__shfl_sync(0xffffffffu, row_of, r)) * d;
-          Raw8<T> raw[kCh];
-#pragma unroll
-          for (int h = 0; h < kCh; ++h)
-            if (c0 + 256 * h < d) raw[h] = load8(row + c0 + 256 * h);
-#pragma unroll
-          for (int h = 0; h < kCh; ++h)
-            if (c0 + 256 * h < d) {
-              float v[8];
-              unpack8(raw[h], v);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) acc[h][j] += v[j];
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < kCh; ++h)
-          if (c0 + 256 * h < d) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[h][j] *= scale;
-            store8(out + c0 + 256 * h, acc[h]);
-          }
-      }
-    } else {
-      constexpr int kCh = 8;
-      for (int c0 = lane; c0 - lane < d; c0 += 32 * kCh) {
-        float acc[kCh] = {};
-        for (int r = 0; r < k; ++r) {
-          const T* row = dy + static_cast<long long>(__shfl_sync(0xffffffffu, row_of, r)) * d;
-#pragma unroll
-          for (int h = 0; h < kCh; ++h)
-            if (c0 + 32 * h < d) acc[h] += as_float(row[c0 + 32 * h]);
-        }
-#pragma unroll
-        for (int h = 0; h < kCh; ++h)
-          if (c0 + 32 * h < d) store1(out + c0 + 32 * h, acc[h] * scale);
-      }
+  auto start_of = [&](int i) { return i == 0 ? base : hist[(kSortWarps - 1) * span + i - 1]; };
+  if (n > kSlab) {  // else the second kernel does not look for runs
+    for (int i = base + tid; i < base + block_total; i += kSortThreads) runs.run_start[i] = -1;
+    if (lo + ids == V)  // places behind the last valid token
+      for (int i = base + block_total + tid; i < n; i += kSortThreads) runs.run_start[i] = -1;
+    __syncthreads();
+    for (int m = warp; m < n_many; m += kSortWarps) {
+      const int i = listed[span - 1 - m], start = start_of(i);
+      for (int j = lane; j < count[i]; j += 32) runs.run_start[start + j] = start;
     }
+  }
+  // A warp takes a piece of 256 columns of an id's rows; what it waits for is a chain of lookups and one random access to
+  // memory (2,000 to 4,000 cycles), so of ids with one token it takes four at a time.
+  const int pieces = (d + 255) / 256;
+  auto position_of = [&](int i, int r) { return local ? sorted[start_of(i) - base + r] : runs.order[start_of(i) + r]; };
+#pragma unroll 1
+  for (int item = warp * kItems; item < n_single * pieces; item += kSortWarps * kItems) {
+    int from = 0, to = 0, c0 = d;  // lane u: the u-th item's
+    if (lane < kItems && item + lane < n_single * pieces) {
+      const int i = single[(item + lane) / pieces];
+      from = position_of(i, 0), to = lo + i, c0 = ((item + lane) % pieces) * 256;
+    }
+    copy_rows<T, P, kVec>(dy, dE, from, to, c0, d, scale, lane);
+  }
+#pragma unroll 1
+  for (int item = warp; item < n_few * pieces; item += kSortWarps) {
+    const int i = listed[item / pieces], piece = item % pieces;
+    const int k = count[i], row_of = lane < k ? position_of(i, lane) : 0;
+    sum_rows<T, P, kVec>(dy, row_of, k, dE + static_cast<long long>(lo + i) * d, 256 * piece, d, scale, lane);
   }
 }
 
@@ -257,12 +382,12 @@ __device__ __forceinline__ void values8(const __nv_bfloat16* p, bool, float (&v)
 template <bool kVec, bool kFresh, typename Row, typename Put>
 __device__ __forceinline__ void block_row_sum(int rows, int d, int width, float* red, Row row, Put put) {
   constexpr int kPer = kVec ? 8 : 1;
-  const int groups = blockDim.x / width, g = threadIdx.x / width, c = threadIdx.x % width;
+  const int groups = blockDim.x / width, g = threadIdx.x / width, c = threadIdx.x - g * width;
   for (int c0 = 0; c0 < d; c0 += width * kPer) {
     const int col = c0 + c * kPer;
     float acc[kPer] = {};
-    if (col < d) {
-#pragma unroll 8
+    if (col < d && g < groups) {
+#pragma unroll 4
       for (int r = g; r < rows; r += groups) {
         const auto* p = row(r) + col;
         if (kVec) {
@@ -289,12 +414,24 @@ __device__ __forceinline__ void block_row_sum(int rows, int d, int width, float*
 }
 
 template <typename T, typename P, bool kVec>
-__global__ void __launch_bounds__(256) embedding_runs_kernel(const T* __restrict__ dy, P* __restrict__ dE, int n, int d,
-                                                             float scale, Runs runs, float* __restrict__ partial) {
+__global__ void __launch_bounds__(kRunThreads, 4) embedding_runs_kernel(const T* __restrict__ dy, P* __restrict__ dE, int n, int V,
+                                                                     int d, float scale, Runs runs,
+                                                                     float* __restrict__ partial, int slabs, int per) {
   __shared__ int where[kSlab], place[kSlab], last;
-  __shared__ float red[256 * 8];
+  __shared__ float red[kRunThreads * 8];
   wait_for_previous();
-  const int slab = blockIdx.x, begin = slab * kSlab, stop = min(n, begin + kSlab);
+  // Blocks with a slab and blocks with `per` ids, whose rows without a token they write, take turns while there are both:
+  // the former wait for loads, the latter do not.
+  const int zero_blocks = gridDim.x - slabs, pairs = min(slabs, zero_blocks), b = blockIdx.x;
+  const bool zeros = b < 2 * pairs ? b & 1 : slabs <= zero_blocks;
+  const int mine = b < 2 * pairs ? b / 2 : b - pairs;
+  if (zeros) {
+    const int from = mine * per, to = min(V, from + per);
+    for (int i = from + threadIdx.x / 32; i < to; i += kRunThreads / 32)
+      if (runs.empty[i]) write_zeros(dE + static_cast<long long>(i) * d, d, threadIdx.x & 31);
+    return;
+  }
+  const int slab = mine, begin = slab * kSlab, stop = min(n, begin + kSlab);
   if (threadIdx.x < kSlab) {
     const bool in = begin + static_cast<int>(threadIdx.x) < stop;
     where[threadIdx.x] = in ? runs.run_start[begin + threadIdx.x] : -1;
@@ -302,8 +439,7 @@ __global__ void __launch_bounds__(256) embedding_runs_kernel(const T* __restrict
   }
   __syncthreads();
   constexpr int kPer = kVec ? 8 : 1;
-  int width = 32;
-  while (width < 256 && width * kPer < d) width *= 2;
+  const int width = min(kRunThreads, (d + kPer - 1) / kPer);  // as many groups of threads as the block has room for
   // Two runs at most: one that comes in over the slab's beginning, one that starts in it.
   for (int which = 0; which < 2; ++which) {
     int a = 0, b;
@@ -315,12 +451,12 @@ __global__ void __launch_bounds__(256) embedding_runs_kernel(const T* __restrict
     }
     const int start = where[a], slot = start / kSlab, end = runs.end[slot], id = runs.id[slot];
     b = min(kSlab, end - begin);
-    float* mine = partial + (2ll * slab + which) * d;
+    float* own_part = partial + (2ll * slab + which) * d;
     block_row_sum<kVec, false>(
         b - a, d, width, red, [&](int r) { return dy + static_cast<long long>(place[a + r]) * d; },
         [&](int col, const float(&v)[kPer]) {
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) mine[col + j] = v[j];
+          for (int j = 0; j < kPer; ++j) own_part[col + j] = v[j];
         });
     __threadfence();
     __syncthreads();
@@ -350,33 +486,39 @@ __global__ void __launch_bounds__(256) embedding_runs_kernel(const T* __restrict
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename P, typename T, bool kVec>
-int lookup(const void* tokens, int wide, const void* table, void* y, long long n, long long V, int d, float scale,
+int lookup(const void* tokens, int wide, const void* table, void* y, int* ids, long long n, long long V, int d, float scale,
            int* status, int* refused, cudaStream_t st) {
   const int blocks = static_cast<int>(std::min<long long>((n + 31) / 32, 148 * 8));
   embedding_lookup_kernel<P, T, kVec><<<blocks, 256, 0, st>>>(tokens, wide, static_cast<const P*>(table),
-                                                              static_cast<T*>(y), n, V, d, scale, status, refused);
+                                                              static_cast<T*>(y), ids, n, V, d, scale, status, refused);
   return cudaGetLastError() == cudaSuccess ? 0 : 1;
 }
 
 template <typename T, typename P, bool kVec>
-int grad(const void* tokens, int wide, const void* dy, void* dE, int n, long long V, int d, float scale, int* ints,
-         float* partial, cudaStream_t st) {
-  const long long blocks_min = (V + kMaxSpan - 1) / kMaxSpan;
-  const int span = static_cast<int>((V + std::max(148ll, blocks_min) - 1) / std::max(148ll, blocks_min));
-  const int blocks = static_cast<int>((V + span - 1) / span);
-  const int slabs = (n + kSlab - 1) / kSlab;
-  const Runs runs{ints, ints + n, ints + 2ll * n, ints + 2ll * n + slabs, ints + 2ll * n + 2ll * slabs};
-  const size_t smem = static_cast<size_t>(span) * (kSortWarps + 1) * sizeof(int);
+int grad(const int* ids, const void* dy, void* dE, int n, int V, int d, float scale, int* ints, float* partial,
+         cudaStream_t st) {
+  // a block an SM, or more where a span would not fit
+  const int blocks_min = std::max(148, (V + kMaxSpan - 1) / kMaxSpan);
+  const int span = (V + blocks_min - 1) / blocks_min, blocks = (V + span - 1) / span;
+  const int slabs = n > kSlab ? (n + kSlab - 1) / kSlab : 0;  // else no id has more tokens than a slab
+  const long long all = (n + kSlab - 1) / kSlab;
+  const Runs runs{ints, ints + n, ints + 2ll * n, ints + 2ll * n + all, ints + 2ll * n + 2 * all,
+                  reinterpret_cast<uint8_t*>(ints + 2ll * n + 3 * all)};
+  const size_t smem = (static_cast<size_t>(span) * (kSortWarps + 3) + 2 * kSortWarps * kNoted) * sizeof(int);
   auto kern = embedding_sort_kernel<T, P, kVec>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSpan * (kSortWarps + 1) * 4) !=
-      cudaSuccess)
+  static bool sized = false;  // the same answer whoever asks first
+  if (!sized && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (kMaxSpan * (kSortWarps + 3) + 2 * kSortWarps * kNoted) * 4) != cudaSuccess)
     return 2;
-  kern<<<blocks, kSortThreads, smem, st>>>(tokens, wide, static_cast<const T*>(dy), static_cast<P*>(dE), n, V, d, scale,
-                                           span, runs);
+  sized = true;
+  // half of L2 may hold the rows until they are summed
+  const int ahead = static_cast<long long>(n) * d * static_cast<long long>(sizeof(T)) <= (64ll << 20);
+  kern<<<blocks, kSortThreads, smem, st>>>(ids, static_cast<const T*>(dy), static_cast<P*>(dE), n, V, d, scale, span, ahead,
+                                           runs);
   if (cudaGetLastError() != cudaSuccess) return 1;
-  if (n <= kSlab) return 0;  // no id has more tokens than a slab
-  return launch_after(embedding_runs_kernel<T, P, kVec>, dim3(slabs), dim3(256), 0, st, static_cast<const T*>(dy),
-                      static_cast<P*>(dE), n, d, scale, runs, partial) == cudaSuccess
+  const int per = std::max(16, (V + 148 * 4 - 1) / (148 * 4)), zero_blocks = (V + per - 1) / per;
+  return launch_after(embedding_runs_kernel<T, P, kVec>, dim3(slabs + zero_blocks), dim3(kRunThreads), 0, st,
+                      static_cast<const T*>(dy), static_cast<P*>(dE), n, V, d, scale, runs, partial, slabs, per) == cudaSuccess
              ? 0
              : 1;
 }
@@ -384,16 +526,17 @@ int grad(const void* tokens, int wide, const void* dy, void* dE, int n, long lon
 }  // namespace
 
 // y [n, d] = scale table[tokens]; a token outside [0, V) is reported and gives a zero row. tokens int64 (wide) or int32.
-extern "C" int pd_embedding(const void* tokens, int wide, const void* table, void* y, long long n, long long V, int d,
-                            float scale, int table_fp32, int y_fp32, int* status, int* refused, void* stream) {
-  if (n <= 0 || V <= 0 || d <= 0) return 5;
+// ids [n] (or null) receives them in 32 bits, unknown ones as -1.
+extern "C" int pd_embedding(const void* tokens, int wide, const void* table, void* y, int* ids, long long n, long long V,
+                            int d, float scale, int table_fp32, int y_fp32, int* status, int* refused, void* stream) {
+  if (n <= 0 || V <= 0 || V >= (1ll << 30) || d <= 0) return 5;
   const bool vec = d % 8 == 0 && aligned16(table) && aligned16(y);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = [&](auto p, auto t) {
     using P = decltype(p);
     using T = decltype(t);
-    return vec ? lookup<P, T, true>(tokens, wide, table, y, n, V, d, scale, status, refused, st)
-               : lookup<P, T, false>(tokens, wide, table, y, n, V, d, scale, status, refused, st);
+    return vec ? lookup<P, T, true>(tokens, wide, table, y, ids, n, V, d, scale, status, refused, st)
+               : lookup<P, T, false>(tokens, wide, table, y, ids, n, V, d, scale, status, refused, st);
   };
   using B = __nv_bfloat16;
   if (table_fp32) return y_fp32 ? go(float(), float()) : go(float(), B());
@@ -401,20 +544,23 @@ extern "C" int pd_embedding(const void* tokens, int wide, const void* table, voi
 }
 
 // Scratch of the gradient, in ints and in floats.
-extern "C" long long pd_embedding_grad_ints(long long n) { return 2 * n + 3 * ((n + kSlab - 1) / kSlab); }
+extern "C" long long pd_embedding_grad_ints(long long n, long long V) {
+  return 2 * n + 3 * ((n + kSlab - 1) / kSlab) + (V + 3) / 4;
+}
 extern "C" long long pd_embedding_grad_floats(long long n, int d) { return 2 * ((n + kSlab - 1) / kSlab) * d; }
 
-// dE [V, d], every row of it; tokens outside [0, V) take no part.
-extern "C" int pd_embedding_grad(const void* tokens, int wide, const void* dy, void* dE, long long n, long long V, int d,
-                                 float scale, int dy_fp32, int table_fp32, int* ints, float* partial, void* stream) {
-  if (n < 0 || n >= (1ll << 30) || V <= 0 || V >= (1ll << 31) || d <= 0) return 5;
+// dE [V, d], every row of it; ids as the lookup left them, 16-byte aligned: those outside [0, V) take no part.
+extern "C" int pd_embedding_grad(const int* ids, const void* dy, void* dE, long long n, long long V, int d, float scale,
+                                 int dy_fp32, int table_fp32, int* ints, float* partial, void* stream) {
+  if (n < 0 || n >= (1ll << 30) || V <= 0 || V >= (1ll << 30) || d <= 0 || !aligned16(ids)) return 5;
   const bool vec = d % 8 == 0 && aligned16(dy) && aligned16(dE) && aligned16(partial);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int n32 = static_cast<int>(n), V32 = static_cast<int>(V);
   auto go = [&](auto t, auto p) {
     using T = decltype(t);
     using P = decltype(p);
-    return vec ? grad<T, P, true>(tokens, wide, dy, dE, static_cast<int>(n), V, d, scale, ints, partial, st)
-               : grad<T, P, false>(tokens, wide, dy, dE, static_cast<int>(n), V, d, scale, ints, partial, st);
+    return vec ? grad<T, P, true>(ids, dy, dE, n32, V32, d, scale, ints, partial, st)
+               : grad<T, P, false>(ids, dy, dE, n32, V32, d, scale, ints, partial, st);
   };
   using B = __nv_bfloat16;
   if (dy_fp32) return table_fp32 ? go(float(), float()) : go(float(), B());
