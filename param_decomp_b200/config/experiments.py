@@ -305,7 +305,17 @@ class StreamedOutputEdgeConfig(BaseConfig):
     n_vocab_chunks: PositiveInt
 
 
-LMOutputEdgeConfig = Annotated[MaterializedOutputEdgeConfig | StreamedOutputEdgeConfig, Discriminator("kind")]
+class TopLogitsOutputEdgeConfig(BaseConfig):
+    """The clean side is kept as each position's `k` largest logits and one number for all others, not as `[positions, vocab]`
+    logits: the reconstruction loss is the KL divergence between the two distributions over these `k + 1` events, which is
+    never above the divergence over the whole vocabulary. (Not in the reference.)"""
+
+    kind: Literal["top_logits"] = "top_logits"
+    k: PositiveInt = Field(default=64, le=256)
+
+
+LMOutputEdgeConfig = Annotated[MaterializedOutputEdgeConfig | StreamedOutputEdgeConfig | TopLogitsOutputEdgeConfig,
+                               Discriminator("kind")]
 
 
 class LMTargetConfig(BaseConfig):

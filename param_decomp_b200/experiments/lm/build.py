@@ -102,6 +102,7 @@ def build_lm_run(cfg: X.LMExperimentConfig | X.LMTargetedExperimentConfig, data_
     sites_cfg = cfg.decomposition.sites
     edge = cfg.target.output_edge
     n_chunks = edge.n_vocab_chunks if isinstance(edge, X.StreamedOutputEdgeConfig) else None
+    n_top = edge.k if isinstance(edge, X.TopLogitsOutputEdgeConfig) else None
     backend = cfg.runtime.backend if torch.device(device).type == "cuda" else "eager_torch"
     if arch.family == "qwen35_moe":
         from param_decomp_b200.models import qwen35
@@ -114,7 +115,8 @@ def build_lm_run(cfg: X.LMExperimentConfig | X.LMTargetedExperimentConfig, data_
     else:
         site_cs = resolve_site_cs(sites_cfg, arch)
         model = tf.TransformerDecomposedModel(arch, weights, site_cs, backend=backend,
-                                              attention=cfg.target.attention_implementation, n_vocab_chunks=n_chunks)
+                                              attention=cfg.target.attention_implementation, n_vocab_chunks=n_chunks,
+                                              n_top_logits=n_top)
     if expert_group is not None and ep is None:
         assert expert_mode != "all_to_all", "all_to_all dispatch applies to mixture-of-experts targets"
         model.split_components(expert_group)  # dense target: the tp axis divides every site's component axis

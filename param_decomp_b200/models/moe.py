@@ -316,4 +316,5 @@ def build_moe_model(arch: TransformerArchConfig, weights: dict[str, Tensor], sit
                               ep=ep)
     edge = getattr(target_cfg, "output_edge", None)
     model.n_vocab_chunks = getattr(edge, "n_vocab_chunks", None)  # streamed output edge: chunks of positions
+    model.n_top_logits = getattr(edge, "k", None)  # top-logits output edge
     return model

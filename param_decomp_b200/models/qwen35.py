@@ -378,7 +378,7 @@ class Qwen35DecomposedModel(moe.MoEDecomposedModel):
         want = set(capture)
         tokens = batch.tokens
         B, T = tokens.shape
-        resid = F.embedding(tokens.long(), self.w["embed.weight"])
+        resid = self._embed(tokens, self.w["embed.weight"])
         pos = batch.positions if batch.positions is not None else torch.arange(T, device=tokens.device)[None]
         cos, sin = ports.rope_cos_sin(pos, self.rotary_dim, a.rope_theta)
         taps: dict[str, Tensor] | None = {} if want_taps else None
@@ -422,4 +422,5 @@ def build_qwen35_model(arch: TransformerArchConfig, weights: dict[str, Tensor], 
                                  attention=target_cfg.attention_implementation, ep=ep)
     edge = getattr(target_cfg, "output_edge", None)
     model.n_vocab_chunks = getattr(edge, "n_vocab_chunks", None)  # streamed output edge: chunks of positions
+    model.n_top_logits = getattr(edge, "k", None)  # top-logits output edge
     return model

@@ -135,7 +135,7 @@ class TransformerDecomposedModel:
 
     def __init__(self, arch: TransformerArchConfig, weights: dict[str, Tensor], site_cs: dict[str, int],
                  backend: str = "eager_torch", attention: str = "flash", n_vocab_chunks: int | None = None,
-                 kl_token_chunk: int = 8192) -> None:
+                 kl_token_chunk: int = 8192, n_top_logits: int | None = None, train_kernels: bool = False) -> None:
         assert arch.family in ("glu_transformer", "simple_mlp", "moe"), arch.family
         self.arch = arch
         self.w = weights
@@ -143,6 +143,10 @@ class TransformerDecomposedModel:
         # the eager backend means library ops end to end: torch's fused attention instead of the hand-written kernel
         self.attention_impl = "sdpa" if (backend == "eager_torch" and attention == "flash") else attention
         self.n_vocab_chunks = n_vocab_chunks
+        self.n_top_logits = n_top_logits
+        # the eager backend's model with trainable weights (the pretrainer's): embeddings and LayerNorms on this library's
+        # kernels, which have the weights' gradients
+        self.train_kernels = train_kernels
         self.kl_token_chunk = kl_token_chunk
         self.compute_dtype = weights["embed.weight"].dtype
         self.head_dim = arch.head_dim or arch.d_model // arch.n_head
@@ -245,6 +249,10 @@ class TransformerDecomposedModel:
         if getattr(self.arch, "norm_kind", "rms") == "layer":
             # LayerNorm with bias (GPT-2 style): statistics in fp32, scale and shift in the activation dtype
             # (param_decomp/pretrain/models.py:182-188)
+            if self.train_kernels and x.is_cuda:
+                from param_decomp_b200.ops import elementwise as ew
+
+                return ew.layer_norm(x, w, b, self.arch.rms_eps)
             xf = x.float()
             mean = xf.mean(-1, keepdim=True)
             var = (xf - mean).pow(2).mean(-1, keepdim=True)
@@ -255,6 +263,13 @@ class TransformerDecomposedModel:
 
             return ew.rms_norm(x, w, self.arch.rms_eps)
         return ports.rms_norm(x, w, self.arch.rms_eps)
+
+    def _embed(self, tokens: Tensor, table: Tensor) -> Tensor:
+        if getattr(self, "train_kernels", False) and tokens.is_cuda:
+            from param_decomp_b200.ops.embedding import embedding
+
+            return embedding(tokens, table)
+        return F.embedding(tokens.long(), table)
 
     def _rope(self, x: Tensor, cos: Tensor, sin: Tensor, shared_positions: bool) -> Tensor:
         if getattr(self.arch, "positional", "rope") == "learned":
@@ -355,10 +370,10 @@ class TransformerDecomposedModel:
         want = set(capture)
         tokens = batch.tokens
         B, T = tokens.shape
-        resid = F.embedding(tokens.long(), self.w["embed.weight"])
+        resid = self._embed(tokens, self.w["embed.weight"])
         pos = batch.positions if batch.positions is not None else torch.arange(T, device=tokens.device)[None]
         if getattr(a, "positional", "rope") == "learned":
-            resid = resid + F.embedding(pos.long(), self.w["pos_embed.weight"])
+            resid = resid + self._embed(pos, self.w["pos_embed.weight"])
         cos, sin = ports.rope_cos_sin(pos, self.head_dim, a.rope_theta, a.rope_scaling)
         taps: dict[str, Tensor] | None = {} if want_taps else None
         captures: dict[str, Tensor] = {}
@@ -407,8 +422,16 @@ class TransformerDecomposedModel:
         return F.linear(final_hidden, self.head_weight())
 
     # -- output edge: KL(clean || masked) over the vocabulary ---------------------------------------
-    def _clean_logit_stats(self, hidden: Tensor) -> dict[str, Tensor]:
-        """Fused backend: the clean logits are formed once per step and reused by every draw."""
+    def _clean_logit_stats(self, hidden: Tensor) -> dict[str, Any]:
+        """Fused backend: the clean logits are formed once per step and reused by every draw. `output_edge: top_logits`: so
+        are each position's largest, on either backend."""
+        if getattr(self, "n_top_logits", None) is not None:
+            from param_decomp_b200.ops import vocab_kl
+
+            h, k = hidden.detach().reshape(-1, hidden.shape[-1]), min(self.n_top_logits, self.head_weight().shape[0])
+            if self.backend == "fused_sm100" and hidden.is_cuda:
+                return {"top": vocab_kl.top_logits_from_hidden(h, self.head_weight(), k, self.kl_token_chunk)}
+            return {"top": eager_top_logits_from_hidden(h, self.head_weight(), k, self.kl_token_chunk)}
         if self.backend == "fused_sm100" and hidden.is_cuda and self.n_vocab_chunks is None:
             from param_decomp_b200.ops import vocab_kl
 
@@ -421,6 +444,13 @@ class TransformerDecomposedModel:
         is recomputed in the backward pass (`ops/vocab_kl.py` is the fused kernel of this loss)."""
         hc = clean.output.reshape(-1, clean.output.shape[-1])
         hm = masked.output.reshape(-1, masked.output.shape[-1])
+        if getattr(self, "n_top_logits", None) is not None:
+            top = clean.aux["clean_stats"]["top"]
+            if self.backend == "fused_sm100" and hm.is_cuda:
+                from param_decomp_b200.ops import vocab_kl
+
+                return vocab_kl.top_kl_from_hidden(top, hm, self.head_weight(), self.kl_token_chunk)
+            return eager_top_kl_from_hidden(top, hm, self.head_weight(), self.kl_token_chunk)
         if self.backend == "fused_sm100" and hm.is_cuda:
             from param_decomp_b200.ops import vocab_kl
 
@@ -468,3 +498,25 @@ def chunked_kl_from_hidden(hc: Tensor, hm: Tensor, head: Tensor, chunk: int) -> 
     for s in range(0, n, chunk):
         total = total + _ChunkKL.apply(hc[s:s + chunk], hm[s:s + chunk], head)
     return total / n
+
+
+def eager_top_logits_from_hidden(hc: Tensor, head: Tensor, k: int, chunk: int):
+    """Each position's `k` largest logits, their columns and the logsumexp of the rest, `chunk` positions at a time."""
+    from param_decomp_b200.ops.top_logits import TopLogits, eager_top_logits
+
+    parts = [eager_top_logits(F.linear(hc[s:s + chunk], head), k) for s in range(0, hc.shape[0], chunk)]
+    return TopLogits(*(torch.cat(t) for t in zip(*parts)))
+
+
+def eager_top_kl_from_hidden(top, hm: Tensor, head: Tensor, chunk: int) -> Tensor:
+    """Mean over positions of the divergence from the clean side's top logits; a chunk's logits are formed again in backward."""
+    from torch.utils.checkpoint import checkpoint
+
+    from param_decomp_b200.ops.top_logits import eager_top_kl
+
+    total = hm.new_zeros((), dtype=torch.float32)
+    for s in range(0, hm.shape[0], chunk):
+        part = [t[s:s + chunk] for t in top]
+        run = lambda h, values, indices, tail: eager_top_kl(F.linear(h, head), indices, values, tail).sum()  # noqa: E731
+        total = total + checkpoint(run, hm[s:s + chunk], *part, use_reentrant=False)
+    return total / hm.shape[0]

@@ -16,6 +16,7 @@ from torch import Tensor
 
 from param_decomp_b200.ops import native as nv
 from param_decomp_b200.ops.elementwise import vocab_kl_rows
+from param_decomp_b200.ops.top_logits import TopLogits, top_kl_rows, top_logits
 
 
 def padded_logits(h: Tensor, head: Tensor) -> Tensor:
@@ -91,3 +92,41 @@ class _StreamedKLFromHidden(torch.autograd.Function):
 def kl_from_hidden_streamed(hc: Tensor, hm: Tensor, head: Tensor, rows: int) -> Tensor:
     """`hc`, `hm [n, d]` bf16 final hidden states (clean, masked), `head [V, d]`; `rows` positions per chunk."""
     return _StreamedKLFromHidden.apply(hc, hm, head, rows)
+
+
+def top_logits_from_hidden(hc: Tensor, head: Tensor, k: int, rows: int) -> TopLogits:
+    """`[n, k]` largest logits of `hc [n, d] @ head[V, d]^T` with their columns, and the logsumexp of the others `[n]`; logits
+    exist for `rows` positions at a time."""
+    parts = [top_logits(padded_logits(hc[s:s + rows], head), k) for s in range(0, hc.shape[0], rows)]
+    return parts[0] if len(parts) == 1 else TopLogits(*(torch.cat(t) for t in zip(*parts)))
+
+
+class _TopKLFromHidden(torch.autograd.Function):
+    """Like `_StreamedKLFromHidden`, with one logits GEMM a chunk: the clean side is there already."""
+
+    @staticmethod
+    def forward(ctx, hm: Tensor, head: Tensor, rows: int, values: Tensor, indices: Tensor, tail: Tensor) -> Tensor:  # type: ignore[override]
+        n = hm.shape[0]
+        hm = hm.contiguous()
+        want_grad = ctx.needs_input_grad[0]
+        dh = torch.empty_like(hm) if want_grad else None
+        total = torch.zeros((), device=hm.device, dtype=torch.float32)
+        for s in range(0, n, rows):
+            e = min(n, s + rows)
+            loss, dlm = top_kl_rows(padded_logits(hm[s:e], head), indices[s:e], values[s:e], tail[s:e], want_grad=want_grad)
+            total = total + loss.sum()
+            if want_grad:
+                nv.gemm(dlm, head, dh[s:e], b_mn=True, alpha=1.0 / n)
+        ctx.save_for_backward(dh)
+        return total / n
+
+    @staticmethod
+    def backward(ctx, g: Tensor):  # type: ignore[override]
+        (dh,) = ctx.saved_tensors
+        return dh * g.to(dh.dtype), None, None, None, None, None
+
+
+def top_kl_from_hidden(top: TopLogits, hm: Tensor, head: Tensor, rows: int) -> Tensor:
+    """Mean over positions of the divergence of `softmax(hm @ head^T)` from the clean side's `top` logits, differentiable in
+    `hm [n, d]` bf16; `rows` positions' logits exist at a time."""
+    return _TopKLFromHidden.apply(hm, head, rows, *top)

@@ -10,7 +10,7 @@ YAML keys follow the reference's pretrain configs: `run_name, seed, dtype, globa
 num_iterations, warmup_iters, learning_rate, learning_rate_decay_frac, weight_decay, grad_clip,
 log_every, val_every, val_steps, save_every, model: {model_type, n_layer, n_head, n_embd,
 n_intermediate, vocab_size, n_ctx, rotary_base, n_key_value_heads, rms_norm_eps}, data_layout, data,
-val_data, wandb` (param_decomp/pretrain/configs/*.yaml; pretrain/train.py:263-495; pretrain/models.py).
+val_data, wandb` (plus `kernels`, param_decomp/pretrain/configs/*.yaml; pretrain/train.py:263-495; pretrain/models.py).
 """
 
 from __future__ import annotations
@@ -35,6 +35,7 @@ from param_decomp_b200.core.metrics import MetricsSink, get_logger
 from param_decomp_b200.formats.base import BaseConfig
 from param_decomp_b200.models import transformer as tf
 from param_decomp_b200.models.loaders import save_qwen35_cache, save_simple_mlp_cache
+from param_decomp_b200.ops.top_logits import next_token_loss
 
 
 class PretrainModelConfig(BaseConfig):
@@ -87,6 +88,9 @@ class PretrainConfig(BaseConfig):
     gpus_per_node: PositiveInt = 8
     dtype: Literal["bfloat16", "float32"] = "bfloat16"
     attention_implementation: Literal["flash", "xla", "mosaic"] = "flash"
+    kernels: Literal["torch", "native"] = "torch"
+    """`native`: token and position embeddings, LayerNorms (`GPT2Simple`) and the next-token loss with their gradients on this
+    library's kernels (needs a GPU; not in the reference)."""
     global_batch: PositiveInt
     num_iterations: PositiveInt
     warmup_iters: int = 0
@@ -239,6 +243,9 @@ def pretrain(cfg: PretrainConfig, data_root: Path | None = None, run_id: str | N
     log = get_logger(dp.rank)
     arch = cfg.model.arch()
     dtype = torch.bfloat16 if (cfg.dtype == "bfloat16" and device != "cpu") else torch.float32
+    native = cfg.kernels == "native"
+    if native and not device.startswith("cuda"):
+        raise ValueError(f"kernels: native needs a GPU, not {device}")
     hybrid = arch.family == "qwen35_moe"
     if hybrid:
         from param_decomp_b200.models import qwen35
@@ -272,10 +279,14 @@ def pretrain(cfg: PretrainConfig, data_root: Path | None = None, run_id: str | N
         cls = qwen35.Qwen35DecomposedModel if hybrid else tf.TransformerDecomposedModel
         model = cls(arch, {k: v.to(dtype) for k, v in weights.items()}, {}, backend="eager_torch",
                     attention="xla" if device == "cpu" else cfg.attention_implementation)
+        model.train_kernels = native
         toks = batch.tokens.to(device)
         out = model._run(tf.LMBatch(toks[:, :-1], None if batch.segment_ids is None else batch.segment_ids[:, :-1].to(device)),
                          None, None, (), want_taps=False)
-        logits = model.logits(out.output).float()
+        logits = model.logits(out.output)
+        if native:
+            return next_token_loss(logits, toks[:, 1:])
+        logits = logits.float()
         return F.cross_entropy(logits.reshape(-1, logits.shape[-1]), toks[:, 1:].reshape(-1).long())
 
     def snapshot(step: int) -> None:

@@ -539,3 +539,147 @@ def test_top_kl_of_top_logits_is_the_whole_divergence(nv):
     args = (top.indices.cpu(), top.values.cpu(), top.tail.cpu(), 1.0)
     slope = sum(s * _kl_reference(z.double() + s * h * way, *args)[0].sum() for s in (1, -1)) / (2 * h)
     assert abs(float((grad.cpu().double() * way).sum() - slope)) < 1e-5
+
+
+# ---- a run of them together ---------------------------------------------------------------------------------------------
+
+
+def test_output_edge_of_top_logits_on_the_fused_backend(nv):
+    """Clean top logits and the masked side's loss as a decomposition step takes them, over several chunks of positions: the
+    loss and the hidden state's gradient against 64 bits, and against the whole vocabulary's where k is all but one of it."""
+    from param_decomp_b200.ops import vocab_kl
+
+    g = _gen(21)
+    n, d, V, k = 700, 128, 1003, 64
+    head = (torch.randn(V, d, generator=g) / d**0.5).to(bf).cuda()
+    hc = torch.randn(n, d, generator=g).to(bf).cuda()
+    hm = (hc.float().cpu() + 0.3 * torch.randn(n, d, generator=g)).to(bf).cuda()
+    top = vocab_kl.top_logits_from_hidden(hc, head, k, 256)
+    leaf = hm.clone().requires_grad_(True)
+    loss = vocab_kl.top_kl_from_hidden(top, leaf, head, 256)
+    (grad,) = torch.autograd.grad(loss * 3.0, (leaf,))
+    _done(nv)
+    # the same from the logits that the kernels saw, which were rounded to bf16
+    lc, lm = vocab_kl.padded_logits(hc, head), vocab_kl.padded_logits(hm, head)
+    want = _top_reference(lc.cpu(), k, 1.0)
+    assert torch.equal(top.indices.cpu(), want[1]) and torch.equal(top.values.cpu(), want[0])
+    rows, dz, bound, _ = _kl_reference(lm.cpu(), want[1], want[0], want[2].float(), 1.0)
+    assert abs(float(loss) - float(rows.mean())) <= float(bound.mean()) + (n + 8) * U * float(rows.abs().mean())
+    dh = 3.0 / n * dz @ head.cpu().double()
+    # dz and dh are rounded to bf16 (2^-8 of each), and 3 dh again; the sums of the product in fp32
+    size = 3.0 / n * dz.abs() @ head.cpu().double().abs()
+    assert bool(((grad.cpu().double() - dh).abs() <= (2.0**-8 * 1.01 + V * U) * size + 2.01 * 2.0**-8 * dh.abs()).all())
+
+
+def test_pretraining_step_on_native_kernels(nv, tmp_path):
+    """The pretrainer's model with `kernels: native` against library ops: loss and every weight's gradient of one batch, for
+    the model that has all of them (learned positions, LayerNorm, tied head); then the command's loop, to its snapshot."""
+    from param_decomp_b200.models import transformer as tf
+    from param_decomp_b200.ops.top_logits import next_token_loss
+    from param_decomp_b200.pretrain.train import PretrainConfig, pretrain
+
+    cfg = PretrainConfig.model_validate(dict(
+        run_name="t", seed=1, dtype="float32", global_batch=4, num_iterations=3, learning_rate=1e-3, kernels="native", log_every=1,
+        val_every=3, val_steps=1, save_every=3, model=dict(model_type="GPT2Simple", vocab_size=211, n_layer=2, n_head=2, n_embd=48, n_ctx=16)))
+    arch = cfg.model.arch()
+    w = tf.random_init_weights(arch, 0, f32)
+    g = _gen(5)
+    w = {k: (v + 0.1 * torch.randn(v.shape, generator=g) if "norm" in k else v).cuda().requires_grad_(True) for k, v in w.items()}
+    toks = torch.randint(0, 211, (4, 17), generator=g).cuda()
+    results = []
+    for native in (False, True):
+        model = tf.TransformerDecomposedModel(arch, w, {}, attention="xla", train_kernels=native)
+        logits = model.logits(model._run(tf.LMBatch(toks[:, :-1]), None, None, (), want_taps=False).output)
+        loss = (next_token_loss(logits, toks[:, 1:]) if native
+                else torch.nn.functional.cross_entropy(logits.reshape(-1, 211), toks[:, 1:].reshape(-1)))
+        results.append((loss.detach(), torch.autograd.grad(loss, list(w.values()))))
+    _done(nv)
+    assert abs(float(results[0][0]) - float(results[1][0])) < 1e-5
+    for name, a, b in zip(w, results[0][1], results[1][1]):
+        # fp32 on both sides; library products may be taken in another order
+        assert float((a - b).norm()) <= 1e-4 * float(a.norm()) + 1e-7, name
+    entry = pretrain(cfg, tmp_path, run_id="t-00000007", device="cuda:0")
+    _done(nv)
+    assert "\"val_loss\"" in (entry / "metrics.jsonl").read_text() and list(entry.glob("model_step_3.safetensors"))
+
+
+def test_two_decomposition_steps_with_the_top_logits_edge(nv, tmp_path):
+    """Through the engine on the fused backend, step by step and recorded into a graph: the edge's kernels are captured."""
+    import sys
+    from pathlib import Path
+
+    sys.path.insert(0, str(Path(__file__).parent))
+    from test_lm_ends_cpu import _lm_config
+
+    from param_decomp_b200.config.experiments import LMExperimentConfig
+    from param_decomp_b200.experiments.lm.training import train_lm
+
+    losses = []
+    for recording in ("off", "cuda_graph"):
+        c = _lm_config({"kind": "top_logits", "k": 32}, "fused_sm100", "bfloat16")
+        c["runtime"]["step_recording"] = recording
+        c["pd"]["steps"] = 6
+        c["cadence"] = {"train_log_every": 1, "checkpointing": {"kind": "none"}}
+        c["eval"] = None
+        res = train_lm(LMExperimentConfig.model_validate(c), tmp_path, run_id=f"p-0000ee0{len(losses)}", device="cuda:0")
+        _done(nv)
+        assert res.final_step == 6 and math.isfinite(res.last_metrics["train/loss/total"])
+        losses.append(res.last_metrics["train/loss/total"])
+    assert abs(losses[0] - losses[1]) < 0.05 * abs(losses[0])
+
+
+def test_graphs_and_streams(nv):
+    """Forward and backward of all four captured into two graphs that are replayed in turn with new contents, and run on two
+    streams at once: each result as without."""
+    from param_decomp_b200.ops.elementwise import layer_norm
+    from param_decomp_b200.ops.embedding import embedding
+    from param_decomp_b200.ops.top_logits import top_kl, top_logits
+
+    def inputs(seed):
+        g = _gen(seed)
+        return dict(tokens=torch.randint(0, 300, (900,), generator=g).cuda(), table=torch.randn(300, 64, generator=g).cuda(),
+                    w=torch.randn(64, generator=g).cuda(), b=torch.randn(64, generator=g).cuda(),
+                    head=torch.randn(64, 5003, generator=g).cuda(), teacher=torch.randn(900, 5003, generator=g).cuda())
+
+    def work(s):
+        leaves = [s[k].detach().requires_grad_(True) for k in ("table", "w", "b")]
+        h = layer_norm(embedding(s["tokens"], leaves[0], 8.0), leaves[1], leaves[2], 1e-5)
+        top = top_logits(s["teacher"], 20)
+        loss = top_kl(h @ s["head"], top.indices, top.values, top.tail)
+        return [loss.detach(), *torch.autograd.grad(loss.sum(), leaves)]
+
+    sets = [inputs(i) for i in range(4)]
+    want = [[t.clone() for t in work(s)] for s in sets]
+    _done(nv)
+    held = [{k: v.clone() for k, v in sets[0].items()} for _ in range(2)]
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    for s in held:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            work(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(work(s))
+        graphs.append(graph)
+    for first, second in ((1, 2), (3, 1)):
+        for s, i in zip(held, (first, second)):
+            for k in s:
+                s[k].copy_(sets[i][k])
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out, i in zip(outs, (first, second)):
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got: list = [None, None]
+    for _ in range(5):
+        for j, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[j] = work(sets[j + 1])
+    torch.cuda.synchronize()
+    for j in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[j], want[j + 1]))
+    _done(nv)

@@ -117,3 +117,62 @@ def test_eager_top_kl_of_one_slot_is_cross_entropy():
     torch.testing.assert_close(loss, want)
     ours, theirs = (torch.autograd.grad(t.sum(), (z,))[0] for t in (loss, want))
     torch.testing.assert_close(ours, theirs)
+
+
+def _lm_config(edge: dict, backend: str = "eager_torch", dtype: str = "float32") -> dict:
+    import copy
+
+    import __graft_entry__ as ge
+
+    c = copy.deepcopy(ge.SMOKE_CONFIG)
+    c["runtime"]["backend"] = backend
+    c["target"]["output_edge"] = edge
+    c["target"]["weights_dtype"] = dtype
+    c["target"]["attention_implementation"] = "xla" if dtype == "float32" else "flash"
+    return c
+
+
+def test_output_edge_of_top_logits_parses_and_is_bounded():
+    from pydantic import ValidationError
+
+    from param_decomp_b200.config.experiments import LMExperimentConfig
+
+    cfg = LMExperimentConfig.model_validate(_lm_config({"kind": "top_logits", "k": 16}))
+    assert cfg.target.output_edge.k == 16
+    for k in (0, 257):
+        with pytest.raises(ValidationError):
+            LMExperimentConfig.model_validate(_lm_config({"kind": "top_logits", "k": k}))
+
+
+def test_output_edge_of_top_logits_on_the_eager_backend():
+    """The model's loss against the clean side's top logits is `eager_top_kl` of them, chunk by chunk; with all of the
+    vocabulary it is the loss of the materialised edge, and so is its gradient."""
+    from types import SimpleNamespace
+
+    from param_decomp_b200.config.experiments import TransformerArchConfig
+    from param_decomp_b200.models import transformer as tf
+
+    arch = TransformerArchConfig(family="glu_transformer", n_layer=1, d_model=16, n_head=2, d_ff=24, vocab_size=40, max_seq_len=8)
+    w = tf.random_init_weights(arch, 0, torch.float32)
+    g = torch.Generator().manual_seed(1)
+    hc, hm = torch.randn(2, 7, 16, generator=g) * 20, torch.randn(2, 7, 16, generator=g) * 20
+    grads, losses = [], []
+    for n_top in (None, 40, 5):
+        model = tf.TransformerDecomposedModel(arch, w, {}, attention="xla", n_top_logits=n_top, kl_token_chunk=4)
+        leaf = hm.clone().requires_grad_(True)
+        clean = SimpleNamespace(output=hc, aux={"clean_stats": model._clean_logit_stats(hc)})
+        loss = model.recon_loss(clean, SimpleNamespace(output=leaf))
+        grads.append(torch.autograd.grad(loss, (leaf,))[0])
+        losses.append(loss.detach())
+    torch.testing.assert_close(losses[1], losses[0])
+    torch.testing.assert_close(grads[1], grads[0], atol=1e-6, rtol=1e-4)
+    assert 0 < float(losses[2]) <= float(losses[0])
+
+
+def test_pretraining_on_native_kernels_needs_a_gpu(tmp_path):
+    from param_decomp_b200.pretrain.train import PretrainConfig, pretrain
+
+    cfg = PretrainConfig.model_validate(dict(run_name="t", global_batch=2, num_iterations=1, learning_rate=1e-3, kernels="native",
+                                             model=dict(vocab_size=11, n_layer=1, n_head=1, n_embd=8, n_ctx=4)))
+    with pytest.raises(ValueError, match="native"):
+        pretrain(cfg, tmp_path, run_id="t-00000009")
