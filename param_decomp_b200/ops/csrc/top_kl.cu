@@ -61,10 +61,11 @@ __device__ __forceinline__ MaxSum merge(const MaxSum& x, const MaxSum& y, float 
   const float m = fmaxf(x.m, y.m);
   return MaxSum{m, scaled(x, m, c) + scaled(y, m, c)};
 }
-// Logarithm of the sum, in 64 bits.
-__device__ __forceinline__ double log_of(const MaxSum& x, float c) {
-  const double at = moderate(x.m, c) ? power_of(x.m, c) : static_cast<double>(x.m) * c;
-  return at * 0.6931471805599453 + log(static_cast<double>(x.s));
+// Logarithm of the sum over exp(m / T), in 64 bits.
+constexpr double kLn2 = 0.6931471805599453;
+__device__ __forceinline__ double log_of(const MaxSum& x, float m, float c) {
+  const double at = moderate(x.m, c) ? power_of(x.m, c) - static_cast<double>(m) * c : (static_cast<double>(x.m) - m) * c;
+  return at * kLn2 + log(static_cast<double>(x.s));
 }
 
 struct Row {  // sums over a row: the columns that are not named, and those that are
@@ -91,7 +92,7 @@ struct Teacher {  // of a row
   float edge[16];          // elements at the row's ragged ends, named ones as -inf
   float r, named;          // probability of the tail; of all slots
   int row;                 // or -1: there is no further one
-  float top, total, tail;  // largest of the logits over T and the tail; sum of exponentials relative to it
+  float top, tail;         // largest of the logits over T and the tail; the tail
   bool live;
 };
 
@@ -206,35 +207,45 @@ __device__ void prepare(const Call& call, const RowSlice<T>& rows, long long row
     t.named = live ? s * share : 0.0f;
     t.live = live;
     t.top = top;
-    t.total = total;
     t.tail = tail;
   }
 }
 
-// One warp: the loss of a row. A logarithm of a sum is that of the sum as it stands: its rounding counts on both sides.
+// One warp: the loss of a row, sum_k p_k (a_k - b_k - log E + log Z) + r (log r - log R), with a and b the two sides' logits
+// and E and Z their sums. At a small loss a rounding of E, Z or a p_k would count in full, so all that the slots add to
+// them is formed in 64 bits; that of the student's other logits counts as R - r, which is small there, on the 32 bits of
+// its sum. The student's side is taken relative to m, one of its larger logits.
 __device__ float loss_of(const Call& call, long long row, const Teacher& t, const Row& sums, const float* named, float c,
                          int lane) {
-  const MaxSum all = merge(sums.rest, sums.top, c);
-  const double inv_t = call.inv_t, own_inv_t = static_cast<double>(c) * 0.6931471805599453;  // the sums' own 1 / T
-  const double log_all = log_of(all, c), log_total = log(static_cast<double>(t.total));
-  double sum = 0.0;
-  for (int k0 = 0; k0 < call.K; k0 += 32) {
-    const int k = k0 + lane, column = k < call.K ? t.column[k] : -1;
-    if (column != -1) {
-      const double log_p = value_at(call, row * call.K + k) * inv_t - t.top - log_total;
-      const double log_q = named[column >= 0 ? k : -2 - column] * own_inv_t - log_all;
-      const float p = expf(static_cast<float>(log_p));
-      if (!(p == 0.0f)) sum += p * (log_p - log_q);
+  const double inv_t = call.inv_t, own_inv_t = static_cast<double>(c) * kLn2;  // the sums' own 1 / T
+  const float larger = fmaxf(sums.rest.m, sums.top.m), m = larger > -INFINITY ? larger : 0.0f;
+  double teacher = 0.0, weighted = 0.0, student = 0.0;  // sums over the slots: E's part, that of E p_k (a_k - b_k), Z's part
+  for (int k = lane; k < call.K; k += 32) {
+    const int column = t.column[k];
+    if (column == -1) continue;
+    const double a = value_at(call, row * call.K + k) * inv_t - t.top;
+    const double b = (static_cast<double>(named[column >= 0 ? k : -2 - column]) - m) * own_inv_t;
+    const double e = exp(a);
+    if (!(static_cast<float>(e) == 0.0f)) {  // what is nothing in 32 bits costs nothing where the student's is -inf
+      teacher += e;
+      weighted += e * (a - b);
     }
+    if (column >= 0) student += exp(b);
   }
   __syncwarp();
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (!(t.r == 0.0f)) {
-    const double log_r = static_cast<double>(t.tail) - t.top - log_total;
-    sum += t.r * (log_r - (log_of(sums.rest, c) - log_all));
+  for (int o = 16; o > 0; o >>= 1) {
+    teacher += __shfl_xor_sync(0xffffffffu, teacher, o);
+    weighted += __shfl_xor_sync(0xffffffffu, weighted, o);
+    student += __shfl_xor_sync(0xffffffffu, student, o);
   }
-  return t.live ? static_cast<float>(sum) : 0.0f;
+  const double a_rest = static_cast<double>(t.tail) - t.top, e_rest = t.r == 0.0f ? 0.0 : exp(a_rest);
+  const double log_rest = log_of(sums.rest, m, c), total = teacher + e_rest;
+  const double log_ratio = log(exp(log_rest) + student) - log(total);
+  double sum = 0.0;
+  if (!(teacher == 0.0)) sum += weighted + teacher * log_ratio;
+  if (!(t.r == 0.0f)) sum += e_rest * (a_rest - log_rest + log_ratio);
+  return t.live ? static_cast<float>(sum / total) : 0.0f;
 }
 
 // One object: the address of its barriers goes to inline assembly, so the compiler takes every wait and barrier there for
