@@ -24,6 +24,7 @@ constexpr int kRoom = 512;  // logits collected
 constexpr int kWarps = 8, kThreads = 32 * kWarps;  // that hold a row; one more warp deals rows
 constexpr int kMaxima = 2 * kThreads;
 constexpr int kBins = 512;
+static_assert(kBins >= kRoom, "one array serves both");
 constexpr float kLog2E = 1.4426950408889634f;
 
 __device__ __forceinline__ uint32_t load_cluster_u32(uint32_t addr) {
@@ -565,13 +566,14 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
         }
         T* const row_values = values + static_cast<long long>(r) * k;
         int* const row_indices = indices + static_cast<long long>(r) * k;
+        float* const terms = reinterpret_cast<float*>(sh.hist);  // kRoom of them, its bins serve no longer
         auto put = [&](unsigned long long own, int place) {
           if (place < k) {
             store1(row_values + place, logit_of(own));
             row_indices[place] = column_of(own);
             if (place == k - 1) sh.last = own;
           } else {
-            over += ex2((logit_of(own) - low) * c);  // collected, but not among the k
+            terms[place] = ex2((logit_of(own) - low) * c);  // collected, but not among the k
           }
         };
         if (collected <= kThreads / 2) {
@@ -604,12 +606,12 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
             }
           for (int i = tid; i < collected; i += kThreads) put(sh.kept[i], i);
         }
-        // What is left: the sum relative to the bound with the collected ones that did not make it.
-        over = warp_sum(over);
-        if (lane == 0) sh.red[0][warp] = over;
+        // What is left: the sum relative to the bound with the collected ones that did not make it, added in the order of
+        // their places, not of their arrival.
         sync_first(kThreads);
-        over = 0.0f;
-        for (int w = 0; w < kWarps; ++w) over += sh.red[0][w];
+        float more = 0.0f;
+        for (int i = k + lane; i < collected; i += 32) more += terms[i];
+        over += warp_sum(more);  // every warp for itself
         float2 result = make_float2(low, sum + over);
         if (by_digits || !(over < 1e30f)) result = rest_of(row, sh.last, inv_t, sh.red);
         if (tid == 0) tail[r] = log_sum(result, inv_t);

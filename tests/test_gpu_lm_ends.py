@@ -289,6 +289,19 @@ def test_top_logits_against_a_stable_sort(nv, n, V, k, kind):
     _done(nv)
 
 
+@pytest.mark.parametrize("kind,n,V,k", [(f32, 900, 5003, 20), (bf, 900, 5003, 200), (f32, 300, 151936, 64)])
+def test_top_logits_do_not_change_from_run_to_run(nv, kind, n, V, k):
+    """Logits are collected in the order in which threads come to them; nothing of that is left in the tails."""
+    from param_decomp_b200.ops.top_logits import top_logits
+
+    z = torch.randn(n, V, generator=_gen(3)).to(kind).cuda()
+    first = top_logits(z, k)
+    for _ in range(30):
+        again = top_logits(z, k)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+    _done(nv)
+
+
 @pytest.mark.parametrize("kind", [bf, f32])
 @pytest.mark.parametrize("V,k", [(2003, 40), (50277, 64), (9000, 256)])
 def test_top_logits_of_awkward_rows(nv, V, k, kind):
