@@ -2,7 +2,7 @@
 PY ?= python
 
 .PHONY: build
-build:            ## nvcc (sm_100a) -> ops/_lib/libpdb200.so, g++ -> ops/_lib/libpdhost.so
+build:            ## nvcc (sm_100a) -> ops/_lib/libpdb200.so, g++ -> ops/_lib/libpdhost.so, ops/_lib/pd_autograd.so
 	$(PY) -m param_decomp_b200.ops.build
 
 .PHONY: test

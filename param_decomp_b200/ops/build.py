@@ -119,6 +119,45 @@ def build_host(force: bool = False) -> Path:
     return HOST_LIB_PATH
 
 
+TORCH_SRC = OPS_DIR / "csrc_torch"
+AUTOGRAD_PATH = LIB_DIR / "pd_autograd.so"
+
+
+def build_autograd(force: bool = False) -> Path:
+    """The autograd nodes that live in C++ (`csrc_torch/*.cpp`) into `ops/_lib/pd_autograd.so`, an extension module against
+    torch's headers and the kernel library beside it (`native.autograd()` loads it; there is no other path)."""
+    import sysconfig
+
+    import torch
+
+    build()  # it links against the kernels
+    sources = sorted(TORCH_SRC.glob("*.cpp"))
+    home = Path(torch.__file__).resolve().parent
+    includes = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
+                Path(_nvcc()).resolve().parent.parent / "include"]
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in includes)]
+    libs = [f"-L{home / 'lib'}", f"-L{LIB_DIR}", "-l:libpdb200.so", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10",
+            "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    h = hashlib.sha256(" ".join([torch.__version__, *flags]).encode())
+    for src in sources:
+        h.update(src.read_bytes())
+    stamp = LIB_DIR / "pd_autograd.digest"
+    digest = h.hexdigest()
+    if not force and AUTOGRAD_PATH.exists() and stamp.exists() and stamp.read_text() == digest:
+        return AUTOGRAD_PATH
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler found: the autograd nodes cannot be built")
+    res = subprocess.run([cxx, *flags, *map(str, sources), "-o", str(AUTOGRAD_PATH), *libs], capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("building the autograd nodes failed")
+    stamp.write_text(digest)
+    return AUTOGRAD_PATH
+
+
 if __name__ == "__main__":
     print(build(verbose="-v" in sys.argv, force="--force" in sys.argv))
     print(build_host(force="--force" in sys.argv))
+    print(build_autograd(force="--force" in sys.argv))

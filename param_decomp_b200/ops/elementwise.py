@@ -31,9 +31,6 @@ def _lib():
         lib.pd_swiglu_bwd.argtypes = [P, P, P, P, P, LL, P]
         lib.pd_rowscale.argtypes = [P, P, P, LL, I, P]
         lib.pd_ci_squash.argtypes = [P, P, P, LL, F, P]
-        lib.pd_layer_norm_partial_rows.argtypes = [LL, I]
-        lib.pd_layer_norm_fwd.argtypes = [P, P, P, P, P, P, LL, I, F, I, I, P]
-        lib.pd_layer_norm_bwd.argtypes = [P, P, P, P, P, P, P, P, P, LL, I, I, I, P]
         _configured = True
     return lib
 
@@ -187,59 +184,6 @@ def _flat_rows(t: Tensor, columns: int) -> Tensor:
 
 
 LAYER_NORM_MAX_COLUMNS = 12288
-_layer_norm_partial_rows = lru_cache(maxsize=256)(lambda rows, d: _lib().pd_layer_norm_partial_rows(rows, d))
-
-
-def _layer_norm_fwd(x: Tensor, w: Tensor | None, b: Tensor | None, eps: float, stats: Tensor | None) -> Tensor:
-    """`x [rows, d]` -> y; `stats [2, rows]` (or None) receives the rows' means and reciprocal deviations."""
-    rows, d = x.shape
-    y = torch.empty_like(x)
-    if rows > 0:
-        at = None if stats is None else stats.data_ptr()
-        p = w if w is not None else b
-        _check(_lib().pd_layer_norm_fwd(x.data_ptr(), None if w is None else w.data_ptr(), None if b is None else b.data_ptr(),
-                                        y.data_ptr(), at, None if at is None else at + 4 * rows, rows, d, eps,
-                                        x.dtype is torch.float32, p is not None and p.dtype is torch.float32, _s()),
-               "layer_norm_fwd")
-    return y
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Tensor:  # type: ignore[override]
-        x2 = _flat_rows(x, x.shape[-1])
-        w, b = None if w is None else _dense(w), None if b is None else _dense(b)
-        stats = torch.empty(2, x2.shape[0], device=x.device, dtype=torch.float32)
-        y = _layer_norm_fwd(x2, w, b, eps, stats)
-        ctx.save_for_backward(x2, w, stats)
-        ctx.p_dtype = b.dtype if w is None and b is not None else torch.float32 if w is None else w.dtype
-        return y if x.dim() == 2 else y.view(x.shape)
-
-    @staticmethod
-    def backward(ctx, dy: Tensor):  # type: ignore[override]
-        x2, w, stats = ctx.saved_tensors
-        rows, d = x2.shape
-        want_x, want_w, want_b, _ = ctx.needs_input_grad
-        dev, p_dtype = x2.device, ctx.p_dtype
-        dx = torch.empty_like(x2) if want_x else None
-        dw = torch.empty(d, device=dev, dtype=p_dtype) if want_w else None
-        db = torch.empty(d, device=dev, dtype=p_dtype) if want_b else None
-        if rows > 0:
-            dy2 = _flat_rows(dy, d)
-            partial = None
-            if want_w or want_b:
-                partial = torch.empty(_layer_norm_partial_rows(rows, d), 2, d, device=dev, dtype=torch.float32)
-                nv.count_launch()
-            at = stats.data_ptr()
-            _check(_lib().pd_layer_norm_bwd(x2.data_ptr(), None if w is None else w.data_ptr(), dy2.data_ptr(), at, at + 4 * rows,
-                                            None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
-                                            None if db is None else db.data_ptr(), None if partial is None else partial.data_ptr(),
-                                            rows, d, x2.dtype is torch.float32, p_dtype is torch.float32, _s()), "layer_norm_bwd")
-        else:
-            for grad in (dw, db):
-                if grad is not None:
-                    grad.zero_()
-        return None if dx is None else dx if dy.dim() == 2 else dx.view(dy.shape), dw, db, None
 
 
 def layer_norm(x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Tensor:
@@ -259,11 +203,7 @@ def layer_norm(x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Ten
     if w is not None and b is not None and w.dtype is not b.dtype:
         raise ValueError(f"layer_norm: scale and shift are of one type, not {w.dtype} and {b.dtype}")
     _on_current_device("layer_norm", x, w, b)
-    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad) or (b is not None and b.requires_grad)):
-        return _LayerNorm.apply(x, w, b, eps)
-    x2 = _flat_rows(x, x.shape[-1])
-    y = _layer_norm_fwd(x2, None if w is None else _dense(w), None if b is None else _dense(b), eps, None)
-    return y if x.dim() == 2 else y.view(x.shape)
+    return nv.autograd().layer_norm(x, w, b, eps)
 
 
 class _Rope(torch.autograd.Function):

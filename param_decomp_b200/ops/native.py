@@ -8,12 +8,15 @@ library must load, otherwise `lib()` raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 from functools import lru_cache
 from pathlib import Path
 
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libpdb200.so"
+AUTOGRAD_PATH = LIB_PATH.with_name("pd_autograd.so")
 
 EPI_PLAIN, EPI_MASK_FWD, EPI_MASK_BWD, EPI_FAITH = 0, 1, 2, 3
 ACT_NONE, ACT_GELU, ACT_SILU, ACT_RELU = 0, 1, 2, 3
@@ -67,6 +70,23 @@ def lib() -> C.CDLL:
     return handle
 
 
+_autograd = None
+
+
+def autograd():
+    """The extension module of the autograd nodes that live in C++ (`csrc_torch/`)."""
+    global _autograd
+    if _autograd is None:
+        if not AUTOGRAD_PATH.exists():
+            raise NativeError(f"{AUTOGRAD_PATH} is missing: run `python -m param_decomp_b200.ops.build` (needs g++)")
+        lib()
+        loader = importlib.machinery.ExtensionFileLoader("pd_autograd", str(AUTOGRAD_PATH))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("pd_autograd", loader))
+        loader.exec_module(module)
+        _autograd = module
+    return _autograd
+
+
 _LAUNCHES = 0
 
 
@@ -82,7 +102,7 @@ def count_launch(n: int = 1) -> None:
 
 
 def launch_count() -> int:
-    return _LAUNCHES
+    return _LAUNCHES + (0 if _autograd is None else _autograd.launches())
 
 
 def has_symbol(name: str) -> bool:
@@ -119,15 +139,25 @@ def _status_ptr(device_index: int) -> int:
     return _status_word(device_index).data_ptr()
 
 
+def status_ptr() -> int:
+    """Address of `status_word()`."""
+    return _status_ptr(torch._C._cuda_getDevice())
+
+
 @lru_cache(maxsize=8)
 def _refused_word(device_index: int) -> tuple[torch.Tensor, C.c_int]:
     word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
     return word, C.c_int.from_address(word.data_ptr())
 
 
+@lru_cache(maxsize=8)
+def _refused_ptr(device_index: int) -> int:
+    return _refused_word(device_index)[0].data_ptr()
+
+
 def refused_ptr() -> int:
     """Pinned host int32 a kernel sets beside the status word when it refuses its input, readable without a wait."""
-    return _refused_word(torch._C._cuda_getDevice())[0].data_ptr()
+    return _refused_ptr(torch._C._cuda_getDevice())
 
 
 def raise_refused() -> None:

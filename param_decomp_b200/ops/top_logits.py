@@ -34,10 +34,9 @@ class TopLogits(NamedTuple):
 @lru_cache(maxsize=1)
 def _lib():
     lib = nv.lib()
-    P, LL, I, F, D = C.c_void_p, C.c_longlong, C.c_int, C.c_float, C.c_double
+    P, LL, I, F = C.c_void_p, C.c_longlong, C.c_int, C.c_float
     lib.pd_top_logits.argtypes = [P, LL, I, LL, I, F, P, P, P, I, P, P]
     lib.pd_top_logits_max_columns.argtypes, lib.pd_top_logits_max_columns.restype = [I], LL
-    lib.pd_top_kl.argtypes = [P, LL, I, LL, P, I, P, I, I, P, D, P, P, LL, P, I, P, P, P]
     lib.pd_top_kl_max_columns.argtypes, lib.pd_top_kl_max_columns.restype = [I], LL
     return lib
 
@@ -100,48 +99,6 @@ def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     return TopLogits(values.view(*lead, k), indices.view(*lead, k), tail.view(lead))
 
 
-def _launch(z: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None, temperature: float, loss: Tensor | None,
-            dz: Tensor | None, scale: Tensor | None) -> None:
-    rows, V = z.shape
-    _check(_lib().pd_top_kl(z.data_ptr(), rows, V, _pitch(z), indices.data_ptr(), indices.dtype is torch.int64,
-                            values.data_ptr(), values.dtype is torch.float32, indices.shape[1],
-                            None if tail is None else tail.data_ptr(), 1.0 / temperature,
-                            None if loss is None else loss.data_ptr(), None if dz is None else dz.data_ptr(),
-                            0 if dz is None else dz.stride(0), None if scale is None else scale.data_ptr(),
-                            z.dtype is torch.float32, nv.status_word().data_ptr(), nv.refused_ptr(), _s()), "top_kl")
-
-
-def _grad_like(z: Tensor) -> Tensor:
-    """`[rows, V]` whose rows start at the same address modulo 16 bytes as the rows of `z`."""
-    per = 16 // z.element_size()
-    rows, V = z.shape
-    pitch = V + (_pitch(z) - V) % per
-    first = z.data_ptr() % 16 // z.element_size()
-    return torch.empty(first + rows * pitch, device=z.device, dtype=z.dtype).as_strided((rows, V), (pitch, 1), first)
-
-
-class _TopKL(torch.autograd.Function):
-    """The backward runs the kernel again with the upstream gradient of each row: 2 reads and a write of the logits for
-    both passes, against a read and two writes had the forward kept an unscaled gradient, and nothing is held between."""
-
-    @staticmethod
-    def forward(ctx, z: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None, temperature: float) -> Tensor:  # type: ignore[override]
-        loss = torch.empty(z.shape[0], device=z.device, dtype=torch.float32)
-        if z.shape[0] > 0:
-            _launch(z, indices, values, tail, temperature, loss, None, None)
-        ctx.save_for_backward(z, indices, values, tail)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    def backward(ctx, dloss: Tensor):  # type: ignore[override]
-        z, indices, values, tail = ctx.saved_tensors
-        dz = _grad_like(z)
-        if z.shape[0] > 0:
-            _launch(z, indices, values, tail, ctx.temperature, None, dz, _dense(dloss))
-        return dz, None, None, None, None
-
-
 def _arguments(what: str, logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None, temperature: float):
     _check_logits(what, logits, temperature)
     lead = logits.shape[:-1]
@@ -172,12 +129,7 @@ def top_kl(logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None 
     logsumexp of all other logits over the temperature; without it the teacher has its `k` slots alone. Both sides are taken
     at `temperature`. A row whose teacher has no mass counts zero, with a zero gradient."""
     z, indices, values, tail = _arguments("top_kl", logits, indices, values, tail, temperature)
-    if z.requires_grad and torch.is_grad_enabled():
-        loss = _TopKL.apply(z, indices, values, tail, temperature)
-    else:
-        loss = torch.empty(z.shape[0], device=z.device, dtype=torch.float32)
-        if z.shape[0] > 0:
-            _launch(z, indices, values, tail, temperature, loss, None, None)
+    loss = nv.autograd().top_kl(z, indices, values, tail, temperature, nv.status_ptr(), nv.refused_ptr())
     return loss if logits.dim() == 2 else loss.view(logits.shape[:-1])
 
 
@@ -188,11 +140,7 @@ def top_kl_rows(logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | 
     if logits.dim() != 2:
         raise ValueError(f"top_kl_rows: logits [rows, V], not {tuple(logits.shape)}")
     z, indices, values, tail = _arguments("top_kl_rows", logits.detach(), indices, values, tail, temperature)
-    loss = torch.empty(z.shape[0], device=z.device, dtype=torch.float32)
-    dz = _grad_like(z) if want_grad else None
-    if z.shape[0] > 0:
-        _launch(z, indices, values, tail, temperature, loss, dz, None)
-    return loss, dz
+    return nv.autograd().top_kl_rows(z, indices, values, tail, temperature, want_grad, nv.status_ptr(), nv.refused_ptr())
 
 
 def next_token_loss(logits: Tensor, targets: Tensor) -> Tensor:

@@ -696,3 +696,66 @@ def test_graphs_and_streams(nv):
     for j in range(2):
         assert all(torch.equal(a, b) for a, b in zip(got[j], want[j + 1]))
     _done(nv)
+
+
+def _differentiable():
+    """(name, leaves, function of the leaves) of every operator with a gradient."""
+    from param_decomp_b200.ops.elementwise import layer_norm
+    from param_decomp_b200.ops.embedding import embedding
+    from param_decomp_b200.ops.top_logits import top_kl
+
+    g = _gen(6)
+    leaf = lambda *shape: torch.randn(*shape, generator=g).cuda().requires_grad_(True)  # noqa: E731
+    tokens, idx, t = (torch.randint(0, 50, (40,), generator=g).cuda(), torch.randint(0, 50, (7, 3), generator=g).cuda(),
+                      torch.randn(7, 3, generator=g).cuda())
+    return [("layer_norm", (leaf(5, 24), leaf(24), leaf(24)), lambda x, w, b: layer_norm(x, w, b, 1e-5)),
+            ("embedding", (leaf(50, 8),), lambda table: embedding(tokens, table, 2.0)),
+            ("top_kl", (leaf(7, 50),), lambda z: top_kl(z, idx, t))]
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_second_backwards(nv, which):
+    """A kept graph gives the same gradients again, a freed one raises, and a gradient that is differentiated again raises
+    (alone or beside a path that is differentiable twice) where it would otherwise count as a constant."""
+    name, leaves, f = _differentiable()[which]
+    y = f(*leaves)
+    up = torch.rand(y.shape, generator=_gen(1)).cuda()
+    first = torch.autograd.grad(y, leaves, up, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, up)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(y, leaves, up)
+    y = f(*leaves)
+    mixed = (y * y.detach()).sum() + sum((p ** 3).sum() for p in leaves)
+    grads = torch.autograd.grad(mixed, leaves, create_graph=True)
+    with pytest.raises(RuntimeError, match=f"{name} is not differentiable twice"):
+        torch.autograd.grad(sum(g.sum() for g in grads), leaves)
+    _done(nv)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_some_gradients_and_accumulated_ones(nv, which):
+    """Each leaf's gradient asked for alone; `.grad` added up over two backwards; gradients that come broadcast."""
+    _, leaves, f = _differentiable()[which]
+    y = f(*leaves)
+    whole = torch.autograd.grad(y.sum(), leaves)
+    for i, leaf in enumerate(leaves):
+        (alone,) = torch.autograd.grad(f(*(p if j == i else p.detach() for j, p in enumerate(leaves))).sum(), (leaf,))
+        assert torch.equal(alone, whole[i])
+    for _ in range(2):
+        f(*leaves).sum().backward()
+    assert all(torch.equal(p.grad, 2 * g) for p, g in zip(leaves, whole))
+    with torch.no_grad():
+        assert not f(*leaves).requires_grad and torch.equal(f(*leaves), y)
+    _done(nv)
+
+
+def test_values_changed_between_the_passes_are_noticed(nv):
+    """What a backward reads must be what its forward read."""
+    for _, leaves, f in _differentiable()[::2]:
+        x = leaves[0] * 1.0
+        y = f(x, *leaves[1:])
+        x.add_(1.0)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.sum().backward()
+    _done(nv)

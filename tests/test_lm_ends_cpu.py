@@ -176,3 +176,12 @@ def test_pretraining_on_native_kernels_needs_a_gpu(tmp_path):
                                              model=dict(vocab_size=11, n_layer=1, n_head=1, n_embd=8, n_ctx=4)))
     with pytest.raises(ValueError, match="native"):
         pretrain(cfg, tmp_path, run_id="t-00000009")
+
+
+def test_a_missing_extension_is_said_aloud(monkeypatch, tmp_path):
+    from param_decomp_b200.ops import native
+
+    monkeypatch.setattr(native, "AUTOGRAD_PATH", tmp_path / "pd_autograd.so")
+    monkeypatch.setattr(native, "_autograd", None)
+    with pytest.raises(NativeError, match="ops.build"):
+        native.autograd()
