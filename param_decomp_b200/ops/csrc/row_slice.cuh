@@ -133,17 +133,18 @@ struct RowSlice {
   }
 };
 
-// How rows of V columns are spread: the smallest cluster whose slices leave room for two blocks an SM (`half` bytes);
-// past 8 blocks, up to `whole` bytes. cs = 0: no cluster holds such a row.
+// How rows of V columns are spread: the smallest cluster whose slices leave room for two blocks an SM (`half` bytes, of
+// which `each` a block of the cluster are taken, where there is more than one); past 8 blocks, up to `whole` bytes.
+// cs = 0: no cluster holds such a row.
 struct SlicePlan {
   int cs, slice, per;
 };
 template <typename T>
-inline SlicePlan slice_plan(long long V, int warps, long long half, long long whole) {
+inline SlicePlan slice_plan(long long V, int warps, long long half, long long whole, long long each = 0) {
   constexpr long long kE = 16 / sizeof(T);
   const long long groups = (V + 2 * kE - 2) / kE;  // wherever a row starts
   int cs = 1;
-  while (cs < 8 && (groups + cs - 1) / cs * 16 > half) cs *= 2;
+  while (cs < 8 && (groups + cs - 1) / cs * 16 + (cs > 1 ? cs * each : 0) > half) cs *= 2;
   const long long slice = (groups + cs - 1) / cs;
   if (slice * 16 > whole) return {0, 0, 0};
   return {cs, static_cast<int>(slice), static_cast<int>((slice + warps - 1) / warps)};

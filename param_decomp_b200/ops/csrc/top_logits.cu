@@ -21,10 +21,11 @@ using namespace pd;
 
 constexpr int kMaxK = 256;
 constexpr int kRoom = 512;  // logits collected
-constexpr int kWarps = 8, kThreads = 32 * kWarps;  // that hold a row; one more warp deals rows
+constexpr int kWarps = 8, kThreads = 32 * kWarps;  // that hold a row; one more warp deals rows,
+constexpr int kSelWarps = 4, kSelThreads = 32 * kSelWarps;  // and these select, in a cluster's first block, a row behind
 constexpr int kMaxima = 2 * kThreads;
 constexpr int kBins = 512;
-static_assert(kBins >= kRoom, "one array serves both");
+constexpr int kSelBins = 256;
 constexpr float kLog2E = 1.4426950408889634f;
 
 __device__ __forceinline__ uint32_t load_cluster_u32(uint32_t addr) {
@@ -144,14 +145,20 @@ struct Row {
   __device__ __forceinline__ bool inside(int col) const { return col >= 0 && col < V; }
 };
 
+// The barrier of the warps that select.
+__device__ __forceinline__ void sync_selectors() {
+  __syncwarp();
+  asm volatile("barrier.sync 2, %0;" ::"n"(kSelThreads) : "memory");
+}
+
 // The columns behind the place `last` of the k-th: their maximum m, and the sum of exp((z - m) / T).
 template <typename T>
-__device__ float2 rest_of(const Row<T>& row, unsigned long long last, float inv_t, float (*red)[32]) {
+__device__ float2 rest_of(const Row<T>& row, unsigned long long last, float inv_t, int st, float (*red)[32]) {
   constexpr int kE = Row<T>::kE;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kWarps;
+  const int lane = st & 31, warp = st >> 5, warps = kSelWarps;
   float m = -INFINITY;
   bool nan = false;
-  for (int g = threadIdx.x; g < row.groups; g += kThreads) {
+  for (int g = st; g < row.groups; g += kSelThreads) {
     float v[kE];
     Row<T>::values(row.load(g), v);
 #pragma unroll
@@ -166,9 +173,9 @@ __device__ float2 rest_of(const Row<T>& row, unsigned long long last, float inv_
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   nan = __any_sync(0xffffffffu, nan);
-  sync_first(kThreads);
+  sync_selectors();
   if (lane == 0) red[0][warp] = nan ? NAN : m;
-  sync_first(kThreads);
+  sync_selectors();
   nan = false;
   for (int w = 0; w < warps; ++w) {
     nan |= red[0][w] != red[0][w];
@@ -176,7 +183,7 @@ __device__ float2 rest_of(const Row<T>& row, unsigned long long last, float inv_
   }
   float s = 0.0f;
   if (m > -INFINITY && m < INFINITY) {
-    for (int g = threadIdx.x; g < row.groups; g += kThreads) {
+    for (int g = st; g < row.groups; g += kSelThreads) {
       float v[kE];
       Row<T>::values(row.load(g), v);
 #pragma unroll
@@ -188,28 +195,28 @@ __device__ float2 rest_of(const Row<T>& row, unsigned long long last, float inv_
   }
   s = warp_sum(s);
   if (lane == 0) red[1][warp] = s;
-  sync_first(kThreads);
+  sync_selectors();
   s = 0.0f;
   for (int w = 0; w < warps; ++w) s += red[1][w];
-  sync_first(kThreads);
+  sync_selectors();
   if (nan) return make_float2(INFINITY, NAN);
   return make_float2(m, m == INFINITY ? 1.0f : s);
 }
 
 // The k-th largest (value, column) place by the keys' digits from the top; leaves the k best in `kept` (any order).
 template <typename T>
-__device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* kept, int* hist, int* shared) {
+__device__ void select_by_digits(const Row<T>& row, int k, int tid, unsigned long long* kept, int* hist, int* shared) {
   constexpr int kE = Row<T>::kE;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = tid & 31, warp = tid >> 5;
   uint32_t prefix = 0;
   int need = k;
   constexpr int kDigits = sizeof(T);  // bf16 keys are settled by their upper 16 bits
 #pragma unroll 1
   for (int digit = 0; digit < kDigits; ++digit) {
     const int down = 24 - 8 * digit;
-    for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
-    sync_first(kThreads);
-    for (int g = tid; g < row.groups; g += kThreads) {
+    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+    sync_selectors();
+    for (int g = tid; g < row.groups; g += kSelThreads) {
       float v[kE];
       Row<T>::values(row.load(g), v);
 #pragma unroll
@@ -219,7 +226,7 @@ __device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* k
           atomicAdd(hist + ((key >> down) & 255), 1);
       }
     }
-    sync_first(kThreads);
+    sync_selectors();
     if (warp == 0) {  // lane l holds the eight bins 255 - 8 l and below: from the largest digit down
       int sum = 0;
 #pragma unroll
@@ -243,16 +250,16 @@ __device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* k
         }
       }
     }
-    sync_first(kThreads);
+    sync_selectors();
     prefix = prefix << 8 | static_cast<uint32_t>(shared[0]);
     need = shared[1];
-    sync_first(kThreads);
+    sync_selectors();
   }
   // everything above the k-th key, and the first `need` columns that hold it
   if (tid == 0) shared[0] = shared[1] = 0;
-  sync_first(kThreads);
+  sync_selectors();
   constexpr int kDown = 32 - 8 * kDigits;
-  for (int g0 = 0; g0 < row.groups; g0 += kThreads) {
+  for (int g0 = 0; g0 < row.groups; g0 += kSelThreads) {
     const int g = g0 + tid;
     float v[kE];
     int equal = 0;
@@ -274,9 +281,9 @@ __device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* k
       if (lane >= o) upto += u;
     }
     if (lane == 31) hist[warp] = upto;
-    sync_first(kThreads);
+    sync_selectors();
     int before = shared[1] + upto - equal, all = 0;
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kSelWarps; ++w) {
       if (w < warp) before += hist[w];
       all += hist[w];
     }
@@ -289,37 +296,210 @@ __device__ void select_by_digits(const Row<T>& row, int k, unsigned long long* k
         ++before;
       }
     }
-    sync_first(kThreads);
+    sync_selectors();
     if (tid == 0) shared[1] += all;
-    sync_first(kThreads);
+    sync_selectors();
   }
 }
 
 // log of s exp(m / T); s = 0 for nothing, and for an infinite m whatever it is (NaN stays NaN).
 __device__ __forceinline__ float log_sum(float2 r, float inv_t) { return r.x > -INFINITY && r.x < INFINITY ? r.x * inv_t + logf(r.y) : r.x + 0.0f * r.y; }
 
-struct Shared {  // one object, whose address inline assembly gets: waits there may change any part of it
+// One object, whose address inline assembly gets: waits there may change any part of it. What belongs to a row is there
+// twice and taken in turns: warps of the block may be in neighbouring rows, and the selection of a row goes on while the
+// next one is read.
+struct Shared {
   RowQueue queue;
-  unsigned long long bars[kWarps + 6];
-  unsigned long long kept[kRoom], last;
-  float red[2][32], sums[kWarps], sum;
-  alignas(16) int hist[kBins];
-  int pair[2];
+  unsigned long long bars[kWarps + 10];
+  unsigned long long kept[2][kRoom], last;
+  alignas(16) int hist[2][kBins];
+  float sums[2][kWarps];
+  uint32_t top[2];  // the largest key
+  int found[2], next[2];
+  struct {
+    int row;  // or -1: there is no further one
+    float low, power;
+    bool by_digits;
+  } work[2];
   struct {
     int row;
     float edge[16];
   } ahead[3];  // rows to come, with the elements at their ragged ends
-  uint32_t top;  // the largest key
-  int found, next, abort_flag;
+  // the selecting warps'
+  int bins[kSelBins + 1], pair[2], row;
+  uint32_t ends[2][kSelWarps];
+  float red[2][32];
+  int abort_flag;
 };
+constexpr int kShared = 14848;
+static_assert(sizeof(Shared) <= kShared);
+
+// The selection of the rows that a cluster has read: its first block's selecting warps, thread st of them.
+template <typename T>
+__device__ void select_rows(Shared& sh, const RowSlice<T>& rows, int cs, int k, float inv_t, T* values, int* indices,
+                            float* tail, int* status, uint32_t collected_bar, uint32_t selected_bar, int st) {
+  const int lane = st & 31, sw = st >> 5;
+  const float c = inv_t * kLog2E;
+  for (int n = 0;; ++n) {
+    const int turn = n & 1;
+    if (sw == 0) {  // all of them go on, or none does
+      const uint32_t bar = collected_bar + 8 * turn, phase = (n >> 1) & 1;
+      const bool in_time = cs > 1 ? short_wait<true>(bar, phase, &sh.abort_flag) : short_wait<false>(bar, phase, &sh.abort_flag);
+      if (!in_time && status != nullptr) atomicCAS(status, 0, kTimeoutProducer);
+      if (lane == 0) sh.row = in_time ? sh.work[turn].row : -1;
+    }
+    sync_selectors();
+    const int r = sh.row;
+    if (r < 0) break;
+    const float low = sh.work[turn].low, power = sh.work[turn].power;
+    bool by_digits = sh.work[turn].by_digits;
+    const Row<T> row(rows.row(r), rows.V);
+    unsigned long long* const kept = sh.kept[turn];
+    float sum = 0.0f, over = 0.0f;
+    int collected = 0;
+    if (!by_digits) {
+      if (cs == 1) {
+        collected = sh.found[turn];
+        for (int w = 0; w < kWarps; ++w) sum += sh.sums[turn][w];
+      } else {
+        // every warp reads all counts and sums for itself, then its share of the lists
+        const uint32_t there = mapa_shared(smem_u32(&sh), lane & 7);  // of block lane, where there is one
+        auto of = [&](const void* x) { return there + (smem_u32(x) - smem_u32(&sh)); };
+        const int count = lane < cs ? static_cast<int>(load_cluster_u32(of(sh.found + turn))) : 0;
+        if (lane < cs)
+          for (int w = 0; w < kWarps; ++w) sum += __uint_as_float(load_cluster_u32(of(sh.sums[turn] + w)));
+        sum = warp_sum(sum);
+        int upto = count;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        collected = __shfl_sync(0xffffffffu, upto, 7);
+        for (int b = 1 + sw; b < cs; b += kSelWarps) {
+          const int mine = __shfl_sync(0xffffffffu, count, b), at = __shfl_sync(0xffffffffu, upto, b) - mine;
+          const uint32_t list = mapa_shared(smem_u32(kept), b);
+          for (int i = lane; i < mine && at + i < kRoom; i += 32) kept[at + i] = load_cluster_u64(list + 8 * i);
+        }
+        sync_selectors();
+      }
+    }
+    by_digits |= collected > kRoom;
+    if (by_digits) {
+      select_by_digits(row, k, st, kept, sh.bins, sh.pair);
+      collected = k;
+    } else {
+      const float taken = static_cast<float>(collected) * ex2(fmaf(low, c, -power));
+      over = sum < 1.0625f * taken ? INFINITY : 0.0f;  // too little is left of it
+      sum = (sum - taken) * ex2(fmaf(-low, c, power));  // relative to exp(low / T) from here on
+    }
+    // Places: sorted into 256 bins by key, each then counted within its bin. Every place differs from every other.
+    constexpr int kOwn = kRoom / kSelThreads;
+    unsigned long long own[kOwn];
+    uint32_t hi = 0, lo = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int at = st + i * kSelThreads;
+      own[i] = at < collected ? kept[at] : 0ull;
+      if (at < collected) {
+        const uint32_t key = static_cast<uint32_t>(own[i] >> 32);
+        hi = max(hi, key);
+        lo = min(lo, key);
+      }
+    }
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    if (lane == 0) {
+      sh.ends[0][sw] = hi;
+      sh.ends[1][sw] = lo;
+    }
+    for (int i = st; i < kSelBins; i += kSelThreads) sh.bins[i] = 0;
+    sync_selectors();
+#pragma unroll
+    for (int w = 0; w < kSelWarps; ++w) {
+      hi = max(hi, sh.ends[0][w]);
+      lo = min(lo, sh.ends[1][w]);
+    }
+    const int down = max(0, 24 - __clz(hi - lo));
+    int bin[kOwn], before[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      bin[i] = static_cast<int>((hi - static_cast<uint32_t>(own[i] >> 32)) >> down);
+      before[i] = st + i * kSelThreads < collected ? atomicAdd(sh.bins + bin[i], 1) : 0;
+    }
+    sync_selectors();
+    if (sw == 0) {  // counts become the places at which bins begin
+      int count[kSelBins / 32], all = 0;
+#pragma unroll
+      for (int j = 0; j < kSelBins / 32; ++j) {
+        count[j] = sh.bins[kSelBins / 32 * lane + j];
+        all += count[j];
+      }
+      int upto = all;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      int begin = upto - all;
+#pragma unroll
+      for (int j = 0; j < kSelBins / 32; ++j) {
+        sh.bins[kSelBins / 32 * lane + j] = begin;
+        begin += count[j];
+      }
+      if (lane == 31) sh.bins[kSelBins] = begin;
+    }
+    sync_selectors();
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+      if (st + i * kSelThreads < collected) kept[sh.bins[bin[i]] + before[i]] = own[i];
+    sync_selectors();
+    float more[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      more[i] = 0.0f;
+      before[i] = 0;
+      if (st + i * kSelThreads < collected) {
+        const int from = sh.bins[bin[i]], to = sh.bins[bin[i] + 1];
+        int place = from;
+        for (int j = from; j < to; ++j) place += kept[j] > own[i];
+        if (place < k) {
+          const long long at = static_cast<long long>(r) * k + place;
+          store1(values + at, logit_of(own[i]));
+          indices[at] = column_of(own[i]);
+          if (place == k - 1) sh.last = own[i];
+        } else {
+          more[i] = ex2((logit_of(own[i]) - low) * c);  // collected, but not among the k
+        }
+        before[i] = place;
+      }
+    }
+    sync_selectors();
+    // What is left: the sum relative to the bound with the collected ones that did not make it, added in the order of
+    // their places, not of their arrival.
+    float* const terms = reinterpret_cast<float*>(kept);
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+      if (before[i] >= k) terms[before[i] - k] = more[i];
+    sync_selectors();
+    float added = 0.0f;
+    for (int i = lane; i < collected - k; i += 32) added += terms[i];
+    over += warp_sum(added);  // every warp for itself
+    float2 result = make_float2(low, sum + over);
+    if (by_digits || !(over < 1e30f)) result = rest_of(row, sh.last, inv_t, st, sh.red);
+    if (st == 0) tail[r] = log_sum(result, inv_t);
+    sync_selectors();
+    if (st == 0) mbar_arrive(selected_bar + 8 * turn);
+  }
+}
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* __restrict__ z, long long ld, int V, int k,
+__global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_kernel(const T* __restrict__ z, long long ld, int V, int k,
                                                                       float inv_t, SlicePlan plan, T* __restrict__ values,
                                                                       int* __restrict__ indices, float* __restrict__ tail,
                                                                       int* __restrict__ status) {
   constexpr int kE = Row<T>::kE;
-  extern __shared__ __align__(128) uint8_t smem[];  // the slice; behind it, in a cluster, [cs][kMaxima] maxima
+  extern __shared__ __align__(128) uint8_t smem[];  // the slice; behind it, in a cluster, [2][cs][kMaxima] maxima
   __shared__ __align__(16) Shared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cs = plan.cs;
   const int rank = cs > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -327,14 +507,16 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
   unsigned short* maxima = reinterpret_cast<unsigned short*>(smem + 16ll * plan.slice);
   T* buf = reinterpret_cast<T*>(smem);
   const float c = inv_t * kLog2E;
-  const uint32_t bar0 = smem_u32(sh.bars), ready = bar0 + 8 * kWarps, done = ready + 16, met = ready + 32;
+  const uint32_t bar0 = smem_u32(sh.bars), ready = bar0 + 8 * kWarps, done = ready + 16, selected = ready + 32,
+                 collected = ready + 48, met = ready + 64;
   if (tid == 0) {
-    for (int i = 0; i < kWarps + 4; ++i) mbar_init(bar0 + 8 * i, 1);
+    for (int i = 0; i < kWarps + 6; ++i) mbar_init(bar0 + 8 * i, 1);
+    mbar_init(collected, cs * kWarps);
+    mbar_init(collected + 8, cs * kWarps);
     mbar_init(met, cs);
-    mbar_init(met + 8, cs);
     sh.queue.init();
     sh.abort_flag = 0;
-    sh.top = 0;
+    sh.top[0] = sh.top[1] = 0;
     mbar_fence_init();
   }
   __syncthreads();
@@ -344,7 +526,9 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
   };
   // The n-th completion of a pair of barriers that take turns.
   auto wait_pair = [&](uint32_t pair, int n) { return short_wait<false>(pair + 8 * (n & 1), (n >> 1) & 1, &sh.abort_flag); };
-  if (warp == kWarps) {  // rows to come, two ahead
+  if (warp > kWarps) {
+    if (rank == 0) select_rows(sh, rows, cs, k, inv_t, values, indices, tail, status, collected, selected, tid - kThreads - 32);
+  } else if (warp == kWarps) {  // rows to come, two ahead
     bool more = true;
     if (rank == 0 && lane == 0) sh.queue.ask();
     __syncwarp();
@@ -365,7 +549,7 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
         int col;
         if (rows.edge_place(lane, rows.shift(row), col) >= 0 && col >= 0 && col < V) edge = as_float(rows.row(row)[col]);
       }
-      if (n >= 2) late(wait_pair(done, n - 2));  // the row before the present one has been left
+      if (n >= 2) late(wait_pair(done, n - 2));  // all warps have been past the first barrier of that row
       if (lane < 2 * kE) sh.ahead[n % 3].edge[lane] = edge;
       if (lane == 0) sh.ahead[n % 3].row = row;
       __syncwarp();
@@ -377,11 +561,21 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
     if (lane == 0) rows.request(blockIdx.x / cs, warp, smem, bar0 + 8 * warp, false);
     __syncwarp();
     late(wait_pair(ready, 0));
+    auto hand_over = [&](int n) {  // the warp, to the selecting warps of the first block
+      __syncwarp();
+      if (lane == 0) {
+        if (cs > 1)
+          mbar_arrive_cluster(mapa_shared(collected + 8 * (n & 1), 0));
+        else
+          mbar_arrive(collected + 8 * (n & 1));
+      }
+      __syncwarp();
+    };
     int n = 0;
     for (int r = blockIdx.x / cs; r >= 0; ++n) {
+      const int turn = n & 1;
       const int shift = rows.shift(r), groups = rows.groups(shift);
       const int begin = warp * plan.per + lane, stop = min(groups, (warp + 1) * plan.per);
-      const Row<T> row(rows.row(r), V);
       late(short_wait<false>(bar0 + 8 * warp, n & 1, &sh.abort_flag));
       // a ragged end is written by the warp that reads it
       if (warp == 0 || stop == groups) {
@@ -391,10 +585,10 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
         fence_proxy_async_smem();  // before bulk copies of the next row write there
         __syncwarp();
       }
-      bool by_digits = min(kMaxima, row.groups) < 2 * k;  // from sizes alone: the same in every block
-      float low = 0.0f, sum = 0.0f, over = 0.0f, power = 0.0f;
+      bool by_digits = min(kMaxima, (shift + V + kE - 1) / kE) < 2 * k;  // from sizes alone: the same in every block
+      float low = 0.0f, power = 0.0f;
       uint32_t keys = 0;
-      int collected = 0;
+      int* const hist = sh.hist[turn];
       if (!by_digits) {
         GroupMax<T> m0, m1;
         int g = begin;
@@ -406,45 +600,47 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
         if (g < stop) m0.add(*reinterpret_cast<const uint4*>(smem + 16 * g));
         keys = key_of(m0.value()) >> 16 | (key_of(m1.value()) & 0xFFFF0000u);
         if (cs > 1) {
-          const uint32_t local = smem_u32(maxima + rank * kMaxima + 2 * tid);
+          const uint32_t local = smem_u32(maxima + (turn * cs + rank) * kMaxima + 2 * tid);
           for (int b = 0; b < cs; ++b)
             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(local, b)), "r"(keys) : "memory");
         } else {
           const uint32_t most = __reduce_max_sync(0xffffffffu, max(keys >> 16, keys & 0xFFFFu));
-          if (lane == 0) atomicMax(&sh.top, most);
-          if (tid == 0) sh.found = 0;
+          if (lane == 0) atomicMax(sh.top + turn, most);
         }
-        sh.hist[tid] = sh.hist[tid + kThreads] = 0;
+        hist[tid] = hist[tid + kThreads] = 0;
       }
       if (tid == 0) {  // all warps go on together, or none does: what the barrier below shows them decides
         late(wait_pair(ready, n + 1));
-        sh.next = *static_cast<volatile int*>(&sh.abort_flag) ? -1 : sh.ahead[(n + 1) % 3].row;
+        if (rank == 0 && n >= 2) late(wait_pair(selected, n - 2));  // the list of two rows ago has been read
+        if (cs == 1) sh.found[turn] = 0;
+        sh.next[turn] = *static_cast<volatile int*>(&sh.abort_flag) ? -1 : sh.ahead[(n + 1) % 3].row;
       }
       sync_first(kThreads);
-      const int next = sh.next;
+      const int next = sh.next[turn];
+      if (tid == 0) sh.top[turn ^ 1] = 0;
       if (!by_digits) {
         if (cs > 1) {
           if (warp == 0 && lane < cs) mbar_arrive_cluster(mapa_shared(met, lane));
           __syncwarp();
           late(short_wait<true>(met, n & 1, &sh.abort_flag));
-          for (int b = 0; b < cs; ++b) keys = __vmaxu2(keys, reinterpret_cast<const uint32_t*>(maxima + b * kMaxima)[tid]);
+          for (int b = 0; b < cs; ++b) keys = __vmaxu2(keys, reinterpret_cast<const uint32_t*>(maxima + (turn * cs + b) * kMaxima)[tid]);
           const uint32_t most = __reduce_max_sync(0xffffffffu, max(keys >> 16, keys & 0xFFFFu));
-          if (lane == 0) atomicMax(&sh.top, most);
-          if (tid == 0) sh.found = 0;  // the first block has come to this row: it is done with the last one's list
+          if (lane == 0) atomicMax(sh.top + turn, most);
+          if (tid == 0) sh.found[turn] = 0;  // the first block has come to this row: it has read the list of two rows ago
           sync_first(kThreads);
         }
         // The k-th largest of the maxima in the upper 16 bits of its key, rounded down: by a histogram of their distances
         // from the largest, 128 bins an octave; where that does not reach far enough, of 16 and then of one.
-        const uint32_t top = sh.top;
+        const uint32_t top = sh.top[turn];
         uint32_t bound;
         for (int coarse = 0;; coarse = coarse == 0 ? 3 : 7) {
-          atomicAdd(sh.hist + min(kBins - 1, (top - (keys >> 16)) >> coarse), 1);
-          atomicAdd(sh.hist + min(kBins - 1, (top - (keys & 0xFFFFu)) >> coarse), 1);
+          atomicAdd(hist + min(kBins - 1, (top - (keys >> 16)) >> coarse), 1);
+          atomicAdd(hist + min(kBins - 1, (top - (keys & 0xFFFFu)) >> coarse), 1);
           sync_first(kThreads);
           int count[kBins / 32], total = 0;  // every warp for itself
 #pragma unroll
           for (int i = 0; i < kBins / 128; ++i) {
-            const int4 q = reinterpret_cast<const int4*>(sh.hist)[kBins / 128 * lane + i];
+            const int4 q = reinterpret_cast<const int4*>(hist)[kBins / 128 * lane + i];
             count[4 * i] = q.x, count[4 * i + 1] = q.y, count[4 * i + 2] = q.z, count[4 * i + 3] = q.w;
             total += q.x + q.y + q.z + q.w;
           }
@@ -468,10 +664,9 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
             break;
           }
           sync_first(kThreads);
-          sh.hist[tid] = sh.hist[tid + kThreads] = 0;
+          hist[tid] = hist[tid + kThreads] = 0;
           sync_first(kThreads);
         }
-        if (tid == 0) sh.top = 0;
         low = value_of(bound << 16);
         if (sizeof(T) == 2) low = __uint_as_float(__float_as_uint(low) & 0xFFFF0000u);  // the bf16 number of that key
         // Sums are relative to 2^power, so that one fused multiply-add gives an exponent.
@@ -506,13 +701,13 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
             const int g = begin + 32 * (__ffsll(noted) - 1);
             for (uint32_t bits = reached<T>(*reinterpret_cast<const uint4*>(smem + 16 * g), low); bits != 0; bits &= bits - 1) {
               const int j = __ffs(bits) - 1, col = (rows.g0 + g) * kE - shift + j;
-              const int at = col >= 0 && col < V ? atomicAdd(&sh.found, 1) : kRoom;
-              if (at < kRoom) sh.kept[at] = place_of(as_float(buf[g * kE + j]), col);
+              const int at = col >= 0 && col < V ? atomicAdd(sh.found + turn, 1) : kRoom;
+              if (at < kRoom) sh.kept[turn][at] = place_of(as_float(buf[g * kE + j]), col);
             }
           }
           const float2 a = unpack2(add2(s0, s1));
-          sum = warp_sum(a.x + a.y);
-          if (lane == 0) sh.sums[warp] = sum;
+          const float sum = warp_sum(a.x + a.y);
+          if (lane == 0) sh.sums[turn][warp] = sum;
         }
       }
       __syncwarp();
@@ -521,131 +716,49 @@ __global__ void __launch_bounds__(kThreads + 32, 3) top_logits_kernel(const T* _
         rows.request(next, warp, smem, bar0 + 8 * warp, false);
       }
       __syncwarp();
-      sync_first(kThreads);
-      sum = 0.0f;
-      for (int w = 0; w < kWarps; ++w) sum += sh.sums[w];
-      collected = sh.found;
-      if (cs > 1) {  // the first block takes over; the others write to their lists again when it has come to the next row
-        if (tid == 0) {
-          sh.sum = sum;
-          mbar_arrive_cluster(mapa_shared(met + 8, 0));
-        }
-        __syncwarp();
-        if (rank == 0) {
-          late(short_wait<true>(met + 8, n & 1, &sh.abort_flag));
-          if (!by_digits) {
-            // warp b copies block b's list; every warp reads all counts and sums for itself
-            const int count = lane < cs ? static_cast<int>(load_cluster_u32(mapa_shared(smem_u32(&sh.found), lane))) : 0;
-            sum = lane < cs ? __uint_as_float(load_cluster_u32(mapa_shared(smem_u32(&sh.sum), lane))) : 0.0f;
-            int upto = count;
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) {
-              const int v = __shfl_up_sync(0xffffffffu, upto, o);
-              if (lane >= o) upto += v;
-            }
-            sum = warp_sum(sum);
-            const int mine = __shfl_sync(0xffffffffu, count, warp), at = __shfl_sync(0xffffffffu, upto, warp) - mine;
-            collected = __shfl_sync(0xffffffffu, upto, 7);
-            if (warp > 0 && warp < cs) {
-              const uint32_t list = mapa_shared(smem_u32(sh.kept), warp);
-              for (int i = lane; i < mine && at + i < kRoom; i += 32) sh.kept[at + i] = load_cluster_u64(list + 8 * i);
-            }
-          }
-          sync_first(kThreads);
-        }
+      if (tid == 0) {
+        sh.work[turn].row = r;
+        sh.work[turn].low = low;
+        sh.work[turn].power = power;
+        sh.work[turn].by_digits = by_digits;
       }
-      if (rank == 0) {
-        by_digits |= collected > kRoom;
-        if (by_digits) {
-          select_by_digits(row, k, sh.kept, sh.hist, sh.pair);
-          collected = k;
-        } else {
-          const float taken = static_cast<float>(collected) * ex2(fmaf(low, c, -power));
-          over = sum < 1.0625f * taken ? INFINITY : 0.0f;  // too little is left of it
-          sum = (sum - taken) * ex2(fmaf(-low, c, power));  // relative to exp(low / T) from here on
-        }
-        T* const row_values = values + static_cast<long long>(r) * k;
-        int* const row_indices = indices + static_cast<long long>(r) * k;
-        float* const terms = reinterpret_cast<float*>(sh.hist);  // kRoom of them, its bins serve no longer
-        auto put = [&](unsigned long long own, int place) {
-          if (place < k) {
-            store1(row_values + place, logit_of(own));
-            row_indices[place] = column_of(own);
-            if (place == k - 1) sh.last = own;
-          } else {
-            terms[place] = ex2((logit_of(own) - low) * c);  // collected, but not among the k
-          }
-        };
-        if (collected <= kThreads / 2) {
-          // rank by counting, two threads a place; every place differs from every other
-          const int i = tid >> 1;
-          const unsigned long long own = i < collected ? sh.kept[i] : 0ull;
-          int place = 0;
-          if (i < collected) {
-#pragma unroll 8
-            for (int j = tid & 1; j < collected; j += 2) place += sh.kept[j] > own;
-          }
-          place += __shfl_xor_sync(0xffffffffu, place, 1);
-          if (i < collected && !(tid & 1)) put(own, place);
-        } else {
-          // sort all of them, descending, in 512 places: a warp's 64 by itself, wider steps over the block
-          for (int i = collected + tid; i < kRoom; i += kThreads) sh.kept[i] = 0ull;
-          sync_first(kThreads);
-          for (int size = 2; size <= kRoom; size *= 2)
-            for (int step = size / 2; step > 0; step /= 2) {
-              const int i = 2 * tid - (tid & (step - 1));  // the lower one of the pair
-              const unsigned long long x = sh.kept[i], y = sh.kept[i + step];
-              if ((x < y) == ((i & size) == 0)) {
-                sh.kept[i] = y;
-                sh.kept[i + step] = x;
-              }
-              if (step > 32 || (step == 1 && size >= 64))
-                sync_first(kThreads);
-              else
-                __syncwarp();
-            }
-          for (int i = tid; i < collected; i += kThreads) put(sh.kept[i], i);
-        }
-        // What is left: the sum relative to the bound with the collected ones that did not make it, added in the order of
-        // their places, not of their arrival.
-        sync_first(kThreads);
-        float more = 0.0f;
-        for (int i = k + lane; i < collected; i += 32) more += terms[i];
-        over += warp_sum(more);  // every warp for itself
-        float2 result = make_float2(low, sum + over);
-        if (by_digits || !(over < 1e30f)) result = rest_of(row, sh.last, inv_t, sh.red);
-        if (tid == 0) tail[r] = log_sum(result, inv_t);
-        sync_first(kThreads);  // before the next row collects
-      }
+      hand_over(n);
       if (tid == 0) mbar_arrive(done + 8 * (n & 1));
       __syncwarp();
       r = next;
     }
+    if (tid == 0) {
+      if (rank == 0 && n >= 2) late(wait_pair(selected, n - 2));
+      sh.work[n & 1].row = -1;
+    }
+    hand_over(n);
   }
   __syncwarp();
   if (cs > 1) cluster_sync_all();  // no block leaves while another one may still read from it or store to it
 }
 
+// A slice beside the fixed shared memory and 1 KB of the system's: two blocks an SM; one, with a cluster's maxima beside it.
+constexpr long long kMaximaBytes = 2 * 8 * kMaxima * 2;
+constexpr long long kHalfSm = 113 * 1024 - kShared, kWholeSm = 227 * 1024 - kShared - kMaximaBytes;
+
 template <typename T>
 int top(const void* z, long long rows, int V, long long ld, int k, float inv_t, void* values, int* indices, float* tail,
         int* status, cudaStream_t st) {
-  // Beside a slice, 7 KB of fixed shared memory and 1 KB of the system's: two blocks an SM, or one.
-  constexpr long long kHalfSm = 104 * 1024, kWholeSm = 208 * 1024;
-  const SlicePlan plan = slice_plan<T>(V, kWarps, kHalfSm, kWholeSm);
+  const SlicePlan plan = slice_plan<T>(V, kWarps, kHalfSm, kWholeSm, 2 * kMaxima * 2);
   if (plan.cs == 0) return 5;
-  const int smem = plan.slice * 16 + (plan.cs > 1 ? plan.cs * kMaxima * 2 : 0);
+  const int smem = plan.slice * 16 + (plan.cs > 1 ? 2 * plan.cs * kMaxima * 2 : 0);
   auto kern = top_logits_kernel<T>;
   static bool sized = false;  // the same answer whoever asks first
-  if (!sized && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 217 * 1024) != cudaSuccess) return 2;
+  if (!sized && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kWholeSm + kMaximaBytes) != cudaSuccess) return 2;
   sized = true;
-  return launch_clusters(kern, rows, plan.cs, kThreads + 32, smem, st, static_cast<const T*>(z), ld, V, k, inv_t, plan,
+  return launch_clusters(kern, rows, plan.cs, kThreads + 32 + kSelThreads, smem, st, static_cast<const T*>(z), ld, V, k, inv_t, plan,
                          static_cast<T*>(values), indices, tail, status);
 }
 
 }  // namespace
 
 // Widest row that a cluster holds.
-extern "C" long long pd_top_logits_max_columns(int z_fp32) { return 8ll * 208 * 1024 / (z_fp32 ? 4 : 2) - 16; }
+extern "C" long long pd_top_logits_max_columns(int z_fp32) { return 8 * kWholeSm / (z_fp32 ? 4 : 2) - 16; }
 
 // z [rows, V] in bf16 or fp32, rows ld elements apart; values, indices [rows, k], tail [rows].
 extern "C" int pd_top_logits(const void* z, long long rows, int V, long long ld, int k, float inv_t, void* values,
