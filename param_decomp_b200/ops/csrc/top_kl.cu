@@ -348,7 +348,6 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
     if (lane == 0) rows.request(blockIdx.x / cs, warp, smem, bar0 + 8 * warp, false);
     __syncwarp();
     late(wait_pair(ready, 0));
-    const uint32_t per_inverse = plan.per > 1 ? 0xFFFFFFFFu / plan.per + 1 : 0;  // x / per = x per_inverse >> 32, x per < 2^32
     int n = 0;
     for (int row = blockIdx.x / cs; row >= 0; ++n) {
       const Teacher& t = sh.teacher[n % 3];
@@ -363,7 +362,10 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
         const int at = rows.edge_place(tid, shift, col);
         if (at >= 0) store1(buf + at, t.edge[tid]);
       }
-      // Named columns leave the row: their logits go to every block of the cluster.
+      // Named columns leave the row: their logits go to every block of the cluster. A warp with slots waits for all parts
+      // of the slice, and as a whole: lanes that wait each for their own leave it split for the rest of the kernel.
+      if (32 * warp < call.K)
+        for (int w = 0; w < warps; ++w) late(short_wait<false>(bar0 + 8 * w, n & 1, &sh.abort_flag));
       int mine = -1;  // the column whose gradient this thread writes
       float mine_logit = 0.0f;
       if (tid < call.K && t.column[tid] >= 0 && t.column[tid] < call.V) {
@@ -371,8 +373,6 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
         if (at >= 0 && at < groups * kE) {
           mine = t.column[tid];
           if (g >= rows.whole_first(shift) && g < rows.whole_stop(shift)) {
-            const uint32_t x = g - rows.g0, holder = plan.per > 1 ? __umulhi(x, per_inverse) : x;  // the warp that holds it
-            late(short_wait<false>(bar0 + 8 * holder, n & 1, &sh.abort_flag));
             mine_logit = as_float(buf[at]);
             store1(buf + at, -INFINITY);
           } else {
@@ -424,8 +424,8 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
         }
       }
       if (lane == 0) sh.part[warp] = part;
+      if (warp == 0) late(wait_pair(ready, n + 1));
       if (tid == 0) {  // all warps go on together, or none does: what the barrier below shows them decides
-        late(wait_pair(ready, n + 1));
         sh.next = *static_cast<volatile int*>(&sh.abort_flag) ? -1 : sh.teacher[(n + 1) % 3].row;
       }
       sync_first(nt);

@@ -609,9 +609,11 @@ __global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_ker
         }
         hist[tid] = hist[tid + kThreads] = 0;
       }
-      if (tid == 0) {  // all warps go on together, or none does: what the barrier below shows them decides
+      if (warp == 0) {  // the whole of it: a lane that waits by itself leaves the warp split in two for the rest of the kernel
         late(wait_pair(ready, n + 1));
         if (rank == 0 && n >= 2) late(wait_pair(selected, n - 2));  // the list of two rows ago has been read
+      }
+      if (tid == 0) {  // all warps go on together, or none does: what the barrier below shows them decides
         if (cs == 1) sh.found[turn] = 0;
         sh.next[turn] = *static_cast<volatile int*>(&sh.abort_flag) ? -1 : sh.ahead[(n + 1) % 3].row;
       }
@@ -727,10 +729,8 @@ __global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_ker
       __syncwarp();
       r = next;
     }
-    if (tid == 0) {
-      if (rank == 0 && n >= 2) late(wait_pair(selected, n - 2));
-      sh.work[n & 1].row = -1;
-    }
+    if (warp == 0 && rank == 0 && n >= 2) late(wait_pair(selected, n - 2));
+    if (tid == 0) sh.work[n & 1].row = -1;
     hand_over(n);
   }
   __syncwarp();
