@@ -310,7 +310,7 @@ __device__ __forceinline__ float log_sum(float2 r, float inv_t) { return r.x > -
 // next one is read.
 struct Shared {
   RowQueue queue;
-  unsigned long long bars[kWarps + 10];
+  unsigned long long bars[kWarps + 11];
   unsigned long long kept[2][kRoom], last;
   alignas(16) int hist[2][kBins];
   float sums[2][kWarps];
@@ -334,20 +334,33 @@ struct Shared {
 constexpr int kShared = 14848;
 static_assert(sizeof(Shared) <= kShared);
 
-// The selection of the rows that a cluster has read: its first block's selecting warps, thread st of them.
+// The selection of the rows that a cluster has read: its first block's selecting warps, thread st of them; one warp of the
+// other blocks says when theirs have been. (An arrival at another block's barrier takes up to 2 us to get past what its
+// thread has seen stored: not the warps that read rows do it.)
 template <typename T>
 __device__ void select_rows(Shared& sh, const RowSlice<T>& rows, int cs, int k, float inv_t, T* values, int* indices,
-                            float* tail, int* status, uint32_t collected_bar, uint32_t selected_bar, int st) {
+                            float* tail, int* status, uint32_t collected_bar, uint32_t selected_bar, uint32_t gathered_bar, int rank,
+                            int st) {
   const int lane = st & 31, sw = st >> 5;
   const float c = inv_t * kLog2E;
   for (int n = 0;; ++n) {
     const int turn = n & 1;
     if (sw == 0) {  // all of them go on, or none does
-      const uint32_t bar = collected_bar + 8 * turn, phase = (n >> 1) & 1;
-      const bool in_time = cs > 1 ? short_wait<true>(bar, phase, &sh.abort_flag) : short_wait<false>(bar, phase, &sh.abort_flag);
+      const uint32_t phase = (n >> 1) & 1;
+      bool in_time = short_wait<false>(collected_bar + 8 * turn, phase, &sh.abort_flag);
+      const int next = in_time ? sh.work[turn].row : -1;
+      if (cs > 1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(gathered_bar + 8 * turn, 0));
+        __syncwarp();
+        if (rank == 0) in_time &= short_wait<true>(gathered_bar + 8 * turn, phase, &sh.abort_flag);
+      }
       if (!in_time && status != nullptr) atomicCAS(status, 0, kTimeoutProducer);
-      if (lane == 0) sh.row = in_time ? sh.work[turn].row : -1;
+      if (lane == 0) sh.row = in_time ? next : -1;
+      __syncwarp();
+      if (rank != 0 && next < 0) break;
     }
+    if (rank != 0) continue;
     sync_selectors();
     const int r = sh.row;
     if (r < 0) break;
@@ -511,9 +524,8 @@ __global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_ker
                  collected = ready + 48, met = ready + 64;
   if (tid == 0) {
     for (int i = 0; i < kWarps + 6; ++i) mbar_init(bar0 + 8 * i, 1);
-    mbar_init(collected, cs * kWarps);
-    mbar_init(collected + 8, cs * kWarps);
-    mbar_init(met, cs);
+    for (int i = 0; i < 2; ++i) mbar_init(collected + 8 * i, kWarps);
+    for (int i = 0; i < 3; ++i) mbar_init(met + 8 * i, cs);  // and `gathered`
     sh.queue.init();
     sh.abort_flag = 0;
     sh.top[0] = sh.top[1] = 0;
@@ -527,7 +539,8 @@ __global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_ker
   // The n-th completion of a pair of barriers that take turns.
   auto wait_pair = [&](uint32_t pair, int n) { return short_wait<false>(pair + 8 * (n & 1), (n >> 1) & 1, &sh.abort_flag); };
   if (warp > kWarps) {
-    if (rank == 0) select_rows(sh, rows, cs, k, inv_t, values, indices, tail, status, collected, selected, tid - kThreads - 32);
+    if (rank == 0 || warp == kWarps + 1)
+      select_rows(sh, rows, cs, k, inv_t, values, indices, tail, status, collected, selected, met + 8, rank, tid - kThreads - 32);
   } else if (warp == kWarps) {  // rows to come, two ahead
     bool more = true;
     if (rank == 0 && lane == 0) sh.queue.ask();
@@ -561,14 +574,9 @@ __global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_ker
     if (lane == 0) rows.request(blockIdx.x / cs, warp, smem, bar0 + 8 * warp, false);
     __syncwarp();
     late(wait_pair(ready, 0));
-    auto hand_over = [&](int n) {  // the warp, to the selecting warps of the first block
+    auto hand_over = [&](int n) {  // the warp, to the selecting warps
       __syncwarp();
-      if (lane == 0) {
-        if (cs > 1)
-          mbar_arrive_cluster(mapa_shared(collected + 8 * (n & 1), 0));
-        else
-          mbar_arrive(collected + 8 * (n & 1));
-      }
+      if (lane == 0) mbar_arrive(collected + 8 * (n & 1));
       __syncwarp();
     };
     int n = 0;
@@ -592,7 +600,7 @@ __global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_ker
       if (!by_digits) {
         GroupMax<T> m0, m1;
         int g = begin;
-#pragma unroll 2
+#pragma unroll 4
         for (; g + 32 < stop; g += 64) {
           m0.add(*reinterpret_cast<const uint4*>(smem + 16 * g));
           m1.add(*reinterpret_cast<const uint4*>(smem + 16 * (g + 32)));
