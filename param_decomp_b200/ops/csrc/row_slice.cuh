@@ -153,30 +153,31 @@ inline SlicePlan slice_plan(long long V, int warps, long long half, long long wh
 // Rows are dealt by the launch itself: one cluster a row, of which the first ones start, and a running cluster that wants
 // more work cancels the start of a waiting one and takes its row (`clusterlaunchcontrol`). SMs differ by up to 40% in the
 // bandwidth they get under full load, so equal shares would leave the fast ones waiting.
-// One warp a block calls this; block 0 of the cluster asks, and tells the others.
+// One warp a block calls this; block 0 of the cluster asks, and tells the others, which may be up to three rows late: four
+// barriers take turns, since one that has completed twice reads like one that has not.
 struct RowQueue {
   uint4 answer;  // 16-byte aligned
-  unsigned long long bars[2];  // the answer has come; the next row is known here
+  unsigned long long come, told[4];  // the answer has come; the next row is known here
   int next[4];
 
   // One thread, before the block's first barrier.
   __device__ __forceinline__ void init() {
-    mbar_init(smem_u32(bars), 1);
-    mbar_init(smem_u32(bars + 1), 1);
+    mbar_init(smem_u32(&come), 1);
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(told + i), 1);
   }
   // One thread of block 0: ask for the n-th row (n = 1, 2, ..), not after an answer that there is none.
   __device__ __forceinline__ void ask() {
     fence_proxy_async_smem();
-    mbar_expect_tx(smem_u32(bars), 16);
+    mbar_expect_tx(smem_u32(&come), 16);
     asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
                      smem_u32(&answer)),
-                 "r"(smem_u32(bars))
+                 "r"(smem_u32(&come))
                  : "memory");
   }
   // The warp: the n-th row, or -1. Block 0 must have asked for it.
   __device__ __forceinline__ int take(int n, int rank, int cs, int lane, volatile int* abort_flag, bool& in_time) {
     if (rank == 0) {
-      in_time &= short_wait<false>(smem_u32(bars), (n - 1) & 1, abort_flag);
+      in_time &= short_wait<false>(smem_u32(&come), (n - 1) & 1, abort_flag);
       uint32_t got, x;
       asm volatile(
           "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t.reg .b64 lo, hi;\n\t"
@@ -195,11 +196,11 @@ struct RowQueue {
       if (lane < cs) {
         const uint32_t to = mapa_shared(smem_u32(next + (n & 3)), lane);
         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(row) : "memory");
-        mbar_arrive_cluster(mapa_shared(smem_u32(bars + 1), lane));
+        mbar_arrive_cluster(mapa_shared(smem_u32(told + ((n - 1) & 3)), lane));
       }
       __syncwarp();
     }
-    in_time &= short_wait<true>(smem_u32(bars + 1), (n - 1) & 1, abort_flag);
+    in_time &= short_wait<true>(smem_u32(told + ((n - 1) & 3)), ((n - 1) >> 2) & 1, abort_flag);
     return in_time ? *static_cast<volatile int*>(next + (n & 3)) : -1;
   }
 };

@@ -35,6 +35,8 @@ struct Call {
   void* dz;          // [rows, V], rows ldo apart, each at z's row's address modulo 16; or null
   long long ldo;
   const float* scale;  // [rows]: the gradient's factor; or null
+  float4* sums;        // [rows]: a row's sums, for a gradient that is asked for later; or null
+  const float4* known; // [rows]: the sums of an earlier call with the same row and teacher; or null
   int* status;
   int* refused;
 };
@@ -252,7 +254,7 @@ __device__ float loss_of(const Call& call, long long row, const Teacher& t, cons
 // one that may change any part of it.
 struct Shared {
   RowQueue queue;
-  unsigned long long bars[kWarps + 7];
+  unsigned long long bars[kWarps + 8];
   Teacher teacher[3];
   float named[3][kMaxK];  // student's logits at the columns, in the slots that speak for them
   Row red[kWarps], xch[3][8], sums[2];
@@ -277,7 +279,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
   if (tid == 0) {
     for (int i = 0; i < warps; ++i) mbar_init(bar0 + 8 * i, 1);
     for (int i = 0; i < 6; ++i) mbar_init(ready + 8 * i, 1);
-    mbar_init(met, cs);
+    for (int i = 0; i < 2; ++i) mbar_init(met + 8 * i, cs);
     sh.rows = -1;
     sh.queue.init();
     sh.abort_flag = 0;
@@ -291,6 +293,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
   // The n-th completion of a pair of barriers that take turns: one that is waited for late is not mistaken for the next.
   auto wait_pair = [&](uint32_t pair, int n) { return short_wait<false>(pair + 8 * (n & 1), (n >> 1) & 1, &sh.abort_flag); };
   const bool losses = rank == 0 && call.loss != nullptr;
+  const bool loose = cs > 1 && call.known != nullptr;  // nothing else keeps the cluster's blocks together
   if (warp == warps) {  // the teacher's side, up to two rows ahead
     auto teach = [&](int row, int n) {
       Teacher& t = sh.teacher[n % 3];
@@ -327,15 +330,21 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
     for (int n = 0; sh.teacher[n % 3].row >= 0; ++n) {
       late(wait_pair(summed, n));  // the others are done with the row before,
       if (losses && n > 0) late(wait_pair(lost, n - 1));  // and so is the warp below
+      if (loose && rank == 0 && n > 0) late(wait_pair(met, n - 1));  // all blocks have begun the row before: none is left far behind
       teach(ahead, n + 2);
       ahead = next(n + 3);
     }
   } else if (warp == warps + 1) {  // losses, a row behind
     // What a loss reads is written again three rows on, by whichever block, and not before the teacher of that row is
     // there, which waits for this warp.
-    for (int n = 0; losses; ++n) {
+    for (int n = 0; losses || loose; ++n) {
       late(wait_pair(summed, n));
       if (n == *static_cast<volatile int*>(&sh.rows) || *static_cast<volatile int*>(&sh.abort_flag)) break;
+      if (loose) {
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(met + 8 * (n & 1), 0));
+        __syncwarp();
+        continue;
+      }
       const Teacher& t = sh.teacher[n % 3];
       const float loss = loss_of(call, t.row, t, sh.sums[n & 1], sh.named[n % 3], c, lane);
       if (lane == 0) {
@@ -362,117 +371,136 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
         const int at = rows.edge_place(tid, shift, col);
         if (at >= 0) store1(buf + at, t.edge[tid]);
       }
-      // Named columns leave the row: their logits go to every block of the cluster. A warp with slots waits for all parts
-      // of the slice, and as a whole: lanes that wait each for their own leave it split for the rest of the kernel.
-      if (32 * warp < call.K)
-        for (int w = 0; w < warps; ++w) late(short_wait<false>(bar0 + 8 * w, n & 1, &sh.abort_flag));
-      int mine = -1;  // the column whose gradient this thread writes
+      int mine = -1, next;  // the column whose gradient this thread writes; the row behind this one
       float mine_logit = 0.0f;
-      if (tid < call.K && t.column[tid] >= 0 && t.column[tid] < call.V) {
-        const int place = shift + t.column[tid], g = place / kE, at = place - rows.g0 * kE;
-        if (at >= 0 && at < groups * kE) {
-          mine = t.column[tid];
-          if (g >= rows.whole_first(shift) && g < rows.whole_stop(shift)) {
-            mine_logit = as_float(buf[at]);
-            store1(buf + at, -INFINITY);
-          } else {
-            mine_logit = as_float(rows.row(row)[mine]);  // at a ragged end, which is already without it
-          }
-          const uint32_t local = smem_u32(zk + tid);
-          if (cs > 1)
-            for (int b = 0; b < cs; ++b) store_cluster_f32(mapa_shared(local, b), mine_logit);
-          else
-            zk[tid] = mine_logit;
-        }
-      }
-      fence_proxy_async_smem();  // before bulk copies of the next row write where this row's ends and marks are
-      sync_first(nt);
-      // The slice's sums relative to one of its own logits: they serve as they are unless another one is larger by 2^100.
-      GroupMax<T> gm;
-      if (groups > 0) gm.add(*reinterpret_cast<const uint4*>(smem));
-      if (groups > 1) gm.add(*reinterpret_cast<const uint4*>(smem + 16));
-      const float ref = gm.value();
+      Row sums;
       const f32x2 c2 = pk2(c, c);
-      auto add_up = [&](auto exponent) {  // of a pair of logits
-        f32x2 s0 = 0ull, s1 = 0ull;
-#pragma unroll 4
-        for (int g = begin; g < stop; g += 32) {
-          f32x2 v[kP];
-          pairs_of<T>(*reinterpret_cast<const uint4*>(smem + 16 * g), v);
-#pragma unroll
-          for (int j = 0; j < kP; ++j) {
-            const float2 x = unpack2(exponent(v[j]));
-            const f32x2 e = pk2(ex2(x.x), ex2(x.y));
-            if (j & 1)
-              s1 = add2(s1, e);
-            else
-              s0 = add2(s0, e);
+      if (call.known != nullptr) {  // the row's sums are there: a gradient is all that is left to do
+        const float4 q = call.known[row];
+        sums = Row{{q.x, q.y}, {q.z, q.w}};
+        if (tid < call.K && t.column[tid] >= 0) {
+          const int at = shift + t.column[tid] - rows.g0 * kE;
+          if (at >= 0 && at < groups * kE) {
+            mine = t.column[tid];
+            mine_logit = as_float(rows.row(row)[mine]);
           }
         }
-        const float2 a = unpack2(add2(s0, s1));
-        return a.x + a.y;
-      };
-      float2 part = make_float2(INFINITY, 0.0f);
-      if (moderate(ref, c)) {
-        const float k = -power_of(ref, c);
-        const f32x2 k2 = pk2(k, k);
-        part = make_float2(add_up([&](f32x2 v) { return fma2(v, c2, k2); }), mine >= 0 ? term(mine_logit, ref, c) : 0.0f);
+        if (warp == 0) late(wait_pair(ready, n + 1));
+        if (tid == 0) sh.next = *static_cast<volatile int*>(&sh.abort_flag) ? -1 : sh.teacher[(n + 1) % 3].row;
+        fence_proxy_async_smem();  // before bulk copies of the next row write where this row's ends are
+        sync_first(nt);
+        next = sh.next;
+      } else {
+        // Named columns leave the row: their logits go to every block of the cluster. A warp with slots waits for all parts
+        // of the slice, and as a whole: lanes that wait each for their own leave it split for the rest of the kernel.
+        if (32 * warp < call.K)
+          for (int w = 0; w < warps; ++w) late(short_wait<false>(bar0 + 8 * w, n & 1, &sh.abort_flag));
+        if (tid < call.K && t.column[tid] >= 0 && t.column[tid] < call.V) {
+          const int place = shift + t.column[tid], g = place / kE, at = place - rows.g0 * kE;
+          if (at >= 0 && at < groups * kE) {
+            mine = t.column[tid];
+            if (g >= rows.whole_first(shift) && g < rows.whole_stop(shift)) {
+              mine_logit = as_float(buf[at]);
+              store1(buf + at, -INFINITY);
+            } else {
+              mine_logit = as_float(rows.row(row)[mine]);  // at a ragged end, which is already without it
+            }
+            const uint32_t local = smem_u32(zk + tid);
+            if (cs > 1)
+              for (int b = 0; b < cs; ++b) store_cluster_f32(mapa_shared(local, b), mine_logit);
+            else
+              zk[tid] = mine_logit;
+          }
+        }
+        fence_proxy_async_smem();  // before bulk copies of the next row write where this row's ends and marks are
+        sync_first(nt);
+        // The slice's sums relative to one of its own logits: they serve as they are unless another one is larger by 2^100.
+        GroupMax<T> gm;
+        if (groups > 0) gm.add(*reinterpret_cast<const uint4*>(smem));
+        if (groups > 1) gm.add(*reinterpret_cast<const uint4*>(smem + 16));
+        const float ref = gm.value();
+        auto add_up = [&](auto exponent) {  // of a pair of logits
+          f32x2 s0 = 0ull, s1 = 0ull;
+#pragma unroll 4
+          for (int g = begin; g < stop; g += 32) {
+            f32x2 v[kP];
+            pairs_of<T>(*reinterpret_cast<const uint4*>(smem + 16 * g), v);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
+            for (int j = 0; j < kP; ++j) {
+              const float2 x = unpack2(exponent(v[j]));
+              const f32x2 e = pk2(ex2(x.x), ex2(x.y));
+              if (j & 1)
+                s1 = add2(s1, e);
+              else
+                s0 = add2(s0, e);
+            }
+          }
+          const float2 a = unpack2(add2(s0, s1));
+          return a.x + a.y;
+        };
+        float2 part = make_float2(INFINITY, 0.0f);
+        if (moderate(ref, c)) {
+          const float k = -power_of(ref, c);
+          const f32x2 k2 = pk2(k, k);
+          part = make_float2(add_up([&](f32x2 v) { return fma2(v, c2, k2); }), mine >= 0 ? term(mine_logit, ref, c) : 0.0f);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            part.x += __shfl_xor_sync(0xffffffffu, part.x, o);
+            part.y += __shfl_xor_sync(0xffffffffu, part.y, o);
+          }
+        }
+        if (lane == 0) sh.part[warp] = part;
+        if (warp == 0) late(wait_pair(ready, n + 1));
+        if (tid == 0) {  // all warps go on together, or none does: what the barrier below shows them decides
+          sh.next = *static_cast<volatile int*>(&sh.abort_flag) ? -1 : sh.teacher[(n + 1) % 3].row;
+        }
+        sync_first(nt);
+        next = sh.next;
+        part = sh.part[lane & 7];
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
           part.x += __shfl_xor_sync(0xffffffffu, part.x, o);
           part.y += __shfl_xor_sync(0xffffffffu, part.y, o);
         }
-      }
-      if (lane == 0) sh.part[warp] = part;
-      if (warp == 0) late(wait_pair(ready, n + 1));
-      if (tid == 0) {  // all warps go on together, or none does: what the barrier below shows them decides
-        sh.next = *static_cast<volatile int*>(&sh.abort_flag) ? -1 : sh.teacher[(n + 1) % 3].row;
-      }
-      sync_first(nt);
-      const int next = sh.next;
-      part = sh.part[lane & 7];
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) {
-        part.x += __shfl_xor_sync(0xffffffffu, part.x, o);
-        part.y += __shfl_xor_sync(0xffffffffu, part.y, o);
-      }
-      Row sums{{ref, part.x}, {ref, part.y}};
-      if (!(part.x < 1e30f && part.y < 1e30f)) {  // the same in every thread: sums relative to true maxima
-        GroupMax<T> all;
-        for (int g = begin; g < stop; g += 32) all.add(*reinterpret_cast<const uint4*>(smem + 16 * g));
-        const float own = all.value();
-        sums = Row{{own, 0.0f}, {-INFINITY, 0.0f}};
-        if (mine >= 0 && mine_logit > -INFINITY) sums.top = MaxSum{mine_logit, term(mine_logit, mine_logit, c)};
-        if (moderate(own, c)) {
-          const float k = -power_of(own, c);
-          const f32x2 k2 = pk2(k, k);
-          sums.rest.s = add_up([&](f32x2 v) { return fma2(v, c2, k2); });
-        } else if (own > -INFINITY) {
-          const f32x2 neg = pk2(-own, -own);
-          sums.rest.s = add_up([&](f32x2 v) { return mul2(add2(v, neg), c2); });
+        sums = Row{{ref, part.x}, {ref, part.y}};
+        if (!(part.x < 1e30f && part.y < 1e30f)) {  // the same in every thread: sums relative to true maxima
+          GroupMax<T> all;
+          for (int g = begin; g < stop; g += 32) all.add(*reinterpret_cast<const uint4*>(smem + 16 * g));
+          const float own = all.value();
+          sums = Row{{own, 0.0f}, {-INFINITY, 0.0f}};
+          if (mine >= 0 && mine_logit > -INFINITY) sums.top = MaxSum{mine_logit, term(mine_logit, mine_logit, c)};
+          if (moderate(own, c)) {
+            const float k = -power_of(own, c);
+            const f32x2 k2 = pk2(k, k);
+            sums.rest.s = add_up([&](f32x2 v) { return fma2(v, c2, k2); });
+          } else if (own > -INFINITY) {
+            const f32x2 neg = pk2(-own, -own);
+            sums.rest.s = add_up([&](f32x2 v) { return mul2(add2(v, neg), c2); });
+          }
+          sums = merge_lanes(sums, 32, c);
+          if (lane == 0) sh.red[warp] = sums;
+          sync_first(nt);
+          sums = merge_lanes(sh.red[lane & 7], 8, c);
         }
-        sums = merge_lanes(sums, 32, c);
-        if (lane == 0) sh.red[warp] = sums;
-        sync_first(nt);
-        sums = merge_lanes(sh.red[lane & 7], 8, c);
-      }
-      if (cs > 1) {
-        if (warp == 0 && lane < cs) {
-          const uint32_t to = mapa_shared(smem_u32(&sh.xch[n % 3][rank]), lane);
-          store_cluster_f32(to, sums.rest.m);
-          store_cluster_f32(to + 4, sums.rest.s);
-          store_cluster_f32(to + 8, sums.top.m);
-          store_cluster_f32(to + 12, sums.top.s);
-          mbar_arrive_cluster(mapa_shared(met, lane));  // with it, the named logits that were stored before the barriers
+        if (cs > 1) {
+          if (warp == 0 && lane < cs) {
+            const uint32_t to = mapa_shared(smem_u32(&sh.xch[n % 3][rank]), lane);
+            store_cluster_f32(to, sums.rest.m);
+            store_cluster_f32(to + 4, sums.rest.s);
+            store_cluster_f32(to + 8, sums.top.m);
+            store_cluster_f32(to + 12, sums.top.s);
+            mbar_arrive_cluster(mapa_shared(met, lane));  // with it, the named logits that were stored before the barriers
+          }
+          __syncwarp();
+          late(short_wait<true>(met, n & 1, &sh.abort_flag));
+          const Row none{{-INFINITY, 0.0f}, {-INFINITY, 0.0f}};
+          sums = (lane & 7) < cs ? sh.xch[n % 3][lane & 7] : none;
+          sums = merge_lanes(sums, 8, c);
         }
-        __syncwarp();
-        late(short_wait<true>(met, n & 1, &sh.abort_flag));
-        const Row none{{-INFINITY, 0.0f}, {-INFINITY, 0.0f}};
-        sums = (lane & 7) < cs ? sh.xch[n % 3][lane & 7] : none;
-        sums = merge_lanes(sums, 8, c);
       }
       if (tid == 0) {
         sh.sums[n & 1] = sums;
+        if (call.sums != nullptr && rank == 0) call.sums[t.row] = make_float4(sums.rest.m, sums.rest.s, sums.top.m, sums.top.s);
         mbar_arrive(summed + 8 * (n & 1));
       }
       __syncwarp();
@@ -558,7 +586,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
         ask_for_next();
         sync_first(nt);  // the row's stores are in order before those of the named columns
         if (mine >= 0) {
-          const float q = term(zk[tid], all.m, c) / all.s;
+          const float q = term(mine_logit, all.m, c) / all.s;
           store1(out + mine, live ? (q - t.of_column[tid]) * up : 0.0f);
         }
       } else {
@@ -597,9 +625,12 @@ extern "C" long long pd_top_kl_max_columns(int z_fp32) { return 8 * kWholeSm / (
 
 extern "C" int pd_top_kl(const void* z, long long rows, int V, long long ld, const void* indices, int wide,
                          const void* values, int values_fp32, int K, const float* tail, double inv_t, float* loss, void* dz,
-                         long long ldo, const float* scale, int z_fp32, int* status, int* refused, void* stream) {
+                         long long ldo, const float* scale, float* sums, const float* known, int z_fp32, int* status,
+                         int* refused, void* stream) {
   if (rows <= 0 || rows >= (1ll << 28) || V <= 0 || K <= 0 || K > kMaxK || !(inv_t > 0.0)) return 5;
-  const Call call{z, rows, ld, V, indices, wide, values, values_fp32, K, tail, inv_t, loss, dz, ldo, scale, status, refused};
+  if (known != nullptr && (dz == nullptr || loss != nullptr)) return 5;
+  const Call call{z, rows, ld, V, indices, wide, values, values_fp32, K, tail, inv_t, loss, dz, ldo, scale,
+                  reinterpret_cast<float4*>(sums), reinterpret_cast<const float4*>(known), status, refused};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return z_fp32 ? launch<float>(call, st) : launch<__nv_bfloat16>(call, st);
 }

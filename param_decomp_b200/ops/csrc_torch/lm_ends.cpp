@@ -27,7 +27,7 @@ int pd_embedding_grad(const int* ids, const void* dy, void* dE, long long n, lon
                       int table_fp32, int* ints, float* partial, void* stream);
 int pd_top_kl(const void* z, long long rows, int V, long long ld, const void* indices, int wide, const void* values,
               int values_fp32, int K, const float* tail, double inv_t, float* loss, void* dz, long long ldo,
-              const float* scale, int z_fp32, int* status, int* refused, void* stream);
+              const float* scale, float* sums, const float* known, int z_fp32, int* status, int* refused, void* stream);
 }
 
 namespace {
@@ -233,21 +233,25 @@ struct Teacher {
   double temperature;
   int64_t status, refused;
 };
-void run_top_kl(const Tensor& z, const Teacher& t, const Tensor& loss, const Tensor& dz, const Tensor& scale) {
+void run_top_kl(const Tensor& z, const Teacher& t, const Tensor& loss, const Tensor& dz, const Tensor& scale,
+                const Tensor& sums, const Tensor& known) {
   if (z.size(0) == 0) return;
   check(pd_top_kl(z.const_data_ptr(), z.size(0), static_cast<int>(z.size(1)), pitch_of(z), t.indices.const_data_ptr(),
                   t.indices.scalar_type() == at::kLong, t.values.const_data_ptr(), fp32(t.values),
                   static_cast<int>(t.indices.size(1)), static_cast<const float*>(at_or_null(t.tail)), 1.0 / t.temperature,
                   static_cast<float*>(data_or_null(loss)), data_or_null(dz), dz.defined() ? dz.stride(0) : 0,
-                  static_cast<const float*>(at_or_null(scale)), fp32(z), reinterpret_cast<int*>(t.status),
+                  static_cast<const float*>(at_or_null(scale)),
+                  static_cast<float*>(data_or_null(sums)), static_cast<const float*>(at_or_null(known)), fp32(z),
+                  reinterpret_cast<int*>(t.status),
                   reinterpret_cast<int*>(t.refused), current_stream()),
         "top_kl");
 }
 
-// The backward runs the kernel again with the upstream gradient of each row: 2 reads and a write of the logits for both
-// passes, against a read and two writes had the forward kept an unscaled gradient, and nothing is held between.
+// The backward reads the logits again, with the rows' sums that the forward kept: 2 reads and a write of the logits for
+// both passes, against a read and two writes had the forward kept an unscaled gradient.
 struct TopKLBackward : Node {
   SavedVariable z, indices, values, tail;
+  Tensor sums;
   double temperature;
   int64_t status, refused;
 
@@ -255,6 +259,7 @@ struct TopKLBackward : Node {
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     for (SavedVariable* s : {&z, &indices, &values, &tail}) s->reset_data();
+    sums.reset();
   }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -265,7 +270,7 @@ struct TopKLBackward : Node {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       dz = grad_like(zs, pitch_of(zs));
-      run_top_kl(zs, t, Tensor(), dz, grads[0].contiguous());
+      run_top_kl(zs, t, Tensor(), dz, grads[0].contiguous(), Tensor(), sums);
     }
     return once({dz}, *this, "top_kl");
   }
@@ -281,7 +286,8 @@ Tensor top_kl(const Tensor& z, const Tensor& indices, const Tensor& values, cons
   {
     at::AutoDispatchBelowADInplaceOrView below;
     loss = floats({z.size(0)}, z);
-    run_top_kl(z, t, loss, Tensor(), Tensor());
+    if (node) node->sums = floats({z.size(0), 4}, z);
+    run_top_kl(z, t, loss, Tensor(), Tensor(), node ? node->sums : Tensor(), Tensor());
   }
   if (node) {
     node->z = SavedVariable(z, false);
@@ -301,7 +307,8 @@ std::tuple<Tensor, Tensor> top_kl_rows(const Tensor& z, const Tensor& indices, c
                                        int64_t refused) {
   at::AutoDispatchBelowADInplaceOrView below;
   const Tensor loss = floats({z.size(0)}, z), dz = want_grad ? grad_like(z, pitch_of(z)) : Tensor();
-  run_top_kl(z, Teacher{indices, values, given(tail), temperature, status, refused}, loss, dz, Tensor());
+  run_top_kl(z, Teacher{indices, values, given(tail), temperature, status, refused}, loss, dz, Tensor(),
+             Tensor(), Tensor());
   return {loss, dz};
 }
 

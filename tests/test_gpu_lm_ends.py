@@ -425,6 +425,24 @@ def test_top_kl_and_its_gradient(nv, n, V, K, kind):
     _done(nv)
 
 
+@pytest.mark.parametrize("kind,n,V,K", [(bf, 2000, 50277, 3), (bf, 900, 120001, 40), (f32, 700, 60000, 200), (f32, 700, 151936, 1)])
+def test_top_kl_backward_from_kept_sums(nv, kind, n, V, K):
+    """Many rows a cluster of 1 to 8 blocks: the gradient that a backward forms from the sums that the forward kept is, bit for
+    bit, that of one pass, and the losses too."""
+    from param_decomp_b200.ops.top_logits import top_kl, top_kl_rows
+
+    g = torch.Generator(device="cuda").manual_seed(V)
+    z = torch.randn(n, V, generator=g, device="cuda").to(kind)
+    idx = torch.randint(0, V, (n, K), generator=g, device="cuda")
+    t, tail = torch.randn(n, K, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda") + 8.0
+    loss, dz = top_kl_rows(z, idx, t, tail, 2.0)
+    leaf = z.requires_grad_(True)
+    auto = top_kl(leaf, idx, t, tail, 2.0)
+    (grad,) = torch.autograd.grad(auto, (leaf,), torch.ones(n, device="cuda"))
+    _done(nv)
+    assert torch.equal(auto.detach(), loss) and torch.equal(grad, dz)
+
+
 @pytest.mark.parametrize("kind,V", [(bf, 470001), (bf, 884720), (f32, 225001), (f32, 442352)])
 def test_top_kl_of_the_longest_rows(nv, kind, V):
     g = _gen(V)
