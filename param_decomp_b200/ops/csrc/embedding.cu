@@ -26,6 +26,7 @@ constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxSpan = 1280;  // ids a block: 32 counts of 4 bytes each in shared memory
 constexpr int kNoted = 128;     // tokens a warp notes; where there are more, it reads its part again
 constexpr int kRunThreads = 384;
+constexpr int kMaxPer = 512;  // ids of a block that writes zeros
 
 __device__ __forceinline__ long long token_at(const void* tokens, int wide, long long i) {
   return wide ? static_cast<const long long*>(tokens)[i] : static_cast<const int*>(tokens)[i];
@@ -57,7 +58,8 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const void* __res
       atomicCAS(status, 0, kBadToken);
       *static_cast<volatile int*>(refused) = 1;
     }
-    for (int c = kVec ? 8 * lane : lane; c < d; c += kVec ? 256 : 32) {
+    constexpr int kColumns = kVec ? 1 : 4;  // of a lane, 32 apart, where it loads one at a time
+    for (int c = kVec ? 8 * lane : lane; c < d; c += kVec ? 256 : 32 * kColumns) {
       if (kVec) {
         Raw8<P> raw[kRowsAhead];
 #pragma unroll
@@ -78,12 +80,17 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const void* __res
           store8(y + (r0 + k) * d + c, v);
         }
       } else {
-        float v[kRowsAhead];
-#pragma unroll
-        for (int k = 0; k < kRowsAhead; ++k) v[k] = src[k] != nullptr ? as_float(src[k][c]) : 0.0f;
+        float v[kRowsAhead][kColumns];
 #pragma unroll
         for (int k = 0; k < kRowsAhead; ++k)
-          if (r0 + k < n) store1(y + (r0 + k) * d + c, v[k] * scale);
+#pragma unroll
+          for (int j = 0; j < kColumns; ++j)
+            v[k][j] = src[k] != nullptr && c + 32 * j < d ? as_float(src[k][c + 32 * j]) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < kRowsAhead; ++k)
+#pragma unroll
+          for (int j = 0; j < kColumns; ++j)
+            if (r0 + k < n && c + 32 * j < d) store1(y + (r0 + k) * d + c + 32 * j, v[k][j] * scale);
       }
     }
   }
@@ -99,16 +106,38 @@ struct Runs {        // what the first kernel tells the second
   uint8_t* empty;    // [V] the id has no token
 };
 
-// Zeros in a row, by one warp: whole 16-byte pieces, the ends element by element.
+// A block: zeros in those rows [from, to) of the table's gradient that have no token. All of them as one stretch of 16-byte
+// pieces, whatever the rows' own alignment: rows of 515 fp32 begin at any of them.
 template <typename P>
-__device__ __forceinline__ void write_zeros(P* to, int count, int lane) {
-  const int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(to) & 15)) % 16 / sizeof(P));
-  const int first = min(head, count), pieces = (count - first) * static_cast<int>(sizeof(P)) / 16;
-  const int rest = first + pieces * 16 / static_cast<int>(sizeof(P));
-  if (lane < first) store1(to + lane, 0.0f);
-  if (rest + lane < count) store1(to + rest + lane, 0.0f);  // fewer than 16 bytes
-  uint4* p = reinterpret_cast<uint4*>(to + first);
-  for (int i = lane; i < pieces; i += 32) p[i] = make_uint4(0u, 0u, 0u, 0u);
+__device__ void write_zeros(P* __restrict__ dE, int from, int to, int d, const uint8_t* __restrict__ is_empty,
+                            uint8_t* empty) {
+  constexpr int kE = 16 / sizeof(P);
+  for (int i = threadIdx.x; i < to - from; i += kRunThreads) empty[i] = is_empty[from + i];
+  __syncthreads();
+  P* const base = dE + static_cast<long long>(from) * d;
+  const long long total = static_cast<long long>(to - from) * d;
+  const long long head = min(total, static_cast<long long>((16 - (reinterpret_cast<uintptr_t>(base) & 15)) % 16 / sizeof(P)));
+  const long long pieces = (total - head) / kE, tail = head + pieces * kE;
+  const long long edge = threadIdx.x < kE ? threadIdx.x : tail + threadIdx.x - kE;
+  if (threadIdx.x < kE ? edge < head : edge < total && threadIdx.x < 2 * kE)
+    if (empty[edge / d]) store1(base + edge, 0.0f);
+  long long e = head + static_cast<long long>(kE) * threadIdx.x;
+  constexpr int kStep = kE * kRunThreads;
+  int row = static_cast<int>(e / d), rem = static_cast<int>(e % d);
+  for (long long p = threadIdx.x; p < pieces; p += kRunThreads, e += kStep) {
+    const bool inside = rem + kE <= d;
+    if (inside || d >= kE ? empty[row] && (inside || empty[row + 1]) : false) {
+      *reinterpret_cast<uint4*>(base + e) = make_uint4(0u, 0u, 0u, 0u);
+    } else if (!inside) {
+      for (int j = 0, r = row, m = rem; j < kE; ++j) {
+        if (empty[r]) store1(base + e + j, 0.0f);
+        if (++m == d) m = 0, ++r;
+      }
+    }
+    row += kStep / d;
+    rem += kStep % d;
+    if (rem >= d) rem -= d, ++row;
+  }
 }
 
 // One warp: scale times rows of dy, each in one piece of 256 columns; lane u names the u-th row, its place in the table and
@@ -419,6 +448,7 @@ __global__ void __launch_bounds__(kRunThreads, 4) embedding_runs_kernel(const T*
                                                                      float* __restrict__ partial, int slabs, int per) {
   __shared__ int where[kSlab], place[kSlab], last;
   __shared__ float red[kRunThreads * 8];
+  __shared__ uint8_t empty[kMaxPer + 1];
   wait_for_previous();
   // Blocks with a slab and blocks with `per` ids, whose rows without a token they write, take turns while there are both:
   // the former wait for loads, the latter do not.
@@ -426,9 +456,7 @@ __global__ void __launch_bounds__(kRunThreads, 4) embedding_runs_kernel(const T*
   const bool zeros = b < 2 * pairs ? b & 1 : slabs <= zero_blocks;
   const int mine = b < 2 * pairs ? b / 2 : b - pairs;
   if (zeros) {
-    const int from = mine * per, to = min(V, from + per);
-    for (int i = from + threadIdx.x / 32; i < to; i += kRunThreads / 32)
-      if (runs.empty[i]) write_zeros(dE + static_cast<long long>(i) * d, d, threadIdx.x & 31);
+    write_zeros(dE, mine * per, min(V, (mine + 1) * per), d, runs.empty, empty);
     return;
   }
   const int slab = mine, begin = slab * kSlab, stop = min(n, begin + kSlab);
@@ -516,7 +544,9 @@ int grad(const int* ids, const void* dy, void* dE, int n, int V, int d, float sc
   kern<<<blocks, kSortThreads, smem, st>>>(ids, static_cast<const T*>(dy), static_cast<P*>(dE), n, V, d, scale, span, ahead,
                                            runs);
   if (cudaGetLastError() != cudaSuccess) return 1;
-  const int per = std::max(16, (V + 148 * 4 - 1) / (148 * 4)), zero_blocks = (V + per - 1) / per;
+  // Blocks that write zeros take about 32 KB each, so that those which run at one time write one stretch of the table: with
+  // 592 blocks for all of it, a stretch each, 151,936 rows of 515 fp32 took 90 us, so 69.
+  const int per = static_cast<int>(std::clamp<long long>(32768 / (static_cast<long long>(d) * sizeof(P)), 16, kMaxPer)), zero_blocks = (V + per - 1) / per;
   return launch_after(embedding_runs_kernel<T, P, kVec>, dim3(slabs + zero_blocks), dim3(kRunThreads), 0, st,
                       static_cast<const T*>(dy), static_cast<P*>(dE), n, V, d, scale, runs, partial, slabs, per) == cudaSuccess
              ? 0

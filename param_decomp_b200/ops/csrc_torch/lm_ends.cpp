@@ -25,6 +25,8 @@ long long pd_embedding_grad_ints(long long n, long long V);
 long long pd_embedding_grad_floats(long long n, int d);
 int pd_embedding_grad(const int* ids, const void* dy, void* dE, long long n, long long V, int d, float scale, int dy_fp32,
                       int table_fp32, int* ints, float* partial, void* stream);
+int pd_top_logits(const void* z, long long rows, int V, long long ld, int k, float inv_t, void* values, int* indices,
+                  float* tail, int z_fp32, int* status, void* stream);
 int pd_top_kl(const void* z, long long rows, int V, long long ld, const void* indices, int wide, const void* values,
               int values_fp32, int K, const float* tail, double inv_t, float* loss, void* dz, long long ldo,
               const float* scale, float* sums, const float* known, int z_fp32, int* status, int* refused, void* stream);
@@ -217,7 +219,7 @@ Tensor embedding(const Tensor& tokens_in, const Tensor& table_in, double scale, 
   return y;
 }
 
-// ---- distillation loss
+// ---- top logits and distillation loss
 
 // [rows, V] whose rows start at the same address modulo 16 bytes as the rows of z.
 Tensor grad_like(const Tensor& z, long long pitch_in) {
@@ -227,6 +229,21 @@ Tensor grad_like(const Tensor& z, long long pitch_in) {
   return at::empty({first + rows * pitch}, z.options()).as_strided({rows, V}, {pitch, 1}, first);
 }
 long long pitch_of(const Tensor& z) { return z.size(0) > 1 ? z.stride(0) : z.size(1); }
+
+// z [rows, V], neighbouring columns; the results in the shape `lead`, which holds as many rows.
+std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& z, std::vector<int64_t> lead, int64_t k, double temperature,
+                                              int64_t status) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  const Tensor tail = floats(lead, z);
+  lead.push_back(k);
+  const Tensor values = at::empty(lead, z.options()), indices = at::empty(lead, z.options().dtype(at::kInt));
+  if (z.size(0) > 0)
+    check(pd_top_logits(z.const_data_ptr(), z.size(0), static_cast<int>(z.size(1)), pitch_of(z), static_cast<int>(k),
+                        static_cast<float>(1.0 / temperature), values.mutable_data_ptr(), indices.mutable_data_ptr<int>(),
+                        tail.mutable_data_ptr<float>(), fp32(z), reinterpret_cast<int*>(status), current_stream()),
+          "top_logits");
+  return {values, indices, tail};
+}
 
 struct Teacher {
   Tensor indices, values, tail;
@@ -318,6 +335,7 @@ PYBIND11_MODULE(pd_autograd, m) {
   const auto free = pybind11::call_guard<pybind11::gil_scoped_release>();
   m.def("layer_norm", &layer_norm, free);
   m.def("embedding", &embedding, free);
+  m.def("top_logits", &top_logits, free);
   m.def("top_kl", &top_kl, free);
   m.def("top_kl_rows", &top_kl_rows, free);
   m.def("launches", [] { return launches.load(); });

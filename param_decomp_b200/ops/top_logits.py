@@ -20,7 +20,7 @@ import torch
 from torch import Tensor
 
 from param_decomp_b200.ops import native as nv
-from param_decomp_b200.ops.elementwise import _FLOAT, _check, _dense, _flat_rows, _on_current_device, _s
+from param_decomp_b200.ops.elementwise import _FLOAT, _dense, _flat_rows, _on_current_device
 
 MAX_K = 256
 
@@ -31,20 +31,12 @@ class TopLogits(NamedTuple):
     tail: Tensor  # [...] fp32 logsumexp of all other logits over the temperature (-inf where k is the whole row)
 
 
-@lru_cache(maxsize=1)
-def _lib():
-    lib = nv.lib()
-    P, LL, I, F = C.c_void_p, C.c_longlong, C.c_int, C.c_float
-    lib.pd_top_logits.argtypes = [P, LL, I, LL, I, F, P, P, P, I, P, P]
-    lib.pd_top_logits_max_columns.argtypes, lib.pd_top_logits_max_columns.restype = [I], LL
-    lib.pd_top_kl_max_columns.argtypes, lib.pd_top_kl_max_columns.restype = [I], LL
-    return lib
-
-
 @lru_cache(maxsize=4)
 def _max_columns(what: str, fp32: bool) -> int:
     """The widest row that a cluster's shared memory holds."""
-    return (_lib().pd_top_logits_max_columns if what == "top_logits" else _lib().pd_top_kl_max_columns)(fp32)
+    f = nv.lib().pd_top_logits_max_columns if what == "top_logits" else nv.lib().pd_top_kl_max_columns
+    f.argtypes, f.restype = [C.c_int], C.c_longlong
+    return f(fp32)
 
 
 def _check_width(what: str, logits: Tensor) -> None:
@@ -86,17 +78,7 @@ def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:
         raise ValueError(f"top_logits: k from 1 to {min(V, MAX_K)}, not {k}")
     _on_current_device("top_logits", logits)
     _check_width("top_logits", logits)
-    lead = logits.shape[:-1]
-    z = _rows_of(logits.detach())
-    rows = z.shape[0]
-    values = torch.empty(rows, k, device=z.device, dtype=z.dtype)
-    indices = torch.empty(rows, k, device=z.device, dtype=torch.int32)
-    tail = torch.empty(rows, device=z.device, dtype=torch.float32)
-    if rows > 0:
-        _check(_lib().pd_top_logits(z.data_ptr(), rows, V, _pitch(z), k, 1.0 / temperature, values.data_ptr(),
-                                    indices.data_ptr(), tail.data_ptr(), z.dtype is torch.float32,
-                                    nv.status_word().data_ptr(), _s()), "top_logits")
-    return TopLogits(values.view(*lead, k), indices.view(*lead, k), tail.view(lead))
+    return TopLogits(*nv.autograd().top_logits(_rows_of(logits.detach()), logits.shape[:-1], k, temperature, nv.status_ptr()))
 
 
 def _arguments(what: str, logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None, temperature: float):

@@ -777,3 +777,22 @@ def test_values_changed_between_the_passes_are_noticed(nv):
         with pytest.raises(RuntimeError, match="inplace"):
             y.sum().backward()
     _done(nv)
+
+
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("V,d,n", [(700, 1, 60), (5000, 2, 40), (1201, 3, 900), (900, 5, 1), (40000, 7, 300), (2000, 9, 0), (3001, 515, 77),
+                                   (600, 8, 500), (160000, 24, 1000)])
+def test_every_row_of_an_embedding_gradient_is_written(nv, V, d, n, kind):
+    """Rows at every alignment between rows of zeros: whole numbers, so the sums are exact; memory held other values before."""
+    from param_decomp_b200.ops.embedding import embedding
+
+    g = _gen(V + d)
+    tokens, dy = torch.randint(0, V, (n,), generator=g), torch.randint(-2, 3, (n, d), generator=g).float()
+    want = torch.zeros(V, d).index_add_(0, tokens, dy)
+    table = torch.zeros(V, d, dtype=kind).cuda().requires_grad_(True)
+    for _ in range(2):
+        (grad,) = torch.autograd.grad(embedding(tokens.cuda(), table), (table,), dy.to(kind).cuda())
+        assert torch.equal(grad.float().cpu(), want)
+        grad.fill_(5.0)
+        del grad
+    _done(nv)
