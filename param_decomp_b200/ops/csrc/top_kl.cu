@@ -12,6 +12,11 @@
 // of, not a difference, and relative to a logit that is in it: a rest far below the named logits keeps its value.
 // The teacher's side is a chain of dependent steps on K numbers, and so is a loss, formed in 64 bits because it is a small
 // difference of logarithms: a warp of its own does each, up to two rows ahead of the others and a row behind them.
+// A gradient that is asked for by itself starts from the row's sums that an earlier call left (`known`): no sums, no exchange.
+// Measured: loss and gradient of 8192 rows of 50,277 bf16, K = 64: 315 us, 5.2 TB/s, 0.81 of copy bandwidth. 1031 rows of
+// 151,936 fp32, K = 32, a loss and then its gradient: 367 us for 1.88 GB, 5.1 TB/s (443 when the gradient formed the sums
+// again); the loss by itself waits for the cluster's exchange of sums, about 1.7 us a row. Rows to come asked for in L2 were
+// slower (370 us for 315 at 50,277).
 #include "row_slice.cuh"
 
 namespace {
@@ -42,9 +47,10 @@ struct Call {
 };
 
 // A sum of exp(z / T) = 2^(c z) is kept as m, one of its z (the largest, or one that is not far below it), and s, the sum
-// relative to a power of two near that z's own term: 2^k, k = c m to the nearest whole number. One fused multiply-add then gives an exponent, c z - k, without the
-// rounding of c m in it, and a change of k is exact. (Where |c m| is so large that whole numbers are no closer than its
-// rounding, as for logits masked with the type's lowest value, s is relative to exp(m / T) itself.)
+// relative to a power of two near that z's own term: 2^k, k = c m to the nearest whole number. One fused multiply-add then
+// gives an exponent, c z - k, without the rounding of c m in it, and a change of k is exact. (Where |c m| is so large that
+// whole numbers are no closer than its rounding, as for logits masked with the type's lowest value, s is relative to
+// exp(m / T) itself.)
 struct MaxSum {
   float m, s;
 };

@@ -6,11 +6,17 @@
 // largest T_0 of those (over the cluster's blocks, of the threads of one number taken together) is a lower bound of the k-th
 // largest logit, and a tight one (k = 64 of 512 maxima: about 68 logits reach it). Second: logits that reach T_0 are
 // collected with their columns, and exponentials are summed with every logit cut off at T_0, whose term is taken off again
-// once a collected logit. The cluster's first block ranks the collected ones by counting, with (logit, column) as one
-// number, so the order in which they arrived does not matter.
+// once a collected logit. Four more warps of the cluster's first block place the collected ones, sorted into 256 bins by key
+// and counted within a bin, with (logit, column) as one number, so the order in which they arrived does not matter; the
+// others read the next row meanwhile.
 // A row that defeats the bound (fewer than 2 k groups of 16 bytes, ties in masses, rows of -inf) is selected out of global
 // memory by its keys' digits instead, exactly and at any number of ties, and a rest that is small beside what was taken off
 // is summed by itself.
+// Measured: 8192 rows of 50,277 bf16, k = 64: 210 us, 3.9 TB/s (250 with the placing in the readers' path). A row takes a
+// block 7.5 us, of which the sums are 2.9 (two blocks an SM share 16 exponentials a clock), the maxima 1.5, bound and
+// collecting 2.3, waiting for the row 0.5. 1031 rows of 151,936 fp32, k = 256, clusters of 8: 216 us, 2.9 TB/s (390 with the
+// placing in the path, and a warp that was split by a lane that waited alone): a row takes 6.8 us, of which 1 to 2 are the
+// exchange of maxima. Asking for rows to come in L2 gained nothing (217 and 307 us).
 #include <algorithm>
 
 #include "row_slice.cuh"
