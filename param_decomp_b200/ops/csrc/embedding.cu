@@ -537,11 +537,9 @@ int grad(const int* ids, const void* dy, void* dE, int n, int V, int d, float sc
                   reinterpret_cast<uint8_t*>(ints + 2ll * n + 3 * all)};
   const size_t smem = (static_cast<size_t>(span) * (kSortWarps + 3) + 2 * kSortWarps * kNoted) * sizeof(int);
   auto kern = embedding_sort_kernel<T, P, kVec>;
-  static bool sized = false;  // the same answer whoever asks first
-  if (!sized && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (kMaxSpan * (kSortWarps + 3) + 2 * kSortWarps * kNoted) * 4) != cudaSuccess)
-    return 2;
-  sized = true;
+  static std::atomic<unsigned long long> asked{0};
+  constexpr int kMostBytes = (kMaxSpan * (kSortWarps + 3) + 2 * kSortWarps * kNoted) * 4;
+  if (!make_room(asked, reinterpret_cast<const void*>(kern), kMostBytes)) return 2;
   // half of L2 may hold the rows until they are summed
   const int ahead = static_cast<long long>(n) * d * static_cast<long long>(sizeof(T)) <= (64ll << 20);
   kern<<<blocks, kSortThreads, smem, st>>>(ids, static_cast<const T*>(dy), static_cast<P*>(dE), n, V, d, scale, span, ahead,

@@ -481,30 +481,27 @@ inline int rows_of(const Shape& s, bool fp32, bool backward) {
   return s.ch > 1 ? 1 : s.wpr > 8 || (fp32 && backward) ? 2 : 4;
 }
 
-// Blocks that fit the machine at once, at most one a handful of rows. What fits an SM is asked once a kernel and block
-// size (`fit`, zero at first; the answer is the same whoever writes it).
-template <typename K>
-inline int grid_for(K kern, int* fit, int threads, size_t smem, long long rows, int rpb) {
-  int& per_sm = fit[threads / 32];
-  if (per_sm == 0 && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1)) {
-    per_sm = 0;
-    return 0;
-  }
-  return static_cast<int>(std::min<long long>((rows + rpb - 1) / rpb, 148ll * per_sm));
-}
+// What is asked once about a kernel: its room, and how many blocks of a size fit an SM (0: not yet).
+struct Fit {
+  std::atomic<unsigned long long> asked{0};
+  std::atomic<int> per_sm[kMaxWarps + 1] = {};
+};
 
 template <typename T, int kCh, int kRows, int kTensors, bool kVec>
 inline size_t slots_bytes(int threads) {
   using Copies = Ahead<T, kCh, kRows, kTensors>;
   return kVec ? static_cast<size_t>(Copies::kStages) * Copies::kPieces * threads * 16 : 0;
 }
-// The blocks of a kernel that walks rows, or 0; `fit` as for grid_for.
+// The blocks of a kernel that walks rows: as many as fit the machine at once, at most one a handful of rows. 0: none fits.
 template <typename K>
-inline int prepare(K kern, int* fit, int threads, size_t smem, long long rows, int rpb) {
-  if (fit[threads / 32] == 0 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024) != cudaSuccess)
-    return 0;
-  return grid_for(kern, fit, threads, smem, rows, rpb);
+inline int prepare(K kern, Fit& fit, int threads, size_t smem, long long rows, int rpb) {
+  if (!make_room(fit.asked, reinterpret_cast<const void*>(kern), 216 * 1024)) return 0;
+  int per_sm = fit.per_sm[threads / 32].load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1) return 0;
+    fit.per_sm[threads / 32].store(per_sm, std::memory_order_relaxed);
+  }
+  return static_cast<int>(std::min<long long>((rows + rpb - 1) / rpb, 148ll * per_sm));
 }
 
 template <typename T, int kCh, int kRows, bool kVec>
@@ -513,7 +510,7 @@ int fwd(const void* x, const void* w, const void* b, void* y, float* mean, float
   const int threads = 32 * s.wpr * s.groups;
   const size_t smem = slots_bytes<T, kCh, kRows, 1, kVec>(threads);
   auto kern = layer_norm_fwd_kernel<T, kCh, kRows, kVec>;
-  static int fit[kMaxWarps + 1];
+  static Fit fit;
   const int grid = prepare(kern, fit, threads, smem, rows, kRows * s.groups);
   if (grid == 0) return 2;
   kern<<<grid, threads, smem, st>>>(static_cast<const T*>(x), w, b, static_cast<T*>(y), mean, rstd, static_cast<int>(rows), d, eps, s.wpr,
@@ -528,7 +525,7 @@ int bwd(const void* x, const void* w, const void* dy, const float* mean, const f
   const size_t sums = kParams && s.groups > 1 ? static_cast<size_t>(16 * s.wpr * 256) : 0;  // 2 d floats and more
   const size_t smem = std::max(sums, slots_bytes<T, kCh, kRows, 2, kVec>(threads));
   auto kern = layer_norm_bwd_kernel<T, kCh, kRows, kVec, kParams>;
-  static int fit[kMaxWarps + 1];
+  static Fit fit;
   int grid = prepare(kern, fit, threads, smem, rows, kRows * s.groups);
   if (grid == 0) return 2;
   if (kParams) grid = std::min(grid, max_blocks);

@@ -2,6 +2,8 @@
 // and launches that overlap their set-up with the end of the kernel before them.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace pd {
@@ -52,6 +54,17 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// A kernel's dynamic shared memory, asked for once a device: a bit each in a word that belongs to the kernel.
+inline bool make_room(std::atomic<unsigned long long>& asked, const void* kern, int bytes) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const unsigned long long bit = 1ull << (device & 63);
+  if (asked.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  asked.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 // A kernel launched with `launch_after` may begin before the kernel ahead of it in the stream has ended: it calls

@@ -618,9 +618,8 @@ int launch(const Call& call, cudaStream_t st) {
   if (plan.cs == 0) return 5;
   const int smem = plan.slice * 16, threads = 32 * (kWarps + 2);
   auto kern = top_kl_kernel<T>;
-  static bool sized = false;  // the same answer whoever asks first
-  if (!sized && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kWholeSm) != cudaSuccess) return 2;
-  sized = true;
+  static std::atomic<unsigned long long> asked{0};
+  if (!make_room(asked, reinterpret_cast<const void*>(kern), kWholeSm)) return 2;
   return launch_clusters(kern, call.rows, plan.cs, threads, smem, st, call, plan);
 }
 

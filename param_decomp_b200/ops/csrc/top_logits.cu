@@ -762,9 +762,8 @@ int top(const void* z, long long rows, int V, long long ld, int k, float inv_t, 
   if (plan.cs == 0) return 5;
   const int smem = plan.slice * 16 + (plan.cs > 1 ? 2 * plan.cs * kMaxima * 2 : 0);
   auto kern = top_logits_kernel<T>;
-  static bool sized = false;  // the same answer whoever asks first
-  if (!sized && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kWholeSm + kMaximaBytes) != cudaSuccess) return 2;
-  sized = true;
+  static std::atomic<unsigned long long> asked{0};
+  if (!make_room(asked, reinterpret_cast<const void*>(kern), kWholeSm + kMaximaBytes)) return 2;
   return launch_clusters(kern, rows, plan.cs, kThreads + 32 + kSelThreads, smem, st, static_cast<const T*>(z), ld, V, k, inv_t, plan,
                          static_cast<T*>(values), indices, tail, status);
 }

@@ -73,6 +73,8 @@ std::shared_ptr<N> node_of(const T&... inputs) {
 }
 template <typename... T>
 bool wanted(const T&... inputs) {
+  for (const Tensor& t : {inputs...})
+    TORCH_CHECK(!torch::autograd::isFwGradDefined(t), "the kernels have no forward-mode derivative");
   return at::GradMode::is_enabled() && torch::autograd::any_variable_requires_grad(variable_list{inputs...});
 }
 

@@ -796,3 +796,15 @@ def test_every_row_of_an_embedding_gradient_is_written(nv, V, d, n, kind):
         grad.fill_(5.0)
         del grad
     _done(nv)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_is_refused(nv, which):
+    import torch.autograd.forward_ad as fwd
+
+    _, leaves, f = _differentiable()[which]
+    with fwd.dual_level():
+        dual = fwd.make_dual(leaves[0].detach(), torch.ones_like(leaves[0]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            f(dual, *leaves[1:])
+    _done(nv)
