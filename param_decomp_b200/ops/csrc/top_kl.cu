@@ -14,9 +14,9 @@
 // difference of logarithms: a warp of its own does each, up to two rows ahead of the others and a row behind them.
 // A gradient that is asked for by itself starts from the row's sums that an earlier call left (`known`): no sums, no exchange.
 // Measured: loss and gradient of 8192 rows of 50,277 bf16, K = 64: 315 us, 5.2 TB/s, 0.81 of copy bandwidth. 1031 rows of
-// 151,936 fp32, K = 32, a loss and then its gradient: 367 us for 1.88 GB, 5.1 TB/s (443 when the gradient formed the sums
-// again); the loss by itself waits for the cluster's exchange of sums, about 1.7 us a row. Rows to come asked for in L2 were
-// slower (370 us for 315 at 50,277).
+// 151,936 fp32, K = 32, a loss and then its gradient: 341 us for 1.88 GB, 5.5 TB/s, 0.85 of copy bandwidth (443 when the
+// gradient formed the sums again; 367 when the blocks waited for the exchange of sums, 1.7 us a row, where no gradient is
+// asked for and only the first block needs them). Rows to come asked for in L2 were slower (370 us for 315 at 50,277).
 #include "row_slice.cuh"
 
 namespace {
@@ -260,15 +260,18 @@ __device__ float loss_of(const Call& call, long long row, const Teacher& t, cons
 // one that may change any part of it.
 struct Shared {
   RowQueue queue;
-  unsigned long long bars[kWarps + 8];
+  unsigned long long bars[kWarps + 12];
   Teacher teacher[3];
   float named[3][kMaxK];  // student's logits at the columns, in the slots that speak for them
-  Row red[kWarps], xch[3][8], sums[2];
+  Row red[kWarps], xch[3][8], sums[3];  // of the last three rows, as `named`: blocks may be two rows apart
   float2 part[kWarps];
   int next;  // the row behind the present one, or -1
   int rows;  // this cluster has had, once there is no further one
   int abort_flag;
 };
+
+constexpr int kShared = 11264;
+static_assert(sizeof(Shared) <= kShared);
 
 template <typename T>
 __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call call, const SlicePlan plan) {
@@ -281,11 +284,11 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
   const float c = static_cast<float>(call.inv_t * 1.4426950408889634);
   const RowSlice<T> rows{static_cast<const T*>(call.z), call.ld, call.V, rank * plan.slice, plan.slice, plan.per};
   T* buf = reinterpret_cast<T*>(smem);
-  const uint32_t bar0 = smem_u32(sh.bars), ready = bar0 + 8 * kWarps, summed = ready + 16, lost = ready + 32, met = ready + 48;
+  const uint32_t bar0 = smem_u32(sh.bars), ready = bar0 + 8 * kWarps, lost = ready + 16, summed = ready + 32, met = ready + 64;
   if (tid == 0) {
     for (int i = 0; i < warps; ++i) mbar_init(bar0 + 8 * i, 1);
-    for (int i = 0; i < 6; ++i) mbar_init(ready + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(met + 8 * i, cs);
+    for (int i = 0; i < 8; ++i) mbar_init(ready + 8 * i, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(met + 8 * i, cs);
     sh.rows = -1;
     sh.queue.init();
     sh.abort_flag = 0;
@@ -298,8 +301,23 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
   };
   // The n-th completion of a pair of barriers that take turns: one that is waited for late is not mistaken for the next.
   auto wait_pair = [&](uint32_t pair, int n) { return short_wait<false>(pair + 8 * (n & 1), (n >> 1) & 1, &sh.abort_flag); };
+  // The n-th completion of four that take turns.
+  auto wait_four = [&](uint32_t four, int n) { return short_wait<false>(four + 8 * (n & 3), (n >> 2) & 1, &sh.abort_flag); };
+  auto wait_met = [&](int n) { return short_wait<true>(met + 8 * (n & 3), (n >> 2) & 1, &sh.abort_flag); };
   const bool losses = rank == 0 && call.loss != nullptr;
   const bool loose = cs > 1 && call.known != nullptr;  // nothing else keeps the cluster's blocks together
+  const bool apart = cs > 1 && call.dz == nullptr;     // only the first block needs the cluster's sums, and not to go on
+  auto send = [&](const Row& sums, int n, int block) {  // this block's part of a row's
+    const uint32_t to = mapa_shared(smem_u32(&sh.xch[n % 3][rank]), block);
+    store_cluster_f32(to, sums.rest.m);
+    store_cluster_f32(to + 4, sums.rest.s);
+    store_cluster_f32(to + 8, sums.top.m);
+    store_cluster_f32(to + 12, sums.top.s);
+  };
+  auto met_sums = [&](int n) {  // the warp
+    const Row none{{-INFINITY, 0.0f}, {-INFINITY, 0.0f}};
+    return merge_lanes((lane & 7) < cs ? sh.xch[n % 3][lane & 7] : none, 8, c);
+  };
   if (warp == warps) {  // the teacher's side, up to two rows ahead
     auto teach = [&](int row, int n) {
       Teacher& t = sh.teacher[n % 3];
@@ -334,25 +352,34 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
     teach(next(1), 1);
     int ahead = next(2);
     for (int n = 0; sh.teacher[n % 3].row >= 0; ++n) {
-      late(wait_pair(summed, n));  // the others are done with the row before,
+      late(wait_four(summed, n));  // the others are done with the row before,
       if (losses && n > 0) late(wait_pair(lost, n - 1));  // and so is the warp below
-      if (loose && rank == 0 && n > 0) late(wait_pair(met, n - 1));  // all blocks have begun the row before: none is left far behind
+      if (loose && rank == 0 && n > 0) late(wait_met(n - 1));  // all blocks have begun the row before: none is left far behind
       teach(ahead, n + 2);
+      if (apart && rank == 0) late(wait_pair(lost, n));  // all blocks have handed this row over: its places serve the third one on
       ahead = next(n + 3);
     }
   } else if (warp == warps + 1) {  // losses, a row behind
-    // What a loss reads is written again three rows on, by whichever block, and not before the teacher of that row is
+    // What a loss reads is written again by a row that is not told to any block before the teacher of the row behind is
     // there, which waits for this warp.
-    for (int n = 0; losses || loose; ++n) {
-      late(wait_pair(summed, n));
+    for (int n = 0; losses || loose || apart; ++n) {
+      late(wait_four(summed, n));
       if (n == *static_cast<volatile int*>(&sh.rows) || *static_cast<volatile int*>(&sh.abort_flag)) break;
-      if (loose) {
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(met + 8 * (n & 1), 0));
+      Row sums = sh.sums[n % 3];
+      if (loose || apart) {
+        if (lane == 0) {
+          if (apart) send(sums, n, 0);
+          mbar_arrive_cluster(mapa_shared(met + 8 * (n & 3), 0));  // with it, the named logits that were stored before the barriers
+        }
         __syncwarp();
-        continue;
+        if (loose || rank != 0) continue;
+        late(wait_met(n));
+        sums = met_sums(n);
       }
       const Teacher& t = sh.teacher[n % 3];
-      const float loss = loss_of(call, t.row, t, sh.sums[n & 1], sh.named[n % 3], c, lane);
+      if (call.sums != nullptr && lane == 0)
+        call.sums[t.row] = make_float4(sums.rest.m, sums.rest.s, sums.top.m, sums.top.s);
+      const float loss = loss_of(call, t.row, t, sums, sh.named[n % 3], c, lane);
       if (lane == 0) {
         call.loss[t.row] = loss;
         mbar_arrive(lost + 8 * (n & 1));
@@ -397,7 +424,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
         sync_first(nt);
         next = sh.next;
       } else {
-        // Named columns leave the row: their logits go to every block of the cluster. A warp with slots waits for all parts
+        // Named columns leave the row: their logits go to the first block, for the loss. A warp with slots waits for all parts
         // of the slice, and as a whole: lanes that wait each for their own leave it split for the rest of the kernel.
         if (32 * warp < call.K)
           for (int w = 0; w < warps; ++w) late(short_wait<false>(bar0 + 8 * w, n & 1, &sh.abort_flag));
@@ -411,9 +438,8 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
             } else {
               mine_logit = as_float(rows.row(row)[mine]);  // at a ragged end, which is already without it
             }
-            const uint32_t local = smem_u32(zk + tid);
             if (cs > 1)
-              for (int b = 0; b < cs; ++b) store_cluster_f32(mapa_shared(local, b), mine_logit);
+              store_cluster_f32(mapa_shared(smem_u32(zk + tid), 0), mine_logit);
             else
               zk[tid] = mine_logit;
           }
@@ -488,26 +514,19 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
           sync_first(nt);
           sums = merge_lanes(sh.red[lane & 7], 8, c);
         }
-        if (cs > 1) {
+        if (cs > 1 && !apart) {
           if (warp == 0 && lane < cs) {
-            const uint32_t to = mapa_shared(smem_u32(&sh.xch[n % 3][rank]), lane);
-            store_cluster_f32(to, sums.rest.m);
-            store_cluster_f32(to + 4, sums.rest.s);
-            store_cluster_f32(to + 8, sums.top.m);
-            store_cluster_f32(to + 12, sums.top.s);
-            mbar_arrive_cluster(mapa_shared(met, lane));  // with it, the named logits that were stored before the barriers
+            send(sums, n, lane);
+            mbar_arrive_cluster(mapa_shared(met + 8 * (n & 3), lane));
           }
           __syncwarp();
-          late(short_wait<true>(met, n & 1, &sh.abort_flag));
-          const Row none{{-INFINITY, 0.0f}, {-INFINITY, 0.0f}};
-          sums = (lane & 7) < cs ? sh.xch[n % 3][lane & 7] : none;
-          sums = merge_lanes(sums, 8, c);
+          late(wait_met(n));
+          sums = met_sums(n);
         }
       }
       if (tid == 0) {
-        sh.sums[n & 1] = sums;
-        if (call.sums != nullptr && rank == 0) call.sums[t.row] = make_float4(sums.rest.m, sums.rest.s, sums.top.m, sums.top.s);
-        mbar_arrive(summed + 8 * (n & 1));
+        sh.sums[n % 3] = sums;
+        mbar_arrive(summed + 8 * (n & 3));
       }
       __syncwarp();
       auto ask_for_next = [&] {  // the warp's part of it
@@ -602,15 +621,15 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
     }
     if (tid == 0) {
       *static_cast<volatile int*>(&sh.rows) = n;
-      mbar_arrive(summed + 8 * (n & 1));
+      mbar_arrive(summed + 8 * (n & 3));
     }
   }
   __syncwarp();
   if (cs > 1) cluster_sync_all();  // no block leaves while another one may still store to it
 }
 
-// Beside a slice, 10 KB of fixed shared memory and 1 KB of the system's: two blocks an SM, or one.
-constexpr long long kHalfSm = 102 * 1024, kWholeSm = 216 * 1024;
+// A slice beside the fixed shared memory and 1 KB of the system's: two blocks an SM, or one.
+constexpr long long kHalfSm = 113 * 1024 - kShared, kWholeSm = 227 * 1024 - kShared;
 
 template <typename T>
 int launch(const Call& call, cudaStream_t st) {
@@ -633,7 +652,7 @@ extern "C" int pd_top_kl(const void* z, long long rows, int V, long long ld, con
                          long long ldo, const float* scale, float* sums, const float* known, int z_fp32, int* status,
                          int* refused, void* stream) {
   if (rows <= 0 || rows >= (1ll << 28) || V <= 0 || K <= 0 || K > kMaxK || !(inv_t > 0.0)) return 5;
-  if (known != nullptr && (dz == nullptr || loss != nullptr)) return 5;
+  if ((dz == nullptr && loss == nullptr) || (known != nullptr && (dz == nullptr || loss != nullptr))) return 5;
   const Call call{z, rows, ld, V, indices, wide, values, values_fp32, K, tail, inv_t, loss, dz, ldo, scale,
                   reinterpret_cast<float4*>(sums), reinterpret_cast<const float4*>(known), status, refused};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
