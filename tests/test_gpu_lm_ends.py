@@ -808,3 +808,31 @@ def test_forward_mode_is_refused(nv, which):
         with pytest.raises(RuntimeError, match="forward-mode"):
             f(dual, *leaves[1:])
     _done(nv)
+
+
+@pytest.mark.parametrize("kind,V", [(f32, 60000), (bf, 151936), (f32, 300007)])
+def test_clusters_on_two_streams_at_once(nv, kind, V):
+    """Rows spread over 4 and 8 blocks, two calls of each kernel at a time: each result as alone."""
+    from param_decomp_b200.ops.top_logits import top_kl, top_logits
+
+    def work(z, idx, t):
+        leaf = z.detach().requires_grad_(True)
+        loss = top_kl(leaf, idx, t, None, 1.5)
+        return [*top_logits(z, 50), loss.detach(), *torch.autograd.grad(loss.sum(), (leaf,))]
+
+    sets = []
+    for i in range(2):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        sets.append((torch.randn(90, V, generator=g, device="cuda").to(kind),
+                     torch.randint(0, V, (90, 33), generator=g, device="cuda"), torch.randn(90, 33, generator=g, device="cuda")))
+    want = [work(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(work(*s))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+    _done(nv)
