@@ -19,7 +19,7 @@ def nv():
         pytest.skip("no CUDA device")
     from param_decomp_b200.ops import native
 
-    native.lib()  # must load: no silent fallback on a GPU box
+    native.lib()  # must load: nothing falls back to another path where there is a GPU
     return native
 
 
