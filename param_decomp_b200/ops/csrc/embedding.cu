@@ -3,16 +3,18 @@
 // rows once and writes every row of the table (most of them zeros).
 //
 // The gradient sums each row in fp32 over its tokens in ascending order and rounds once, with two launches and no float
-// atomics. First kernel: block b owns a span of the vocabulary. Its 32 warps read all tokens (from L2, as the lookup left
-// them in 32 bits), each its own consecutive part, note those of the block and count the valid tokens of lower ids, which
-// gives the block's place in the sorted order without asking the other blocks. The noted ones are sorted by counting: id,
+// atomics. First kernel: ids are dealt to the blocks like cards (id v is the v / blocks -th of block v % blocks), since
+// vocabularies hold frequent tokens together: with a span of neighbouring ids a block, 32,768 tokens over 50,277 ids in
+// order of frequency took 270 us, so 56 (58 with ids in no order, either way). A block's 32 warps read all tokens (from L2,
+// as the lookup left them in 32 bits), each its own consecutive part, note those of the block and count those of the blocks
+// before it, which gives the block's place in the sorted order without asking them. The noted ones are sorted by counting: id,
 // then warp, then position, and rows of up to kSlab tokens are summed. Second kernel: ids with more tokens, in slabs of
 // kSlab places of the sorted order, so a token that fills a tenth of the batch is shared by many blocks; a slab's sum goes
 // to scratch and the block that finishes a run last adds its slabs in their order. Rows of dy come in no order that a cache
 // could guess, so the block that finds a token asks for its row in L2 at once, long before it is summed. The rows without a
 // token, most of the bytes, are written by blocks of the second kernel too: zeros at the full rate in the first one made the
 // loads of its sums wait for several microseconds each (32,768 tokens in 50,277 rows of 768: 77 us).
-// Measured there, bf16: lookup 15.6 us (6.4 TB/s, copy bandwidth), first kernel 34, second 27: 76 us with the launches. 6151
+// Measured there, bf16: lookup 15.6 us (6.4 TB/s, copy bandwidth), first kernel 34, second 25: 75 us with the launches. 6151
 // tokens in 151,936 rows of 515 fp32: 11, 26 and 57. The first kernel is a chain of steps, each with its own latency, over
 // all tokens in every block; what the second has to write takes 12 and 48 us of it.
 #include <algorithm>
@@ -28,6 +30,9 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxSpan = 1280;  // ids a block: 32 counts of 4 bytes each in shared memory
 constexpr int kNoted = 128;     // tokens a warp notes; where there are more, it reads its part again
+// Rows a warp asks for in L2 while it reads tokens, the first it finds: where a token fills a tenth of the batch, its block
+// would be busy asking (30,000 cycles for 9,000; 32,768 tokens: 61 us without a limit, 58 at 32 and 16, 59 at 8).
+constexpr int kAhead = 32;
 constexpr int kRunThreads = 384;
 constexpr int kMaxPer = 512;  // ids of a block that writes zeros
 
@@ -253,7 +258,16 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const i
   int* single = listed + span;  // [span] ids with one token
   __shared__ int warp_total[kSortWarps], below_of[kSortWarps], n_few, n_many, n_single;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int lo = blockIdx.x * span, ids = min(span, V - lo);
+  // id b + i blocks is block b's i-th
+  const int blocks = gridDim.x, b = blockIdx.x, ids = (V - b + blocks - 1) / blocks;
+  const unsigned inverse = 0xFFFFFFFFu / blocks;
+  auto id_of = [&](int i) { return b + i * blocks; };
+  auto owner_of = [&](int t, int& i) {  // the block of an id, its place there; no block, past all of them, for -1
+    const unsigned u = static_cast<unsigned>(t), q = __umulhi(u, inverse), r = u - q * blocks;  // q or one less
+    const bool one_less = r >= static_cast<unsigned>(blocks);
+    i = static_cast<int>(one_less ? q + 1 : q);
+    return t < 0 ? 0x7FFFFFFF : static_cast<int>(one_less ? r - blocks : r);
+  };
   for (int i = tid; i < kSortWarps * span; i += kSortThreads) hist[i] = 0;
   if (tid == 0) n_few = n_many = n_single = 0;
   __syncthreads();
@@ -274,24 +288,23 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const i
       f(i, q);
     }
   };
-  auto in_block = [&](int t) { return static_cast<unsigned>(t - lo) < static_cast<unsigned>(ids); };
   scan([&](int i, const int4& q) {
-    const unsigned first = static_cast<unsigned>(lo);  // ids out of the table are -1: never below
-    below += (static_cast<unsigned>(q.x) < first) + (static_cast<unsigned>(q.y) < first) + (static_cast<unsigned>(q.z) < first) +
-             (static_cast<unsigned>(q.w) < first);
-    const bool o0 = in_block(q.x), o1 = in_block(q.y), o2 = in_block(q.z), o3 = in_block(q.w);
+    int i0, i1, i2, i3;
+    const int r0 = owner_of(q.x, i0), r1 = owner_of(q.y, i1), r2 = owner_of(q.z, i2), r3 = owner_of(q.w, i3);
+    below += (r0 < b) + (r1 < b) + (r2 < b) + (r3 < b);
+    const bool o0 = r0 == b, o1 = r1 == b, o2 = r2 == b, o3 = r3 == b;
     if (!__any_sync(0xffffffffu, o0 | o1 | o2 | o3)) return;
     const unsigned b0 = __ballot_sync(0xffffffffu, o0), b1 = __ballot_sync(0xffffffffu, o1),
                    b2 = __ballot_sync(0xffffffffu, o2), b3 = __ballot_sync(0xffffffffu, o3), under = (1u << lane) - 1;
     int at = found + __popc(b0 & under) + __popc(b1 & under) + __popc(b2 & under) + __popc(b3 & under);
-    auto note = [&](bool own, int t, int position) {
+    auto note = [&](bool own, int bin, int position) {
       if (!own) return;
-      atomicAdd(mine + (t - lo), 1);
-      if (ahead) fetch_to_l2(dy + static_cast<long long>(position) * d, d);
+      atomicAdd(mine + bin, 1);
+      if (ahead && at < kAhead) fetch_to_l2(dy + static_cast<long long>(position) * d, d);
       if (at < kNoted) my_noted[at] = position;
       ++at;
     };
-    note(o0, q.x, i), note(o1, q.y, i + 1), note(o2, q.z, i + 2), note(o3, q.w, i + 3);
+    note(o0, i0, i), note(o1, i1, i + 1), note(o2, i2, i + 2), note(o3, i3, i + 3);
     found += __popc(b0) + __popc(b1) + __popc(b2) + __popc(b3);
   });
   below = __reduce_add_sync(0xffffffffu, below);
@@ -322,13 +335,13 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const i
     if (k < each && each * tid + k < ids) {
       const int i = each * tid + k;
       count[i] = totals[k];
-      runs.empty[lo + i] = totals[k] == 0;
+      runs.empty[id_of(i)] = totals[k] == 0;
       if (totals[k] == 1) single[atomicAdd(&n_single, 1)] = i;
       if (totals[k] > 1 && totals[k] <= kSlab) listed[atomicAdd(&n_few, 1)] = i;
       if (totals[k] > kSlab) {
         listed[span - 1 - atomicAdd(&n_many, 1)] = i;
         const int slab = at / kSlab;
-        runs.id[slab] = lo + i;
+        runs.id[slab] = id_of(i);
         runs.end[slab] = at + totals[k];
         runs.done[slab] = 0;
       }
@@ -356,12 +369,15 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const i
   if (found <= kNoted) {
     for (int e = lane; e - lane < found; e += 32) {
       const int position = e < found ? my_noted[e] : -1;
-      place(e < found, e < found ? ids_of[position] - lo : 0, position);
+      int bin = 0;
+      if (e < found) owner_of(ids_of[position], bin);
+      place(e < found, bin, position);
     }
   } else {
     for (int i = from + lane; i - lane < to; i += 32) {
-      const int t = i < to ? ids_of[i] : -1;
-      place(in_block(t), t - lo, i);
+      int bin;
+      const bool own = owner_of(i < to ? ids_of[i] : -1, bin) == b;
+      place(own, bin, i);
     }
   }
   __syncthreads();
@@ -370,7 +386,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const i
   auto start_of = [&](int i) { return i == 0 ? base : hist[(kSortWarps - 1) * span + i - 1]; };
   if (n > kSlab) {  // else the second kernel does not look for runs
     for (int i = base + tid; i < base + block_total; i += kSortThreads) runs.run_start[i] = -1;
-    if (lo + ids == V)  // places behind the last valid token
+    if (b == blocks - 1)  // places behind the last valid token
       for (int i = base + block_total + tid; i < n; i += kSortThreads) runs.run_start[i] = -1;
     __syncthreads();
     for (int m = warp; m < n_many; m += kSortWarps) {
@@ -387,7 +403,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const i
     int from = 0, to = 0, c0 = d;  // lane u: the u-th item's
     if (lane < kItems && item + lane < n_single * pieces) {
       const int i = single[(item + lane) / pieces];
-      from = position_of(i, 0), to = lo + i, c0 = ((item + lane) % pieces) * 256;
+      from = position_of(i, 0), to = id_of(i), c0 = ((item + lane) % pieces) * 256;
     }
     copy_rows<T, P, kVec>(dy, dE, from, to, c0, d, scale, lane);
   }
@@ -395,7 +411,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const i
   for (int item = warp; item < n_few * pieces; item += kSortWarps) {
     const int i = listed[item / pieces], piece = item % pieces;
     const int k = count[i], row_of = lane < k ? position_of(i, lane) : 0;
-    sum_rows<T, P, kVec>(dy, row_of, k, dE + static_cast<long long>(lo + i) * d, 256 * piece, d, scale, lane);
+    sum_rows<T, P, kVec>(dy, row_of, k, dE + static_cast<long long>(id_of(i)) * d, 256 * piece, d, scale, lane);
   }
 }
 

@@ -836,3 +836,18 @@ def test_clusters_on_two_streams_at_once(nv, kind, V):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
     _done(nv)
+
+
+@pytest.mark.parametrize("V,n,d", [(50277, 20000, 64), (2000, 3000, 33), (400000, 5000, 16), (149, 700, 8), (148, 40, 24)])
+def test_embedding_gradient_of_ids_in_order_of_frequency(nv, V, n, d):
+    """Low ids hold most of the tokens, up to thousands each: whole numbers, so the sums are exact."""
+    from param_decomp_b200.ops.embedding import embedding
+
+    g = _gen(V)
+    tokens = (V ** torch.rand(n, generator=g, dtype=torch.float64)).long() - 1
+    dy = torch.randint(-2, 3, (n, d), generator=g).float()
+    want = torch.zeros(V, d).index_add_(0, tokens, dy)
+    table = torch.zeros(V, d).cuda().requires_grad_(True)
+    (grad,) = torch.autograd.grad(embedding(tokens.cuda(), table), (table,), dy.cuda())
+    assert torch.equal(grad.cpu(), want)
+    _done(nv)
