@@ -647,12 +647,20 @@ __global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_ker
           sync_first(kThreads);
         }
         // The k-th largest of the maxima in the upper 16 bits of its key, rounded down: by a histogram of their distances
-        // from the largest, 128 bins an octave; where that does not reach far enough, of 16 and then of one.
+        // from the largest, 512 of them (4 octaves); where that does not reach far enough (a bound near zero or below it, under
+        // a positive maximum), by one of 128 distances a bin and another one of the distances in the bin that was found.
         const uint32_t top = sh.top[turn];
-        uint32_t bound;
-        for (int coarse = 0;; coarse = coarse == 0 ? 3 : 7) {
-          atomicAdd(hist + min(kBins - 1, (top - (keys >> 16)) >> coarse), 1);
-          atomicAdd(hist + min(kBins - 1, (top - (keys & 0xFFFFu)) >> coarse), 1);
+        uint32_t bound, from = 0;
+        int need = k;
+        for (int level = 0;; ++level) {
+          const int down = level == 1 ? 7 : 0;
+          const uint32_t stop_at = level == 2 ? 128u : 0x10000u;  // distances past `from` that count
+          auto note = [&](uint32_t key) {
+            const uint32_t past = top - key - from;  // wraps below `from`
+            if (past < stop_at) atomicAdd(hist + min(kBins - 1u, past >> down), 1);
+          };
+          note(keys >> 16);
+          note(keys & 0xFFFFu);
           sync_first(kThreads);
           int count[kBins / 32], total = 0;  // every warp for itself
 #pragma unroll
@@ -667,18 +675,27 @@ __global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_ker
             const int v = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += v;
           }
-          const int holder = __ffs(__ballot_sync(0xffffffffu, upto >= k)) - 1;  // kMaxima >= 2 k: there is one
+          const int holder = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;  // kMaxima >= 2 k: there is one
           int before = upto - total, bin = 0;
 #pragma unroll
           for (int i = 0; i < kBins / 32; ++i) {
-            bin += before + count[i] < k;
-            before += count[i];
+            if (before + count[i] < need) {
+              before += count[i];
+              ++bin;
+            } else {
+              break;
+            }
           }
+          before = __shfl_sync(0xffffffffu, before, holder);
           bin = __shfl_sync(0xffffffffu, kBins / 32 * lane + min(bin, kBins / 32 - 1), holder);
-          if (bin < kBins - 1 || coarse == 7) {
-            const uint32_t reach = (static_cast<uint32_t>(bin + 1) << coarse) - 1;
-            bound = bin < kBins - 1 && reach < top ? top - reach : 0;
+          if (level == 2 || (level == 0 && bin < kBins - 1)) {
+            const uint32_t reach = from + bin;
+            bound = reach < top ? top - reach : 0;
             break;
+          }
+          if (level == 1) {
+            from = static_cast<uint32_t>(bin) << 7;
+            need -= before;
           }
           sync_first(kThreads);
           hist[tid] = hist[tid + kThreads] = 0;
