@@ -289,6 +289,25 @@ def test_top_logits_against_a_stable_sort(nv, n, V, k, kind):
     _done(nv)
 
 
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("n,V,k,steep", [(40, 50277, 64, 1.0), (40, 50277, 256, 1.0), (40, 50277, 256, 2.0), (9, 151936, 64, 2.0),
+                                         (9, 151936, 256, 2.0), (6, 9000, 256, 4.0), (5, 3000, 100, 3.0), (3, 400001, 256, 1.5)])
+def test_top_logits_of_columns_in_order_of_frequency(nv, n, V, k, steep, kind):
+    """Logits about a mean that falls with the logarithm of the column, above and below zero: the largest are neighbours, more
+    reach the first bound than there is room for. The same in every run."""
+    from param_decomp_b200.ops.top_logits import top_logits
+
+    z = torch.randn(n, V, generator=_gen(V + k)) * 1.5 - steep * torch.log(torch.arange(1, V + 1).float()) + 2.0
+    z[0] -= 40.0
+    z = z.to(kind)
+    _check_top(z.cuda(), k)
+    _check_top(z.cuda(), k, 3.0)
+    first = top_logits(z.cuda(), k)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, top_logits(z.cuda(), k)))
+    _done(nv)
+
+
 @pytest.mark.parametrize("kind,n,V,k", [(f32, 900, 5003, 20), (bf, 900, 5003, 200), (f32, 300, 151936, 64)])
 def test_top_logits_do_not_change_from_run_to_run(nv, kind, n, V, k):
     """Logits are collected in the order in which threads come to them; nothing of that is left in the tails."""
