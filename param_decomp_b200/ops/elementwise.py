@@ -3,7 +3,6 @@
 from __future__ import annotations
 
 import ctypes as C
-from functools import lru_cache
 
 import torch
 from torch import Tensor
