@@ -765,7 +765,16 @@ __global__ void __launch_bounds__(kThreads + 32 + kSelThreads, 2) top_logits_ker
       __syncwarp();
       r = next;
     }
-    if (warp == 0 && rank == 0 && n >= 2) late(wait_pair(selected, n - 2));
+    // Before the end is written over the entry of two rows ago the cluster meets as it does in every row: the first block has
+    // waited for that row's selection, so the warps that relay, and the barriers they arrive on, are past it in all blocks.
+    if (warp == 0) {
+      if (rank == 0 && n >= 2) late(wait_pair(selected, n - 2));
+      if (cs > 1) {
+        if (lane < cs) mbar_arrive_cluster(mapa_shared(met, lane));
+        __syncwarp();
+        late(short_wait<true>(met, n & 1, &sh.abort_flag));
+      }
+    }
     if (tid == 0) sh.work[n & 1].row = -1;
     hand_over(n);
   }

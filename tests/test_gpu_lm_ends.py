@@ -870,3 +870,24 @@ def test_embedding_gradient_of_ids_in_order_of_frequency(nv, V, n, d):
     (grad,) = torch.autograd.grad(embedding(tokens.cuda(), table), (table,), dy.cuda())
     assert torch.equal(grad.cpu(), want)
     _done(nv)
+
+
+@pytest.mark.parametrize("kind,V,k", [(bf, 120001, 40), (f32, 60000, 7), (f32, 151936, 64), (bf, 400001, 20)])
+def test_top_logits_of_the_last_rows_of_a_cluster(nv, kind, V, k):
+    """Clusters of 2 to 8 blocks that have one to a few rows each, some of them rows that the readers pass over at once and the
+    selection takes long for: the last two rows of every cluster are handed over as all others are."""
+    from param_decomp_b200.ops.top_logits import top_logits
+
+    g = _gen(k)
+    z = torch.randn(161, V, generator=g)
+    z[1::5] = -math.inf
+    z[1::5, 3:3 + 2 * k:2] = 1.0
+    z = z.to(kind)
+    want = _top_reference(z, k, 1.0)
+    z = z.cuda()
+    for n in (2, 19, 37, 75, 76, 110, 149, 161):
+        first = top_logits(z[:n], k)
+        assert torch.equal(first.indices.cpu(), want[1][:n]) and torch.equal(first.values.cpu(), want[0][:n])
+        for _ in range(20):
+            assert all(torch.equal(a, b) for a, b in zip(first, top_logits(z[:n], k)))
+    _done(nv)
