@@ -230,7 +230,9 @@ Tensor grad_like(const Tensor& z, long long pitch_in) {
   const long long first = static_cast<long long>(reinterpret_cast<uintptr_t>(z.const_data_ptr()) % 16) / size;
   return at::empty({first + rows * pitch}, z.options()).as_strided({rows, V}, {pitch, 1}, first);
 }
-long long pitch_of(const Tensor& z) { return z.size(0) > 1 ? z.stride(0) : z.size(1); }
+// A single row's stride may be anything; where it is that of a padded matrix, the gradient is laid out like it too: products
+// that read it want rows of whole 16 bytes, of one row as of many.
+long long pitch_of(const Tensor& z) { return z.size(0) > 1 || z.stride(0) > z.size(1) ? z.stride(0) : z.size(1); }
 
 // z [rows, V], neighbouring columns; the results in the shape `lead`, which holds as many rows.
 std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& z, std::vector<int64_t> lead, int64_t k, double temperature,

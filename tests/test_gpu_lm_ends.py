@@ -891,3 +891,33 @@ def test_top_logits_of_the_last_rows_of_a_cluster(nv, kind, V, k):
         for _ in range(20):
             assert all(torch.equal(a, b) for a, b in zip(first, top_logits(z[:n], k)))
     _done(nv)
+
+
+@pytest.mark.parametrize("n,V", [(1, 1003), (257, 1003), (513, 2001), (2, 50277), (1, 50277)])
+def test_output_edge_with_a_chunk_of_one_position(nv, n, V):
+    """The last chunk has one row, of a width that is no whole number of 16 bytes: loss and gradient as in one chunk, whose
+    products add up in the same order for every row; and the gradient's rows lie like the logits'."""
+    from param_decomp_b200.ops import vocab_kl
+    from param_decomp_b200.ops.top_logits import top_kl_rows
+
+    g = _gen(n + V)
+    d, k, rows = 128, 16, 256 if n > 2 else 1
+    head = (torch.randn(V, d, generator=g) / d**0.5).to(bf).cuda()
+    hc, hm = (torch.randn(n, d, generator=g).to(bf).cuda() for _ in range(2))
+    results = []
+    for chunk in (rows, 1024):
+        top = vocab_kl.top_logits_from_hidden(hc, head, k, chunk)
+        leaf = hm.clone().requires_grad_(True)
+        loss = vocab_kl.top_kl_from_hidden(top, leaf, head, chunk)
+        results.append((loss.detach(), torch.autograd.grad(loss, (leaf,))[0]))
+    _done(nv)
+    lm = vocab_kl.padded_logits(hm, head)
+    # the two sums of n losses are in another order
+    assert abs(float(results[0][0]) - float(results[1][0])) <= 2 * (n + 2) * U * float(results[1][0].abs())
+    loss, dz = top_kl_rows(lm[n - 1:], top.indices[n - 1:], top.values[n - 1:], top.tail[n - 1:])
+    assert dz.stride(0) % 8 == lm.stride(0) % 8 == 0
+    want = dz.double().cpu() @ head.double().cpu() / n
+    size = dz.double().abs().cpu() @ head.double().abs().cpu() / n
+    for _, grad in results:  # sums of V products in fp32, rounded to bf16 once as the product is stored, once times the upstream 1
+        off = (grad[n - 1].double().cpu() - want[0]).abs()
+        assert bool((off <= V * U * size[0] + 1.01 * 2.0**-8 * want[0].abs()).all())
