@@ -497,11 +497,26 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
         sums = Row{{ref, part.x}, {ref, part.y}};
         if (!(part.x < 1e30f && part.y < 1e30f)) {  // the same in every thread: sums relative to true maxima
           GroupMax<T> all;
-          for (int g = begin; g < stop; g += 32) all.add(*reinterpret_cast<const uint4*>(smem + 16 * g));
+          bool nan = false;
+          for (int g = begin; g < stop; g += 32) {
+            const uint4 q = *reinterpret_cast<const uint4*>(smem + 16 * g);
+            all.add(q);
+            f32x2 v[kP];
+            pairs_of<T>(q, v);
+#pragma unroll
+            for (int j = 0; j < kP; ++j) {
+              const float2 x = unpack2(v[j]);
+              nan |= x.x != x.x || x.y != x.y;
+            }
+          }
           const float own = all.value();
           sums = Row{{own, 0.0f}, {-INFINITY, 0.0f}};
           if (mine >= 0 && mine_logit > -INFINITY) sums.top = MaxSum{mine_logit, term(mine_logit, mine_logit, c)};
-          if (moderate(own, c)) {
+          // a maximum passes NaN over: beside nothing but -inf it would be lost
+          if (mine_logit != mine_logit) sums.top.s = NAN;
+          if (nan) {
+            sums.rest.s = NAN;
+          } else if (moderate(own, c)) {
             const float k = -power_of(own, c);
             const f32x2 k2 = pk2(k, k);
             sums.rest.s = add_up([&](f32x2 v) { return fma2(v, c2, k2); });
@@ -542,7 +557,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
         const bool live = t.live;
         // the difference R - r from whichever side is small
         const float gap = t.r > 0.5f ? t.named - scaled(sums.top, all.m, c) / all.s : scaled(rest, all.m, c) / all.s - t.r;
-        float f = rest.s == 0.0f ? 0.0f : gap / rest.s * up;  // of an exponential as relative to rest.m
+        float f = rest.s == 0.0f ? 0.0f * all.s : gap / rest.s * up;  // of an exponential as relative to rest.m; NaN stays NaN
         T* const out = static_cast<T*>(call.dz) + static_cast<long long>(row) * call.ldo;  // column 0
         T* const slice_out = out + (rows.g0 * kE - shift);
         const int inner_first = rows.whole_first(shift) - rows.g0, inner_stop = rows.whole_stop(shift) - rows.g0;

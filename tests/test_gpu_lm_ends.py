@@ -921,3 +921,42 @@ def test_output_edge_with_a_chunk_of_one_position(nv, n, V):
     for _, grad in results:  # sums of V products in fp32, rounded to bf16 once as the product is stored, once times the upstream 1
         off = (grad[n - 1].double().cpu() - want[0]).abs()
         assert bool((off <= V * U * size[0] + 1.01 * 2.0**-8 * want[0].abs()).all())
+
+
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("V", [1, 7, 1001, 2001, 50277, 300001])
+def test_top_kl_of_rows_with_nan(nv, V, kind):
+    """One NaN among a row's logits (named, not named, the last column, beside nothing but -inf) makes the row's loss and all of
+    its gradient NaN, in every form, and no other row's."""
+    from param_decomp_b200.ops.top_logits import top_kl, top_kl_rows
+
+    g = _gen(V)
+    n, K, nan = 8, min(3, V), float("nan")
+    z = torch.randn(n, V, generator=g).to(kind)
+    idx = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(n)])
+    idx[1, 0] = 0
+    t, tail = torch.randn(n, K, generator=g), torch.randn(n, generator=g)
+    bad = z.clone()
+    bad[1, 0] = nan  # named
+    bad[3, V - 1] = nan
+    bad[4] = -math.inf
+    bad[4, V // 2] = nan
+    bad[5] = -math.inf
+    bad[5, V - 1] = nan
+    bad[6] = torch.finfo(kind).min
+    bad[6, V // 3] = nan
+    rows, rest = [1, 3, 4, 5, 6], [0, 2, 7]
+    at_odd = lambda a: torch.nn.functional.pad(a, (1, 2), value=9.0).cuda()[:, 1:V + 1]  # noqa: E731
+    for x, clean in ((bad.cuda(), z.cuda()), (at_odd(bad), at_odd(z))):  # addresses decide the order of sums
+        for tails in (tail.cuda(), None):
+            want, dz = top_kl_rows(clean, idx.cuda(), t.cuda(), tails)
+            loss, grad = top_kl_rows(x, idx.cuda(), t.cuda(), tails)
+            leaf = x.detach().requires_grad_(True)
+            auto = top_kl(leaf, idx.cuda(), t.cuda(), tails)
+            (auto_grad,) = torch.autograd.grad(auto.sum(), (leaf,))
+            for got, got_grad in ((loss, grad), (auto.detach(), auto_grad)):
+                assert bool(got[rows].isnan().all()) and bool(got_grad[rows].isnan().all())
+                assert torch.equal(got[rest], want[rest]) and torch.equal(got_grad[rest], dz[rest])
+                assert not bool(got[rest].isnan().any()) and not bool(got_grad[rest].isnan().any())
+            assert bool(top_kl_rows(x, idx.cuda(), t.cuda(), tails, want_grad=False)[0][rows].isnan().all())
+    _done(nv)
