@@ -601,9 +601,23 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 3) top_kl_kernel(const Call
             put([&](const uint4& w) { return words(w, [&](f32x2 v) { return fma2(v, c2, k2); }); });
           else
             put([&](const uint4& w) { return words(w, [&](f32x2 v) { return mul2(add2(v, neg), c2); }); });
+        } else if (const float power = power_of(rest.m, c); moderate(rest.m, c) && fabsf(power) > 512.0f) {
+          // far from zero the exponent has no bits left for the logarithm of f, which the next branch adds to it
+          const f32x2 k2 = pk2(-power, -power), f2 = pk2(f, f);
+          put([&](const uint4& w) {
+            f32x2 v[kP];
+            pairs_of<T>(w, v);
+            uint32_t o[kP];
+#pragma unroll
+            for (int j = 0; j < kP; ++j) {
+              const float2 x = unpack2(fma2(v[j], c2, k2));
+              o[j] = pack_bf16_2(mul2(pk2(ex2(x.x), ex2(x.y)), f2));
+            }
+            return make_uint4(o[0], o[1], o[2], o[3]);
+          });
         } else {
-          // f goes into the exponent, its sign into the word: what the exponent's rounding costs (below 2^-18 of the value)
-          // is far below the result's half step
+          // f goes into the exponent, its sign into the word: with it an exponent of up to 512 + 150 is rounded to 2^-15, so a
+          // value is off by 2^-15.5 of itself at most, by 2^-17.5 where the exponent is below 128: far below its half step
           const float lf = log2f(fabsf(f)), k = moderate(rest.m, c) ? lf - power_of(rest.m, c) : 0.0f;
           const f32x2 k2 = pk2(k, k), neg = pk2(-rest.m, -rest.m), lf2 = pk2(lf, lf);
           const uint32_t sign = f < 0.0f ? 0x80008000u : 0u;

@@ -960,3 +960,31 @@ def test_top_kl_of_rows_with_nan(nv, V, kind):
                 assert not bool(got[rest].isnan().any()) and not bool(got_grad[rest].isnan().any())
             assert bool(top_kl_rows(x, idx.cuda(), t.cuda(), tails, want_grad=False)[0][rows].isnan().all())
     _done(nv)
+
+
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("V", [1003, 50277, 120001])
+def test_top_kl_of_logits_far_from_zero(nv, V, kind):
+    """A large offset common to a row, or a small temperature, on either side: many logits share the largest values (two bf16
+    numbers that differ are hundreds apart there), and each one's gradient is as exact as around zero."""
+    from param_decomp_b200.ops.top_logits import top_kl, top_kl_rows
+
+    g = _gen(V)
+    n, K = 8, 5
+    z = torch.randint(-2, 1, (n, V), generator=g) * 1024.0
+    z += torch.tensor([99840.0, -99840.0, 45056.0, 300032.0, 0.0, -3e6, 6000.0, 500.0])[:, None]
+    z = z.to(kind)
+    idx = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(n)])
+    t, tail = torch.randn(n, K, generator=g), torch.randn(n, generator=g)
+    small = (torch.randint(-8, 1, (n, V), generator=g) * 0.25 + 45.0).to(kind)
+    for x, tails, T in ((z, tail, 1.0), (z, None, 1.0), (small, tail, 0.001), (-small, None, 0.01)):
+        loss, dz, lb, db = _kl_reference(x, idx, t, tails, T)
+        # an exponential below 2^-126 is zero; a gradient is at most 1 / T times its row's exponentials
+        db = db + 2.0**-126 / T
+        tails = None if tails is None else tails.cuda()
+        got, grad = top_kl_rows(x.cuda(), idx.cuda(), t.cuda(), tails, T)
+        _within(got, loss, lb, "loss")
+        _within(grad, dz, db, "dz")
+        leaf = x.cuda().requires_grad_(True)
+        _within(torch.autograd.grad(top_kl(leaf, idx.cuda(), t.cuda(), tails, T).sum(), (leaf,))[0], dz, db, "dz")
+    _done(nv)
