@@ -100,7 +100,8 @@ struct Teacher {  // of a row
   float edge[16];          // elements at the row's ragged ends, named ones as -inf
   float r, named;          // probability of the tail; of all slots
   int row;                 // or -1: there is no further one
-  float top, tail;         // largest of the logits over T and the tail; the tail
+  float most;              // largest of the logits, or 0 where none is above -inf
+  double most_at, tail_at; // it over T, and the tail, relative to the larger of the two
   bool live;
 };
 
@@ -148,17 +149,21 @@ __device__ void prepare(const Call& call, const RowSlice<T>& rows, long long row
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   nan = __any_sync(0xffffffffu, nan) || tail != tail;
-  const float inv_t = static_cast<float>(call.inv_t), over_t = m * inv_t, top = fmaxf(over_t, tail);
+  // The largest over T in 64 bits (in 32 a row of the type's lowest value would have no mass at T < 1), and rounded before
+  // anything is taken off it: what a fused multiply-add keeps of the product is 10^22 there.
+  const float inv_t = static_cast<float>(call.inv_t), most = m > -INFINITY ? m : 0.0f;
+  const double over_t = __dmul_rn(m, call.inv_t), top = fmax(over_t, static_cast<double>(tail));
   const bool live = nan || top > -INFINITY;
-  const float below = m > -INFINITY ? over_t - top : 0.0f;
+  const double most_at = m > -INFINITY ? over_t - top : 0.0, tail_at = tail == -INFINITY ? tail : tail - top;
+  const float below = static_cast<float>(most_at);
   float p[kPer], s = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    p[i] = v[i] == -INFINITY ? 0.0f : expf((v[i] - m) * inv_t + below);
+    p[i] = v[i] == -INFINITY ? 0.0f : expf((v[i] - most) * inv_t + below);
     s += p[i];
   }
   s = warp_sum(s);
-  const float rest = tail == -INFINITY ? 0.0f : expf(tail - top), total = live ? s + rest : 1.0f, share = 1.0f / total;
+  const float rest = tail == -INFINITY ? 0.0f : expf(static_cast<float>(tail_at)), total = live ? s + rest : 1.0f, share = 1.0f / total;
   // does a column come twice?
   bool twice = false;
 #pragma unroll
@@ -214,8 +219,9 @@ __device__ void prepare(const Call& call, const RowSlice<T>& rows, long long row
     t.r = live ? rest * share : 0.0f;
     t.named = live ? s * share : 0.0f;
     t.live = live;
-    t.top = top;
-    t.tail = tail;
+    t.most = most;
+    t.most_at = most_at;
+    t.tail_at = tail_at;
   }
 }
 
@@ -231,7 +237,7 @@ __device__ float loss_of(const Call& call, long long row, const Teacher& t, cons
   for (int k = lane; k < call.K; k += 32) {
     const int column = t.column[k];
     if (column == -1) continue;
-    const double a = value_at(call, row * call.K + k) * inv_t - t.top;
+    const double a = (static_cast<double>(value_at(call, row * call.K + k)) - t.most) * inv_t + t.most_at;
     const double b = (static_cast<double>(named[column >= 0 ? k : -2 - column]) - m) * own_inv_t;
     const double e = exp(a);
     if (!(static_cast<float>(e) == 0.0f)) {  // what is nothing in 32 bits costs nothing where the student's is -inf
@@ -247,7 +253,7 @@ __device__ float loss_of(const Call& call, long long row, const Teacher& t, cons
     weighted += __shfl_xor_sync(0xffffffffu, weighted, o);
     student += __shfl_xor_sync(0xffffffffu, student, o);
   }
-  const double a_rest = static_cast<double>(t.tail) - t.top, e_rest = t.r == 0.0f ? 0.0 : exp(a_rest);
+  const double a_rest = t.tail_at, e_rest = t.r == 0.0f ? 0.0 : exp(a_rest);
   const double log_rest = log_of(sums.rest, m, c), total = teacher + e_rest;
   const double log_ratio = log(exp(log_rest) + student) - log(total);
   double sum = 0.0;

@@ -144,12 +144,14 @@ def eager_top_kl(logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor |
                  temperature: float = 1.0) -> Tensor:
     used = indices >= 0
     columns = indices.long().clamp(min=0)
-    logq = torch.log_softmax((logits if logits.dtype == torch.float64 else logits.float()) / temperature, -1)
+    z = logits if logits.dtype == torch.float64 else logits.float()
+    top = z.detach().amax(-1, keepdim=True)  # taken off first: the type's lowest value over a temperature may leave fp32
+    logq = torch.log_softmax((z - torch.where(top.isfinite(), top, 0.0)) / temperature, -1)
     low = torch.full_like(logq[..., :1], float("-inf"))
-    teacher = torch.where(used, values.to(logq.dtype) / temperature, low)
-    teacher = torch.cat([teacher, low if tail is None else tail.to(logq.dtype).unsqueeze(-1)], -1)
+    teacher = torch.where(used, values.double() / temperature, low.double())
+    teacher = torch.cat([teacher, (low if tail is None else tail.unsqueeze(-1)).double()], -1)
     live = (teacher > float("-inf")).any(-1, keepdim=True)
-    logp = torch.log_softmax(torch.where(live, teacher, 0.0), -1)
+    logp = torch.log_softmax(torch.where(live, teacher, 0.0), -1).to(logq.dtype)
     # unused slots point at column 0 and must not name it
     named = torch.zeros_like(logq).scatter_add_(-1, columns, used.to(logq.dtype)) > 0
     others = logq.masked_fill(named, float("-inf"))

@@ -988,3 +988,50 @@ def test_top_kl_of_logits_far_from_zero(nv, V, kind):
         leaf = x.cuda().requires_grad_(True)
         _within(torch.autograd.grad(top_kl(leaf, idx.cuda(), t.cuda(), tails, T).sum(), (leaf,))[0], dz, db, "dz")
     _done(nv)
+
+
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("K,T", [(3, 0.7), (40, 0.001), (130, 0.5), (5, 2.0**-120), (5, 2.0**120)])
+def test_top_kl_of_a_teacher_past_the_range_of_fp32(nv, K, T, kind):
+    """A teacher's logits over the temperature leave fp32 on either side (all of them masked with the type's lowest value, among
+    others): the row counts like any other, with the same probabilities as around zero."""
+    from param_decomp_b200.ops.top_logits import top_kl_rows
+
+    g = _gen(K)
+    n, V = 7, 1003
+    most = torch.finfo(kind).max
+    z = (torch.randn(n, V, generator=g) * min(T, 1.0)).to(kind)
+    idx = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(n)])
+    t = torch.randn(n, K, generator=g)
+    t[1], t[2] = -most, most
+    t[3], t[3, 1:] = most, -most
+    t[4, 1:], t[5] = -most, most / 2
+    t[5, 0] = most
+    t, tail = t.to(kind), torch.randn(n, generator=g)
+    tail[1], tail[2] = -math.inf, -math.inf
+    for tails in (None, tail):
+        loss, dz, lb, db = _kl_reference(z, idx, t, tails, T)
+        got, grad = top_kl_rows(z.cuda(), idx.cuda(), t.cuda(), None if tails is None else tails.cuda(), T)
+        # what the reference's own 64 bits lose of a log probability of 1e38 and more beside one of zero is nothing here
+        fine = loss.isfinite() & (loss.abs() < 1e30)
+        assert bool(fine[1:3].all()) and bool(fine.any())
+        _within(got[fine.cuda()], loss[fine], lb[fine], "loss")
+        # an exponential below 2^-126, or a gradient, may be zero
+        _within(grad, dz, db + 2.0**-126 * (1.0 + 1.0 / T), "dz")
+    _done(nv)
+
+
+def test_top_kl_of_a_teacher_with_nan(nv):
+    """A NaN in a used slot or in the tail makes the row's loss and all of its gradient NaN, one in an unused slot nothing."""
+    from param_decomp_b200.ops.top_logits import top_kl_rows
+
+    g = _gen(12)
+    z, t, tail = torch.randn(5, 600, generator=g), torch.randn(5, 3, generator=g), torch.randn(5, generator=g)
+    idx = torch.stack([torch.randperm(600, generator=g)[:3] for _ in range(5)])
+    idx[3, 1] = -1
+    want, dz = top_kl_rows(z.cuda(), idx.cuda(), t.cuda(), tail.cuda())
+    t[1, 2], t[3, 1], t[4], tail[2], tail[4] = float("nan"), float("nan"), -math.inf, float("nan"), float("nan")
+    loss, grad = top_kl_rows(z.cuda(), idx.cuda(), t.cuda(), tail.cuda())
+    assert bool(loss[[1, 2, 4]].isnan().all()) and bool(grad[[1, 2, 4]].isnan().all())
+    assert torch.equal(loss[[0, 3]], want[[0, 3]]) and torch.equal(grad[[0, 3]], dz[[0, 3]])
+    _done(nv)

@@ -185,3 +185,13 @@ def test_a_missing_extension_is_said_aloud(monkeypatch, tmp_path):
     monkeypatch.setattr(native, "_autograd", None)
     with pytest.raises(NativeError, match="ops.build"):
         native.autograd()
+
+
+@pytest.mark.parametrize("T", [0.5, 0.7, 1.0, 3.0])
+def test_eager_top_kl_of_rows_of_the_lowest_value(T):
+    """Teacher or student masked in every place with the type's lowest value: a level row, whatever the temperature makes of it."""
+    low = torch.finfo(F32).min
+    z, t, idx = torch.zeros(3, 4), torch.zeros(3, 2), torch.tensor([[0, 2]] * 3)
+    z[1], t[2] = low, low
+    loss = eager_top_kl(z, idx, t, None, T)
+    torch.testing.assert_close(loss, torch.full((3,), math.log(2.0)))
