@@ -65,8 +65,8 @@ def _check_logits(what: str, logits: Tensor, temperature: float) -> None:
         raise ValueError(f"{what}: logits of shape {tuple(logits.shape)}")
     if logits.numel() // logits.shape[-1] >= 1 << 28:
         raise ValueError(f"{what}: fewer than 2^28 rows")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"{what}: the temperature is positive, not {temperature}")
+    if not 2.0**-120 <= temperature <= 2.0**120:  # its inverse is taken in fp32
+        raise ValueError(f"{what}: a temperature from 2^-120 to 2^120, not {temperature}")
 
 
 def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:

@@ -187,6 +187,15 @@ def test_a_missing_extension_is_said_aloud(monkeypatch, tmp_path):
         native.autograd()
 
 
+@pytest.mark.parametrize("T", [2.0**-121, 2.0**121, 1e-300, 1e300])
+def test_temperatures_whose_inverse_leaves_fp32_are_refused(T):
+    z = torch.zeros(2, 8)
+    for call in (lambda: top_logits(z, 1, T), lambda: top_kl(z, _IDX, torch.zeros(2, 3), None, T),
+                 lambda: top_kl_rows(z, _IDX, torch.zeros(2, 3), None, T)):
+        with pytest.raises(ValueError, match="temperature"):
+            call()
+
+
 @pytest.mark.parametrize("T", [0.5, 0.7, 1.0, 3.0])
 def test_eager_top_kl_of_rows_of_the_lowest_value(T):
     """Teacher or student masked in every place with the type's lowest value: a level row, whatever the temperature makes of it."""
