@@ -46,7 +46,7 @@ def ce_and_kl(ctx: StepContext, state: TrainState, batch: Any, rounding_threshol
     ce: dict[str, float] = {}
     for name, masks in variants.items():
         res = model.masked_forward(weights, batch, masks)
-        out[f"kl/{name}"] = float(model.recon_loss(clean, res))
+        out[f"kl/{name}"] = float(model.output_kl(clean, res))  # over the whole vocabulary at every output edge
         ce[name] = float(model.ce_loss(res, batch.tokens))
         out[f"ce/{name}"] = ce[name]
     for name in variants:

@@ -439,24 +439,32 @@ class TransformerDecomposedModel:
         return {}  # streamed output edge: no `[positions, vocab]` tensor is ever kept
 
     def recon_loss(self, clean: ForwardResult, masked: ForwardResult) -> Tensor:
-        """Mean over positions of `KL(softmax(clean logits) || softmax(masked logits))`.
+        """The loss of the output edge: `output_kl`, or with `output_edge: top_logits` the divergence over the clean side's
+        largest logits and the rest as one event."""
+        if getattr(self, "n_top_logits", None) is None:
+            return self.output_kl(clean, masked)
+        hm = masked.output.reshape(-1, masked.output.shape[-1])
+        top = clean.aux["clean_stats"]["top"]
+        if self.backend == "fused_sm100" and hm.is_cuda:
+            from param_decomp_b200.ops import vocab_kl
+
+            return vocab_kl.top_kl_from_hidden(top, hm, self.head_weight(), self.kl_token_chunk)
+        return eager_top_kl_from_hidden(top, hm, self.head_weight(), self.kl_token_chunk)
+
+    def output_kl(self, clean: ForwardResult, masked: ForwardResult) -> Tensor:
+        """Mean over positions of `KL(softmax(clean logits) || softmax(masked logits))`, whatever the output edge keeps.
         Logits are never held for the whole batch: positions are processed in chunks and each chunk
         is recomputed in the backward pass (`ops/vocab_kl.py` is the fused kernel of this loss)."""
         hc = clean.output.reshape(-1, clean.output.shape[-1])
         hm = masked.output.reshape(-1, masked.output.shape[-1])
-        if getattr(self, "n_top_logits", None) is not None:
-            top = clean.aux["clean_stats"]["top"]
-            if self.backend == "fused_sm100" and hm.is_cuda:
-                from param_decomp_b200.ops import vocab_kl
-
-                return vocab_kl.top_kl_from_hidden(top, hm, self.head_weight(), self.kl_token_chunk)
-            return eager_top_kl_from_hidden(top, hm, self.head_weight(), self.kl_token_chunk)
         if self.backend == "fused_sm100" and hm.is_cuda:
             from param_decomp_b200.ops import vocab_kl
 
             if self.n_vocab_chunks is not None:  # `output_edge: streamed`: chunks of positions, logits never whole
                 rows = (-(-hm.shape[0] // self.n_vocab_chunks) + 127) // 128 * 128
                 return vocab_kl.kl_from_hidden_streamed(hc, hm, self.head_weight(), rows)
+            if getattr(self, "n_top_logits", None) is not None:
+                return vocab_kl.kl_from_hidden_streamed(hc, hm, self.head_weight(), self.kl_token_chunk)
             return vocab_kl.kl_from_hidden(clean.aux["clean_stats"]["logits"], hm, self.head_weight())
         return chunked_kl_from_hidden(hc, hm, self.head_weight(), self.kl_token_chunk)
 

@@ -1035,3 +1035,28 @@ def test_top_kl_of_a_teacher_with_nan(nv):
     assert bool(loss[[1, 2, 4]].isnan().all()) and bool(grad[[1, 2, 4]].isnan().all())
     assert torch.equal(loss[[0, 3]], want[[0, 3]]) and torch.equal(grad[[0, 3]], dz[[0, 3]])
     _done(nv)
+
+
+@pytest.mark.parametrize("n", [700, 257, 1])
+def test_evaluated_divergence_with_the_top_logits_edge_on_the_fused_backend(nv, n):
+    """The divergence over the whole vocabulary, in chunks, is that of the materialised edge; the edge's loss is not above it."""
+    from types import SimpleNamespace
+
+    from param_decomp_b200.config.experiments import TransformerArchConfig
+    from param_decomp_b200.models import transformer as tf
+
+    arch = TransformerArchConfig(family="glu_transformer", n_layer=1, d_model=128, n_head=2, d_ff=128, vocab_size=1003, max_seq_len=n)
+    w = {k: v.to(bf).cuda() for k, v in tf.random_init_weights(arch, 0, f32).items()}
+    g = _gen(n)
+    hc, hm = ((torch.randn(1, n, 128, generator=g) * 4).to(bf).cuda() for _ in range(2))
+    values = []
+    for n_top in (None, 16):
+        model = tf.TransformerDecomposedModel(arch, w, {}, backend="fused_sm100", n_top_logits=n_top, kl_token_chunk=256)
+        clean, masked = SimpleNamespace(output=hc, aux={"clean_stats": model._clean_logit_stats(hc)}), SimpleNamespace(output=hm)
+        with torch.no_grad():
+            values.append((float(model.output_kl(clean, masked)), float(model.recon_loss(clean, masked))))
+    _done(nv)
+    assert values[0][0] == values[0][1]
+    # the same rows' values, added in another order
+    assert abs(values[1][0] - values[0][0]) <= 2 * (n + 2) * U * values[0][0]
+    assert 0 < values[1][1] <= values[1][0]

@@ -1,6 +1,7 @@
 """Layer norm, token embedding, top logits and the distillation loss without a GPU: what their entry points refuse, and the
 plain statements of the last two."""
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -204,3 +205,28 @@ def test_eager_top_kl_of_rows_of_the_lowest_value(T):
     z[1], t[2] = low, low
     loss = eager_top_kl(z, idx, t, None, T)
     torch.testing.assert_close(loss, torch.full((3,), math.log(2.0)))
+
+
+def test_evaluated_divergences_do_not_depend_on_the_output_edge():
+    """`kl/<variant>` is the divergence over the whole vocabulary; the loss of the edge is its own."""
+    from param_decomp_b200.config.experiments import LMExperimentConfig
+    from param_decomp_b200.core.objective import build_objective
+    from param_decomp_b200.core.run import init_train_state
+    from param_decomp_b200.core.train import StepContext
+    from param_decomp_b200.evals.lm import ce_and_kl
+    from param_decomp_b200.experiments.lm.build import build_lm_run
+
+    results, edge_loss = [], []
+    for edge in ({"kind": "materialized"}, {"kind": "top_logits", "k": 3}):
+        cfg = LMExperimentConfig.model_validate(_lm_config(edge))
+        run = build_lm_run(cfg, None, "cpu")
+        obj = build_objective(cfg.pd)
+        ctx = StepContext.build(run.model, obj, cfg.pd, lazy_masks=False)
+        state = init_train_state(run.model, run.ci_fn, cfg.pd, obj, torch.device("cpu"), cfg.pd.batch_size, cfg.data.seq_len)
+        batch = run.sample_eval(0)
+        results.append(ce_and_kl(ctx, state, batch))
+        clean = run.model.clean_forward(batch)
+        half = SimpleNamespace(output=clean.output * 0.5)
+        edge_loss.append(float(run.model.recon_loss(clean, half)))
+    assert results[0] == results[1] and results[0]["kl/zero_masked"] > 0
+    assert 0 < edge_loss[1] < edge_loss[0]
