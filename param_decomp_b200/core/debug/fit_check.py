@@ -37,6 +37,7 @@ class FitReport:
 
 def estimate(cfg: Any, n_gpus: int = 1, pool_gib: float = 170.0) -> FitReport:
     from param_decomp_b200.core.objective import build_objective
+    from param_decomp_b200.models.transformer import KL_TOKEN_CHUNK
 
     arch = cfg.target.spec.arch if hasattr(cfg.target.spec, "arch") else None
     assert arch is not None, "the fit check needs an inline architecture (random_init target) or a resolved one"
@@ -91,14 +92,21 @@ def estimate(cfg: Any, n_gpus: int = 1, pool_gib: float = 170.0) -> FitReport:
               for din, dout, C, mult in sites)
     ci_act = sum(rows * ((C if mult == 1.0 else C // E * k) * 2 * 3 + ci_hidden * 2) for _, _, C, mult in sites)
     resid = rows * d * 2 * L * 6
-    logits = rows * ((V + 63) // 64 * 64) * 2
+    row_of_logits = (V + 63) // 64 * 64 * 2
+    edge = cfg.target.output_edge
+    if edge.kind == "top_logits":  # a chunk's masked logits and gradient beside the last chunk's, clean top logits of all rows
+        logits = 3 * min(rows, KL_TOKEN_CHUNK) * row_of_logits + rows * (edge.k * (2 + 4) + 4)
+        logits_of = "logit buffers (chunks, top logits)"
+    else:
+        logits = 3 * rows * row_of_logits
+        logits_of = "logit buffers (clean, masked, gradient)"
     detail = dict(persistent)
     detail[f"site activations x {n_draws} draws"] = act * n_draws / G
     detail["CI function activations"] = ci_act / G
     detail["residual stream / block activations"] = resid * (1 + n_draws) / G
-    detail["logit buffers (clean, masked, gradient)"] = 3 * logits / G
+    detail[logits_of] = logits / G
     total = sum(detail.values()) * 1.15
-    return FitReport(sum(persistent.values()), (act * n_draws + ci_act + resid * (1 + n_draws)) / G, 3 * logits / G, total,
+    return FitReport(sum(persistent.values()), (act * n_draws + ci_act + resid * (1 + n_draws)) / G, logits / G, total,
                      pool_gib, total <= pool_gib, detail)
 
 

@@ -130,12 +130,15 @@ def alignment_for(arch: TransformerArchConfig, kind: str) -> NonlinearityAlignme
     return None
 
 
+KL_TOKEN_CHUNK = 8192  # positions whose logits exist at a time, where logits are not kept whole
+
+
 class TransformerDecomposedModel:
     has_position_axis = True
 
     def __init__(self, arch: TransformerArchConfig, weights: dict[str, Tensor], site_cs: dict[str, int],
                  backend: str = "eager_torch", attention: str = "flash", n_vocab_chunks: int | None = None,
-                 kl_token_chunk: int = 8192, n_top_logits: int | None = None, train_kernels: bool = False) -> None:
+                 kl_token_chunk: int = KL_TOKEN_CHUNK, n_top_logits: int | None = None, train_kernels: bool = False) -> None:
         assert arch.family in ("glu_transformer", "simple_mlp", "moe"), arch.family
         self.arch = arch
         self.w = weights

@@ -2,7 +2,7 @@
 import torch
 import torch.distributed as dist
 
-from param_decomp_b200.config.experiments import LMExperimentConfig
+from param_decomp_b200.config.experiments import LMExperimentConfig, MaterializedOutputEdgeConfig, TopLogitsOutputEdgeConfig
 from param_decomp_b200.core.debug import fit_check, memory_ledger
 from param_decomp_b200.core.debug.census import census
 
@@ -22,6 +22,25 @@ def test_fit_check_orders_configs():
         update={"fsdp": 8, "tp": 1})})})
     assert not fit_check.estimate(flat, 8).fits
     assert "TOTAL" in str(one)
+
+
+def test_fit_check_of_the_top_logits_edge():
+    """The clean side is k pairs a position, the masked side a chunk of positions: less than whole logits from a chunk's rows on,
+    and beyond that only the pairs grow with the batch."""
+    cfg = LMExperimentConfig.from_file("param_decomp_b200/experiments/configs/lm_llama4l_c4096.yaml")
+
+    def edge_gib(edge, rows):
+        target = cfg.target.model_copy(update={"output_edge": edge})
+        pd = cfg.pd.model_copy(update={"batch_size": rows // cfg.data.seq_len})
+        return fit_check.estimate(cfg.model_copy(update={"target": target, "pd": pd}), 1).output_edge_gib
+
+    top, whole = TopLogitsOutputEdgeConfig(k=64), MaterializedOutputEdgeConfig()
+    V = cfg.target.spec.arch.vocab_size
+    pairs = 64 * 6 + 4
+    chunk = 3 * 8192 * ((V + 63) // 64 * 64) * 2
+    for rows in (8192, 65536):
+        assert abs(edge_gib(top, rows) * 2**30 - (chunk + rows * pairs)) < 1
+        assert abs(edge_gib(whole, rows) * 2**30 - chunk / 8192 * rows) < 1
 
 
 def test_memory_ledger_roundtrip(tmp_path):
