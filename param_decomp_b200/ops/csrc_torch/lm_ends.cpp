@@ -95,10 +95,11 @@ struct LayerNormBackward : Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(3);
-    const Tensor xs = x.unpack(), ws = w.unpack();
+    const Tensor x_back = x.unpack(), w_back = w.unpack();
     Tensor dx, dw, db;
     {
       at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor xs = dense(x_back), ws = dense(w_back);  // what a saved-tensor hook gives back may lie otherwise
       const int d = static_cast<int>(xs.size(-1));
       const long long rows = xs.numel() / d;
       const auto p_options = xs.options().dtype(p_type);
@@ -234,6 +235,11 @@ Tensor grad_like(const Tensor& z, long long pitch_in) {
 // that read it want rows of whole 16 bytes, of one row as of many.
 long long pitch_of(const Tensor& z) { return z.size(0) > 1 || z.stride(0) > z.size(1) ? z.stride(0) : z.size(1); }
 
+// Neighbouring columns, rows that do not overlap.
+bool in_rows(const Tensor& z) {
+  return (z.size(1) == 1 || z.stride(1) == 1) && (z.size(0) <= 1 || z.stride(0) >= z.size(1));
+}
+
 // z [rows, V], neighbouring columns; the results in the shape `lead`, which holds as many rows.
 std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& z, std::vector<int64_t> lead, int64_t k, double temperature,
                                               int64_t status) {
@@ -285,11 +291,13 @@ struct TopKLBackward : Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(1);
-    const Tensor zs = z.unpack();
-    const Teacher t{indices.unpack(), values.unpack(), tail.unpack(), temperature, status, refused};
+    const Tensor z_back = z.unpack(), indices_back = indices.unpack(), values_back = values.unpack(), tail_back = tail.unpack();
     Tensor dz;
     {
       at::AutoDispatchBelowADInplaceOrView below;
+      // what a saved-tensor hook gives back may lie otherwise than what was saved
+      const Tensor zs = in_rows(z_back) ? z_back : z_back.contiguous();
+      const Teacher t{dense(indices_back), dense(values_back), dense(tail_back), temperature, status, refused};
       dz = grad_like(zs, pitch_of(zs));
       run_top_kl(zs, t, Tensor(), dz, grads[0].contiguous(), Tensor(), sums);
     }

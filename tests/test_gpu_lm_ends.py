@@ -1060,3 +1060,35 @@ def test_evaluated_divergence_with_the_top_logits_edge_on_the_fused_backend(nv, 
     # the same rows' values, added in another order
     assert abs(values[1][0] - values[0][0]) <= 2 * (n + 2) * U * values[0][0]
     assert 0 < values[1][1] <= values[1][0]
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_hooks_on_the_nodes(nv, which):
+    """Tensors saved on the host, or given back in another layout; recomputation of a checkpoint; hooks that see and change
+    gradients: each with the gradients that the formula gives."""
+    from torch.utils.checkpoint import checkpoint
+
+    _, leaves, f = _differentiable()[which]
+    up = torch.rand(f(*leaves).shape, generator=_gen(2)).cuda()
+    want = torch.autograd.grad(f(*leaves), leaves, up)
+    turned = lambda t: t if t.dim() < 2 else t.t().contiguous().t()  # noqa: E731  (the same values by columns)
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t, turned)):
+        with hooks:
+            y = f(*leaves)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, up), want))
+    y = checkpoint(f, *leaves, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, up), want))
+    seen = []
+    y = f(*leaves)
+    y.register_hook(lambda g: 2.0 * g)
+    mids = [p * 1.0 for p in leaves]
+    z = f(*mids)
+    for m in mids:
+        m.register_hook(lambda g: seen.append(g.clone()))
+    assert all(torch.equal(a, 2.0 * b) for a, b in zip(torch.autograd.grad(y, leaves, up), want))
+    grads = torch.autograd.grad(z, leaves, up)
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+    assert len(seen) == len(leaves) and all(any(torch.equal(a, b) for a in seen if a.shape == b.shape) for b in want)
+    with torch.autograd.detect_anomaly():
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(f(*leaves), leaves, up), want))
+    _done(nv)
