@@ -1092,3 +1092,127 @@ def test_hooks_on_the_nodes(nv, which):
     with torch.autograd.detect_anomaly():
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(f(*leaves), leaves, up), want))
     _done(nv)
+
+
+@pytest.mark.parametrize("table_type,out_type", [(bf, bf), (f32, f32), (f32, bf)])
+@pytest.mark.parametrize("n,V,d", [(30000, 1, 24), (30000, 3, 33), (70000, 100, 40), (40000, 300, 264), (200000, 450, 8), (25000, 700, 515),
+                                   (50000, 189441, 16)])
+def test_embedding_gradient_of_blocks_with_many_tokens(nv, n, V, d, table_type, out_type):
+    """More tokens of one block's ids than it sorts on chip (4096), more in a warp's part than it notes (128), beside ids of the
+    same block with one token, a few and a slab's worth of them: against whole numbers, whose sums are exact."""
+    from param_decomp_b200.ops.embedding import embedding
+
+    g = _gen(n + V)
+    blocks = -(-V // -(-V // max(148, -(-V // 1280))))  # ids v, v + blocks, .. belong to block v % blocks
+    tokens = torch.zeros(n, dtype=torch.int64)
+    tokens[torch.rand(n, generator=g) < 0.4] = min(1, V - 1)
+    where = torch.randperm(n, generator=g)
+    at = 0
+    for first in (0, 1):  # the two full blocks: neighbours of their id with 1, 2, 31, 32, 33 and 100 tokens
+        for i, count in enumerate((1, 2, 31, 32, 33, 100), start=1):
+            if first + i * blocks < V:
+                tokens[where[at:at + count]] = first + i * blocks
+                at += count
+    some = where[at:at + n // 8]
+    tokens[some] = torch.randint(0, V, (len(some),), generator=g)
+    assert int(torch.bincount(tokens % blocks).max()) > 4096
+    dy = torch.randint(-2, 3, (n, d), generator=g).float()
+    want = torch.zeros(V, d, dtype=torch.float64).index_add_(0, tokens, dy.double())
+    table = torch.zeros(V, d, dtype=table_type).cuda().requires_grad_(True)
+    for ids in (tokens, torch.sort(tokens)[0], torch.sort(tokens, descending=True)[0]):
+        order = torch.sort(tokens, stable=True, descending=bool(ids[0] > ids[-1]))[1] if ids is not tokens else torch.arange(n)
+        y = embedding(ids.cuda(), table, 1.0, out_dtype=out_type)
+        (grad,) = torch.autograd.grad(y, (table,), dy[order].to(out_type).cuda())
+        # sums of whole numbers below 2^24 are exact; the result is rounded once
+        assert torch.equal(grad.cpu(), want.to(table_type))
+    _done(nv)
+
+
+def test_embedding_gradient_of_a_full_block_in_64_bits(nv):
+    """The same paths with values that round: each row's sum to within the roundings of as many additions."""
+    from param_decomp_b200.ops.embedding import embedding
+
+    g = _gen(31)
+    n, V, d = 30000, 500, 136
+    tokens, dy = _zipf(n, V, g), torch.randn(n, d, generator=g)
+    tokens[::3] = 7
+    table = torch.zeros(V, d).cuda().requires_grad_(True)
+    (grad,) = torch.autograd.grad(embedding(tokens.cuda(), table), (table,), dy.cuda())
+    want = torch.zeros(V, d, dtype=torch.float64).index_add_(0, tokens, dy.double())
+    sizes = torch.zeros(V, d, dtype=torch.float64).index_add_(0, tokens, dy.double().abs())
+    _within(grad, want, (torch.bincount(tokens, minlength=V).double()[:, None] + 2) * U * sizes, "dE")
+    _done(nv)
+
+
+@pytest.mark.parametrize("kind", [bf, f32])
+@pytest.mark.parametrize("rows,d", [(32771, 768), (70001, 256), (5003, 4096), (2003, 8192), (2005, 12288), (9001, 2048), (33003, 264),
+                                    (20001, 500), (4001, 2047)])
+def test_layer_norm_over_many_handfuls(nv, rows, d, kind):
+    """Every group of warps walks more handfuls of rows than shared memory holds at a time, up to about twenty (the last ragged): its
+    places are filled anew, the weights' sums run on over all of them."""
+    from param_decomp_b200.ops.elementwise import layer_norm
+
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn(rows, d, generator=g, device="cuda") * 2 + 1).to(kind)
+    x[rows // 2:] *= 3.0  # rows differ: one that is read in another's place shows
+    w, b = (1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(kind), torch.randn(d, generator=g, device="cuda").to(kind)
+    dy = torch.randn(rows, d, generator=g, device="cuda").to(kind)
+    want, bounds = _norm_reference(x, w, b, dy, 1e-5)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = layer_norm(*leaves, 1e-5)
+    grads = torch.autograd.grad(y, leaves, dy)
+    _done(nv)
+    for name, got in zip(("y", "dx", "dw", "db"), (y, *grads)):
+        _within(got, want[name], bounds[name], name)
+    assert all(torch.equal(a, c) for a, c in zip(grads, torch.autograd.grad(layer_norm(*leaves, 1e-5), leaves, dy)))
+    (alone,) = torch.autograd.grad(layer_norm(leaves[0], leaves[1].detach(), leaves[2].detach(), 1e-5), (leaves[0],), dy)
+    assert torch.equal(alone, grads[0])
+
+
+def test_hybrid_target_with_the_top_logits_edge_fused_against_eager(nv):
+    """Gated delta rule, attention and routed experts through three steps with the edge, on both backends; and what evaluations
+    call the divergence, with chunks."""
+    from types import SimpleNamespace
+
+    from param_decomp_b200.config.experiments import LMExperimentConfig
+    from param_decomp_b200.core.objective import build_objective
+    from param_decomp_b200.core.run import init_train_state
+    from param_decomp_b200.core.train import StepContext, train_step
+    from param_decomp_b200.experiments.lm.build import build_lm_run
+    from param_decomp_b200.models import qwen35
+
+    arch = dict(family="qwen35_moe", n_layer=2, d_model=64, n_head=4, n_kv_head=2, head_dim=64, d_ff=64, vocab_size=509,
+                max_seq_len=64, n_experts=4, experts_per_token=2, full_attention_interval=2, partial_rotary_factor=0.5,
+                linear_num_key_heads=2, linear_key_head_dim=64, linear_num_value_heads=4, linear_value_head_dim=64,
+                linear_conv_kernel_dim=4, shared_expert_intermediate=64)
+    raw = LMExperimentConfig.from_file("param_decomp_b200/experiments/configs/lm_moe4l_e42.yaml").model_dump(mode="json")
+    raw["target"]["spec"]["arch"] = arch
+    raw["target"]["output_edge"] = {"kind": "top_logits", "k": 32}
+    raw["decomposition"]["sites"] = {"kind": "qwen36_moe", "layers": {"kind": "all"},
+                                     "cs": {k: (128 if k.startswith("experts_") else 64) for k in qwen35.KIND_ORDER}}
+    raw["decomposition"]["ci"] = {"type": "layerwise_mlp", "hidden_dims": [64]}
+    raw["data"]["seq_len"] = 64
+    raw["pd"]["batch_size"] = 4
+    dev = torch.device("cuda", 0)
+    res = {}
+    for backend in ("eager_torch", "fused_sm100"):
+        raw["runtime"]["backend"] = backend
+        cfg = LMExperimentConfig.model_validate(raw)
+        run = build_lm_run(cfg, None, dev)
+        assert run.model.n_top_logits == 32
+        run.model.kl_token_chunk = 255  # the last chunk has one position
+        obj = build_objective(cfg.pd)
+        fused = backend == "fused_sm100"
+        ctx = StepContext.build(run.model, obj, cfg.pd, lazy_masks=fused)
+        st = init_train_state(run.model, run.ci_fn, cfg.pd, obj, dev, cfg.pd.batch_size, cfg.data.seq_len, use_fused_optim=fused)
+        for s in range(3):
+            m = train_step(ctx, st, run.sample_train(s))
+        with torch.no_grad():
+            clean = run.model.clean_forward(run.sample_eval(0))
+            whole = run.model.output_kl(clean, SimpleNamespace(output=clean.output * 0.5))
+        _done(nv)
+        res[backend] = {k: float(v) for k, v in m.items()} | {"kl": float(whole)}
+    # bf16 weights and activations on both sides, through three updates: a few roundings of 2^-8 each
+    for k in ("loss/total", "loss/FaithfulnessLoss", "loss/StochasticReconLoss", "loss/ImportanceMinimalityLoss", "kl"):
+        a, b = res["eager_torch"][k], res["fused_sm100"][k]
+        assert abs(a - b) <= 5e-2 * abs(a) + 1e-6, (k, a, b)

@@ -230,3 +230,43 @@ def test_evaluated_divergences_do_not_depend_on_the_output_edge():
         edge_loss.append(float(run.model.recon_loss(clean, half)))
     assert results[0] == results[1] and results[0]["kl/zero_masked"] > 0
     assert 0 < edge_loss[1] < edge_loss[0]
+
+
+@pytest.mark.parametrize("family", ["moe", "qwen35_moe"])
+def test_output_edge_of_top_logits_on_mixture_and_hybrid_targets(family):
+    """The edge is wired: a step trains with it, its loss is the divergence from the clean side's top logits, and with k above
+    the vocabulary's size that over the whole vocabulary."""
+    from param_decomp_b200.config.experiments import LMExperimentConfig
+    from param_decomp_b200.core.objective import build_objective
+    from param_decomp_b200.core.run import init_train_state
+    from param_decomp_b200.core.train import StepContext, train_step
+    from param_decomp_b200.experiments.lm.build import build_lm_run
+    from param_decomp_b200.models import qwen35
+    from tests.test_moe import moe_cfg
+    from tests.test_qwen35 import _config
+
+    cs = {k: (12 if k.startswith("experts_") else 8) for k in qwen35.KIND_ORDER}
+    raw = (moe_cfg() if family == "moe" else _config(cs)).model_dump(mode="json")
+    raw["cadence"] = {"checkpointing": {"kind": "none"}}
+    for k in (5, 200):
+        raw["target"]["output_edge"] = {"kind": "top_logits", "k": k}
+        cfg = LMExperimentConfig.model_validate(raw)
+        run = build_lm_run(cfg, None, "cpu")
+        assert run.model.n_top_logits == k
+        obj = build_objective(cfg.pd)
+        ctx = StepContext.build(run.model, obj, cfg.pd, lazy_masks=True)
+        state = init_train_state(run.model, run.ci_fn, cfg.pd, obj, torch.device("cpu"), cfg.pd.batch_size, cfg.data.seq_len)
+        assert math.isfinite(float(train_step(ctx, state, run.sample_train(0))["loss/total"]))
+        with torch.no_grad():
+            clean = run.model.clean_forward(run.sample_eval(0))
+        masked = SimpleNamespace(output=clean.output * 0.5)
+        loss, whole = run.model.recon_loss(clean, masked), run.model.output_kl(clean, masked)
+        logits = run.model.logits(clean.output).flatten(0, -2)
+        top = eager_top_logits(logits, min(k, logits.shape[-1]))
+        assert top.values.shape == clean.aux["clean_stats"]["top"].values.shape
+        want = eager_top_kl(run.model.logits(masked.output).flatten(0, -2), top.indices, top.values, top.tail).mean()
+        torch.testing.assert_close(loss, want)
+        if k == 200:
+            torch.testing.assert_close(loss, whole)
+        else:
+            assert 0 < float(loss) < float(whole)
