@@ -2,7 +2,7 @@
 // Both are bound by HBM: the lookup reads a table row and writes an output row a token, the gradient reads the tokens'
 // rows once and writes every row of the table (most of them zeros).
 //
-// The gradient sums each row in fp32 over its tokens in ascending order and rounds once, with two launches and no float
+// The gradient sums each row in fp32 over its tokens in a fixed order and rounds once, with two launches and no float
 // atomics. First kernel: ids are dealt to the blocks like cards (id v is the v / blocks -th of block v % blocks), since
 // vocabularies hold frequent tokens together: with a span of neighbouring ids a block, 32,768 tokens over 50,277 ids in
 // order of frequency took 270 us, so 56 (58 with ids in no order, either way). A block's 32 warps read all tokens (from L2,

@@ -4,7 +4,7 @@
 //   loss = sum_k p_k (log p_k - log q_{i_k}) + r (log r - log R)
 //   dloss / dz_j = (q_j - p_j) / T at a named column (p summed where a column is named twice), q_j (1 - r / R) / T elsewhere
 // Without a tail r = 0: K = 1 is the cross entropy of one target. A slot with a negative column is unused; a row whose
-// teacher has no mass counts zero with a zero gradient.
+// teacher has no mass counts zero with a zero gradient. The loss counts the slots of a column that is named twice one by one.
 //
 // Rows are held in the shared memory of a cluster of 1 to 8 blocks (`row_slice.cuh`) and read there for the sums and again
 // for the gradient, so a logit crosses HBM once, its gradient once: bound by HBM, beside two exponentials a logit (16 lanes

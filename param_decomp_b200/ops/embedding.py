@@ -1,8 +1,10 @@
 """Token embedding with scaling, and the gradient of its table (`csrc/embedding.cu`).
 
 `y[n] = scale * table[tokens[n]]`; the gradient of row `v` is `scale` times the sum of `dy` over the positions that hold
-token `v`, taken in fp32 in ascending order of position (positions sorted by token), so it does not change from run to
-run, and rounded once to the table's type. Every row of the gradient is written: rows of unseen tokens are zero.
+token `v`, taken in fp32 and rounded once to the table's type. Positions are sorted by token: up to 32 of a token are added
+in ascending order, more by groups of threads over 32 places of the sorted order each, whose sums are added in their order;
+either way the order depends on the sizes and the tokens alone, so the gradient does not change from run to run. Every row of
+it is written: rows of unseen tokens are zero.
 """
 
 from __future__ import annotations

@@ -71,7 +71,8 @@ def _check_logits(what: str, logits: Tensor, temperature: float) -> None:
 
 def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     """The `k` largest of each row of `logits [..., V]` (bf16 or fp32, `1 <= k <= min(V, 256)`), their columns and the
-    logsumexp of `logits / temperature` over the rest of the row. NaN counts as the largest. Not differentiable."""
+    logsumexp of `logits / temperature` (2^-120 to 2^120) over the rest of the row. NaN counts as the largest. Not
+    differentiable."""
     _check_logits("top_logits", logits, temperature)
     V = logits.shape[-1]
     if not 1 <= k <= min(V, MAX_K):
@@ -106,10 +107,14 @@ def top_kl(logits: Tensor, indices: Tensor, values: Tensor, tail: Tensor | None 
     """Divergence of every row from its teacher, `[...]` fp32, differentiable in `logits`.
 
     `logits [..., V]` bf16 or fp32: the student's. `indices`, `values [..., k]`: the teacher's logits and their columns
-    (int32 or int64; negative: an unused slot; a column named more than once has the sum of its probabilities; one that is
-    not below `V` is refused like an unused slot and reported as `native.raise_refused` does). `tail [...]`: the teacher's
-    logsumexp of all other logits over the temperature; without it the teacher has its `k` slots alone. Both sides are taken
-    at `temperature`. A row whose teacher has no mass counts zero, with a zero gradient."""
+    (int32 or int64; negative: an unused slot; one that is not below `V` is refused like an unused slot and reported as
+    `native.raise_refused` does). `tail [...]`: the teacher's logsumexp of all other logits over the temperature; without it
+    the teacher has its `k` slots alone. Both sides are taken at `temperature` (2^-120 to 2^120). A row whose teacher has no
+    mass counts zero, with a zero gradient; a NaN that takes part on either side makes the row's loss and gradient NaN.
+
+    The loss is a sum over slots, `p_k (log p_k - log q_k)` each. The slots of a column that is named more than once share its
+    gradient with the sum of their probabilities, but each counts by its own `p_k`: the loss is then below the divergence by
+    what the split of the column costs, a number that does not depend on `logits`."""
     z, indices, values, tail = _arguments("top_kl", logits, indices, values, tail, temperature)
     loss = nv.autograd().top_kl(z, indices, values, tail, temperature, nv.status_ptr(), nv.refused_ptr())
     return loss if logits.dim() == 2 else loss.view(logits.shape[:-1])
