@@ -1202,3 +1202,11 @@ extern "C" int pd_colsum_bf16(const void* x, float* out, float* partial, long lo
   column_total_kernel<<<(C + 31) / 32, 256, 0, static_cast<cudaStream_t>(stream)>>>(partial, out, gy, C, 1.f);
   return PD_CHECK_LAUNCH();
 }
+
+// The word that kernels on the current device report to, 0 from the start. It belongs to the library and not to torch's
+// allocator: asked for while a graph is captured, that would give memory of the graph, and zero it again in every replay.
+__device__ int status_of_kernels;
+extern "C" int* pd_status_word() {
+  void* p = nullptr;
+  return cudaGetSymbolAddress(&p, status_of_kernels) == cudaSuccess ? static_cast<int*>(p) : nullptr;
+}

@@ -126,7 +126,15 @@ def current_stream_ptr() -> int:
 
 @lru_cache(maxsize=8)
 def _status_word(device_index: int) -> torch.Tensor:
-    return torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", device_index))
+    lib().pd_status_word.restype = C.c_void_p
+    at = lib().pd_status_word()
+    if not at:
+        raise NativeError(f"no status word on cuda:{device_index}")
+
+    class Word:
+        __cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (at, False), "strides": None, "version": 3}
+
+    return torch.as_tensor(Word(), device=torch.device("cuda", device_index))
 
 
 def status_word() -> torch.Tensor:

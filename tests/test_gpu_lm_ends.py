@@ -1216,3 +1216,48 @@ def test_hybrid_target_with_the_top_logits_edge_fused_against_eager(nv):
     for k in ("loss/total", "loss/FaithfulnessLoss", "loss/StochasticReconLoss", "loss/ImportanceMinimalityLoss", "kl"):
         a, b = res["eager_torch"][k], res["fused_sm100"][k]
         assert abs(a - b) <= 5e-2 * abs(a) + 1e-6, (k, a, b)
+
+
+def test_a_first_call_that_is_captured(nv):
+    """In a process whose first calls are captured into a graph: results as without, and replays leave alone what other kernels
+    have reported."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from param_decomp_b200.ops import native
+from param_decomp_b200.ops.elementwise import layer_norm
+from param_decomp_b200.ops.embedding import embedding
+from param_decomp_b200.ops.top_logits import top_kl, top_logits
+
+g = torch.Generator(device="cuda").manual_seed(0)
+tokens, table = torch.arange(100, device="cuda"), torch.randn(200, 600, device="cuda", generator=g, requires_grad=True)
+w = torch.ones(600, device="cuda")
+
+def work():
+    logits = layer_norm(embedding(tokens, table), w, None, 1e-5)
+    top = top_logits(logits.detach() * 1.5, 8)
+    loss = top_kl(logits, top.indices, top.values, top.tail)
+    return [loss.detach(), *torch.autograd.grad(loss.sum(), (table,))]
+
+torch.cuda.synchronize()
+stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=stream):
+    out = work()
+graph.replay()
+torch.cuda.synchronize()
+native.check_status()
+assert all(torch.equal(a, b) for a, b in zip(out, work()))
+embedding(tokens + 150, table)  # ids outside the table: reported
+graph.replay()
+torch.cuda.synchronize()
+try:
+    native.check_status()
+    raise SystemExit("the report is lost")
+except native.NativeError as e:
+    assert "token" in str(e)
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parents[1], capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0, done.stdout + done.stderr
