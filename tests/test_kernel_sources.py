@@ -27,3 +27,13 @@ def test_generic_stores_into_bulk_copy_targets_are_fenced():
     body = _kernels(CSRC / "vocab_kl.cu")["vocab_kl_rows_kernel"]
     stores = [m.end() for m in re.finditer(r"ta\[k\] = tb\[k\] = [^;]*;", body)]
     assert stores and all("fence_proxy_async_smem();" in body[at : at + 60] for at in stores)
+
+
+def test_a_clusters_end_is_handed_over_like_its_rows():
+    """top_logits: what a block's selecting warps read of a row is written again two rows on. A block knows that they have read it
+    from the cluster's meeting in every row; behind the last one, before the end marker, the cluster meets once more."""
+    body = _kernels(CSRC / "top_logits.cu")["top_logits_kernel"]
+    rows, end = body.index("for (int r = blockIdx.x / cs"), body.index("sh.work[n & 1].row = -1")
+    behind = body[body.index("r = next;", rows) : end]
+    meeting = re.search(r"wait_pair\(selected, n - 2\).*mbar_arrive_cluster\(mapa_shared\(met, lane\)\).*short_wait<true>\(met, n & 1", behind, re.S)
+    assert meeting, "no meeting between the last row and the end marker"
