@@ -1261,3 +1261,51 @@ except native.NativeError as e:
 """
     done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parents[1], capture_output=True, text=True, timeout=240)
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_offsets_past_32_bits(nv):
+    """More than 2^32 elements of rows, of a table and of logits: rows on both sides of 2^31 and 2^32 as alone."""
+    from param_decomp_b200.ops.elementwise import layer_norm
+    from param_decomp_b200.ops.embedding import embedding
+    from param_decomp_b200.ops.top_logits import top_kl_rows, top_logits
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    rows, d = (1 << 22) + 5, 1040
+    places = lambda n, d: (0, (1 << 31) // d - 3, (1 << 32) // d - 3, n - 7)  # noqa: E731
+    x = torch.randn(rows, d, device="cuda", generator=g, dtype=bf).requires_grad_(True)
+    w, b = torch.randn(d, device="cuda", generator=g), torch.randn(d, device="cuda", generator=g)
+    y = layer_norm(x, w, b, 1e-5)
+    (dx,) = torch.autograd.grad(y, (x,), x.detach())
+    for s in places(rows, d):
+        part = x.detach()[s:s + 7].clone().requires_grad_(True)
+        alone = layer_norm(part, w, b, 1e-5)
+        assert torch.equal(alone, y[s:s + 7]) and torch.equal(torch.autograd.grad(alone, (part,), part.detach())[0], dx[s:s + 7])
+    del x, y, dx, part, alone
+    V, d, n = (1 << 22) + 3, 1032, (1 << 22) + 9
+    table = torch.randn(V, d, device="cuda", generator=g, dtype=bf).requires_grad_(True)
+    tokens = torch.randint(0, V, (n,), device="cuda", generator=g)
+    tokens[-100:], tokens[1000:1100] = V - 1, V - 2
+    y = embedding(tokens, table)
+    for s in places(n, d):
+        assert torch.equal(y.detach()[s:s + 7], table.detach()[tokens[s:s + 7]])
+    dy = torch.randint(-1, 2, (1, d), device="cuda", generator=g).to(bf)  # a row's gradient is its count times this, exactly
+    (grad,) = torch.autograd.grad(y, (table,), dy.expand(n, d))
+    counts = torch.bincount(tokens, minlength=V)
+    for s in range(0, V, 1 << 18):
+        assert torch.equal(grad[s:s + (1 << 18)].float(), counts[s:s + (1 << 18), None].float() * dy.float())
+    del table, y, grad
+    n, V = 90001, 50277
+    z = torch.randn(n, V, device="cuda", generator=g, dtype=bf)
+    top = top_logits(z, 64)
+    loss, dz = top_kl_rows(z, top.indices, top.values * 0.5, top.tail)
+    for s in places(n, V):
+        s = s // 8 * 8  # rows at the same addresses modulo 16 bytes
+        part = [t[s:s + 7] for t in (z, *top)]
+        assert all(torch.equal(a, b) for a, b in zip(part[1:], top_logits(part[0], 64)))
+        alone = top_kl_rows(part[0], part[2], part[1] * 0.5, part[3])
+        assert torch.equal(alone[0], loss[s:s + 7]) and torch.equal(alone[1], dz[s:s + 7])
+    far = z.view(-1).as_strided((3, 2000), (2_100_000_000, 1))  # by the pitch alone
+    assert all(torch.equal(a, b) for a, b in zip(top_logits(far, 10), top_logits(far.contiguous(), 10)))
+    _done(nv)
+    del z, dz, far
+    torch.cuda.empty_cache()
