@@ -14,7 +14,7 @@
 // could guess, so the block that finds a token asks for its row in L2 at once, long before it is summed. The rows without a
 // token, most of the bytes, are written by blocks of the second kernel too: zeros at the full rate in the first one made the
 // loads of its sums wait for several microseconds each (32,768 tokens in 50,277 rows of 768: 77 us).
-// Measured there, bf16: lookup 15.6 us (6.4 TB/s, copy bandwidth), first kernel 34, second 25: 75 us with the launches. 6151
+// Measured there, bf16: lookup 15.6 us (6.4 TB/s by a row a token, most of them from L2), first kernel 34, second 25: 78 us with the launches. 6151
 // tokens in 151,936 rows of 515 fp32: 11, 26 and 57. The first kernel is a chain of steps, each with its own latency, over
 // all tokens in every block; what the second has to write takes 12 and 48 us of it.
 #include <algorithm>
